@@ -284,6 +284,94 @@ NKB_API int nkb_comm_all_to_all(nkb_comm comm, const void *send, void *recv, siz
 NKB_API int nkb_linear_attention_noalloc(const void *q, const void *k, const void *v, void *out, int64_t B, int64_t H,
                                          int64_t T, int64_t D, void *stream);
 
+/* ---- serving over a paged KV cache ------------------------------------------
+ * Keys and values live in pages: a cache is (pages, page_size, kv_heads,
+ * head_dim) with any strides whose head dimension is contiguous, and
+ * page_table[b][i] names the page that holds positions i * page_size ..
+ * (i + 1) * page_size - 1 of sequence b.  The new tokens of a call lie in
+ * sequence order: sequence b owns tokens q_start[b] .. q_start[b + 1] - 1
+ * (q_start NULL: one token per sequence), and kv_len[b] counts its cached
+ * tokens with the new ones, so its i-th new token of n has position
+ * kv_len[b] - n + i.  page_table, kv_len and q_start are int32 device arrays,
+ * read when the kernels run, so a captured call serves every step of a loop.
+ * Strides are in elements.  Tokens that no sequence owns are left out: their
+ * output rows are zero.  The reference keeps one dense cache, one length and
+ * one position per batch (examples/models/qwen3/kernels/attention.py:95-117);
+ * these calls are its paged, ragged form and have no counterpart there. */
+
+/* k and v rows (tokens, kv_heads, head_dim) go to their sequence's pages; the
+ * first rot_dim dimensions of k, and of q where given, are rotated on the way
+ * as rope does (first half x second half; examples/models/qwen3/kernels/
+ * rope.py:24-45) by the rows of cos / sin (rope_rows, rot_dim / 2) at the
+ * token's position + pos_offset (clamped into the table), in fp32, rounded
+ * once.  A position outside the page table, or a page id outside the cache,
+ * drops that row's store.  q / q_out may be NULL (no queries) and equal (in
+ * place); rot_dim 0 appends without rotating (cos, sin NULL). */
+typedef struct nkb_paged_append_args {
+  const void *k, *v, *q;
+  void *q_out, *k_cache, *v_cache;
+  const int32_t *page_table, *kv_len, *q_start;
+  const void *cos, *sin;
+  int64_t dtype, cache_dtype, rope_dtype; /* NKB_F32, NKB_BF16 or NKB_F16 */
+  int64_t tokens, seqs, q_heads, kv_heads, head_dim, rot_dim;
+  int64_t rope_rows, rope_stride, pos_offset;
+  int64_t k_token, k_head, v_token, v_head, q_token, q_head, q_out_token, q_out_head;
+  int64_t pages, page_size, k_page, k_slot, k_cache_head, v_page, v_slot, v_cache_head;
+  int64_t table_width, table_stride;
+} nkb_paged_append_args;
+NKB_API int nkb_paged_append(const nkb_paged_append_args *args, void *stream);
+
+/* out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j over the cached keys j
+ * that token t of position p sees: j <= p, and where window > 0 also
+ * (j > p - window or j < sinks): a sliding window that keeps the first `sinks`
+ * tokens visible.  Query head h reads kv head h / (q_heads / kv_heads).  A
+ * token that sees no key has a zero row.  prefix_len > 0: every sequence is
+ * preceded by the same prefix_len tokens, held by prefix_pages (int32, one id
+ * per page) and read once for the batch; page_table and kv_len then describe
+ * what follows the prefix, all of the prefix is visible, and window must be 0.
+ * Page ids outside the cache read as zero keys and values.  q, out and the
+ * caches have one dtype; statistics and sums are fp32.  workspace: a device
+ * array of nkb_paged_attention_workspace() bytes for this call alone (its
+ * contents need not be kept or cleared). */
+typedef struct nkb_paged_attention_args {
+  const void *q;
+  void *out;
+  const void *k_cache, *v_cache;
+  const int32_t *page_table, *kv_len, *q_start, *prefix_pages;
+  void *workspace;
+  int64_t dtype, tokens, seqs, q_heads, kv_heads, head_dim;
+  int64_t q_token, q_head, out_token, out_head;
+  int64_t pages, page_size, k_page, k_slot, k_cache_head, v_page, v_slot, v_cache_head;
+  int64_t table_width, table_stride;
+  int64_t window, sinks, prefix_len, workspace_bytes;
+  double scale;
+} nkb_paged_attention_args;
+NKB_API int nkb_paged_attention(const nkb_paged_attention_args *args, void *stream);
+NKB_API int nkb_paged_attention_workspace(const nkb_paged_attention_args *args, size_t *bytes);
+
+/* One token per row of logits (rows, vocab), row stride in elements, drawn with
+ * the row's u in [0, 1).  Weights are e = exp((x - max) / temperature) in fp32,
+ * held as whole multiples of 2^-32, so every sum is exact and the result does
+ * not depend on an order of additions.  Kept: the top_k largest (0 or >= vocab:
+ * all), of them the shortest run in descending order whose weights reach
+ * top_p of their sum (>= 1: all), of those the ones with e >= min_p; equal
+ * logits rank by index.  The token is the first in index order whose running
+ * sum of kept weights exceeds u times their sum.  temperature <= 0: the
+ * largest logit, lowest index first.  NaN logits count as -inf; a row without
+ * a logit above -inf gives -1.  temperature (fp32), top_k (int32), top_p and
+ * min_p (fp32) are per-row device arrays, each NULL for 1, 0, 1, 0; tokens is
+ * int32.  vocab <= 2^21.  The reference samples greedily
+ * (examples/models/qwen3/kernels/sampling.py:113-147). */
+typedef struct nkb_sample_args {
+  const void *logits;
+  const float *u, *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  int32_t *tokens;
+  int64_t dtype, rows, vocab, row_stride;
+} nkb_sample_args;
+NKB_API int nkb_sample_tokens(const nkb_sample_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,135 @@
+// Attention of new tokens over a paged cache, with a sliding window and first
+// tokens that stay visible, or over a prefix that the batch shares:
+//   out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j
+// over the keys j that the token at position p sees (j <= p, and with a window
+// w also j > p - w or j < sinks; all of the prefix).
+#include "paged.cuh"
+
+namespace nkb {
+namespace pattn {
+
+using Args = nkb_paged_attention_args;
+
+constexpr int WARPS = 4, MAX_D = 256;
+
+// Any type, layout, page size and head dimension up to 256: one block per
+// (token, query head), its four warps taking every fourth key; lane l holds
+// dimensions l, l + 32, ... of the query, the running output and each row, so
+// a score is a warp sum.  Running maximum and sum per warp (fp32), joined at
+// the end.
+template <class T>
+__global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const __grid_constant__ Args a) {
+  constexpr int PER = MAX_D / 32;
+  __shared__ int slot;
+  __shared__ float s_m[WARPS], s_l[WARPS], s_o[WARPS][MAX_D];
+  const int t = blockIdx.x, h = blockIdx.y, hk = h / (int)(a.q_heads / a.kv_heads);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, D = (int)a.head_dim;
+  const int b = paged::block_find_seq(a.q_start, (int)a.seqs, t, &slot);
+  const T *kc = static_cast<const T *>(a.k_cache) + hk * a.k_cache_head;
+  const T *vc = static_cast<const T *>(a.v_cache) + hk * a.v_cache_head;
+  float q[PER], o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = lane + 32 * i;
+    q[i] = d < D ? paged::to_f32(static_cast<const T *>(a.q)[t * a.q_token + h * a.q_head + d]) * (float)a.scale : 0.f;
+    o[i] = 0.f;
+  }
+  auto visit = [&](const int32_t *pages, int64_t j) {  // key j of a page list
+    const int page = pages[j / a.page_size];
+    const int64_t s = j % a.page_size;
+    const bool ok = paged::page_ok(page, a.pages);
+    const T *kr = kc + (ok ? page * a.k_page + s * a.k_slot : 0), *vr = vc + (ok ? page * a.v_page + s * a.v_slot : 0);
+    float x = 0.f, v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int d = lane + 32 * i;
+      const bool in = ok && d < D;
+      x += q[i] * (in ? paged::to_f32(kr[d]) : 0.f);
+      v[i] = in ? paged::to_f32(vr[d]) : 0.f;
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+    const float mn = fmaxf(m, x), f = m == -INFINITY ? 0.f : __expf(m - mn), p = mn == -INFINITY ? 0.f : __expf(x - mn);
+    m = mn;
+    l = l * f + p;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = o[i] * f + p * v[i];
+  };
+  if (b >= 0) {
+    for (int64_t j = warp; j < a.prefix_len; j += WARPS) visit(a.prefix_pages, j);
+    const int first = a.q_start ? a.q_start[b] : t, n = a.q_start ? a.q_start[b + 1] - first : 1;
+    const int64_t pos = (int64_t)a.kv_len[b] - n + (t - first), end = min(pos + 1, a.table_width * a.page_size);
+    const int64_t low = a.window > 0 ? max((int64_t)0, pos - a.window + 1) : 0;
+    const int32_t *pages = a.page_table + b * a.table_stride;
+    const int64_t head = min(min(a.sinks, low), end);
+    for (int64_t j = warp; j < head; j += WARPS) visit(pages, j);
+    for (int64_t j = low + warp; j < end; j += WARPS) visit(pages, j);
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (lane + 32 * i < D) s_o[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  float M = -INFINITY, L = 0.f;
+  for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w]);
+  for (int w = 0; w < WARPS; ++w) L += s_m[w] == -INFINITY ? 0.f : s_l[w] * __expf(s_m[w] - M);
+  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
+    float x = 0.f;
+    for (int w = 0; w < WARPS; ++w) x += s_m[w] == -INFINITY ? 0.f : s_o[w][d] * __expf(s_m[w] - M);
+    static_cast<T *>(a.out)[t * a.out_token + h * a.out_head + d] = paged::from_f32<T>(L > 0.f ? x / L : 0.f);
+  }
+}
+
+int check_args(const Args &a) {
+  auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("paged_attention: ") + m); };
+  if (int s = paged::check_cache("paged_attention", a.tokens, a.seqs, a.kv_heads, a.head_dim, a.pages, a.page_size,
+                                 a.table_width, a.table_stride))
+    return s;
+  if (!paged::float_dtype(a.dtype))
+    return fail(NKB_ERR_UNSUPPORTED, "paged_attention: q, out and caches must be float32, bfloat16 or float16");
+  if (a.q_heads < 1 || a.q_heads % a.kv_heads || a.q_heads > 65535) return bad("q_heads must be a multiple of kv_heads");
+  if (a.head_dim > MAX_D) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: head_dim above 256");
+  if (a.window < 0 || a.sinks < 0 || a.prefix_len < 0 || a.prefix_len > INT32_MAX) return bad("window, sinks and prefix_len must not be negative");
+  if (a.prefix_len && a.window) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: a window over a shared prefix");
+  if (a.prefix_len && !a.prefix_pages) return bad("a prefix needs its pages");
+  if (a.tokens && (!a.q || !a.out || !a.kv_len || (a.table_width && !a.page_table) || (a.pages && (!a.k_cache || !a.v_cache))))
+    return bad("NULL array");
+  if (!a.q_start && a.tokens != a.seqs) return bad("without q_start there is one token per sequence");
+  return NKB_OK;
+}
+
+int workspace(const Args &a, size_t *bytes) {
+  if (int s = check_args(a)) return s;
+  *bytes = 0;
+  return NKB_OK;
+}
+
+int run(const Args &a, cudaStream_t st) {
+  size_t need = 0;
+  if (int s = workspace(a, &need)) return s;
+  if (a.workspace_bytes < (int64_t)need || (need && !a.workspace))
+    return fail(NKB_ERR_INVALID, "paged_attention: workspace of " + std::to_string(a.workspace_bytes) + " bytes, " +
+                                     std::to_string(need) + " needed");
+  if (a.tokens == 0) return NKB_OK;
+  paged::with_dtype(a.dtype, [&](auto t) {
+    attn_any_kernel<decltype(t)><<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), WARPS * 32, 0, st>>>(a);
+    return 0;
+  });
+  return launch_status("paged_attention");
+}
+
+}  // namespace pattn
+}  // namespace nkb
+
+extern "C" int nkb_paged_attention_workspace(const nkb_paged_attention_args *args, size_t *bytes) {
+  if (!args || !bytes) return nkb::fail(NKB_ERR_INVALID, "NULL argument");
+  return nkb::pattn::workspace(*args, bytes);
+}
+
+extern "C" int nkb_paged_attention(const nkb_paged_attention_args *args, void *stream) {
+  if (!args) return nkb::fail(NKB_ERR_INVALID, "args is NULL");
+  return nkb::pattn::run(*args, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,226 @@
+"""Serving over a paged KV cache: direct calls on device memory (torch tensors).
+
+The calls of one decode step or one chunk of prompts: ``paged_append`` rotates
+the new tokens' keys (and queries) and stores keys and values in their pages,
+``paged_attention`` attends to them (all of them, or a sliding window with a
+few first tokens), ``prefix_attention`` does so over a prefix that the whole
+batch shares, and ``sample_tokens`` draws the next tokens.  Kernel bodies reach
+the same kernels through ``nkipy_b200.core.tensor_apis``.
+
+Conventions (``include/nkb.h``): a cache is (pages, page_size, kv_heads,
+head_dim) with a contiguous last axis and any other strides; ``page_table``
+(sequences, width), ``kv_len`` (sequences,) and ``q_start`` (sequences + 1,)
+are int32; the new tokens lie in sequence order; ``kv_len`` counts a
+sequence's cached tokens with the new ones; ``q_start=None`` means one new
+token per sequence.  Lengths and tables are read on the device when the
+kernels run, nothing is synchronised, and every launch goes to the current
+torch stream, so a call can be captured into a CUDA graph.
+"""
+
+import ctypes
+import math
+import struct
+
+from nkipy_b200.spike import _nkb, get_spike_singleton
+
+try:
+    import torch
+
+    _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+except ImportError:  # pragma: no cover
+    torch = None
+
+# nkb_paged_append_args, nkb_paged_attention_args, nkb_sample_args: 8-byte fields only
+_APPEND = struct.Struct("=11Q3q6q3q8q8q2q")
+_ATTENTION = struct.Struct("=9Q6q4q8q2q4qd")
+_SAMPLE = struct.Struct("=7Q4q")
+
+
+def _fail(message):
+    raise ValueError(message)
+
+
+def _on_device(*tensors):
+    """The device index of all given tensors (None entries skipped): the runtime's device."""
+    device = get_spike_singleton().device
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _fail(f"expected tensors on cuda:{device} (this process's device), got one on {t.device}")
+    return device
+
+
+def _float(t, name, ndim):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != ndim:
+        _fail(f"{name}: expected {ndim} axes, got shape {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.size(-1) > 1:
+        _fail(f"{name}: the last axis must be contiguous")
+    return code
+
+
+def _int32(t, name, shape):
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name}: expected int32, got {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and t.size(i) != n for i, n in enumerate(shape)):
+        _fail(f"{name}: expected shape {tuple('any' if n is None else n for n in shape)}, got {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.size(-1) > 1:
+        _fail(f"{name}: the last axis must be contiguous")
+
+
+def _batch(page_table, kv_len, q_start, tokens):
+    """Checks a call's page table and lengths; the number of sequences."""
+    _int32(page_table, "page_table", (None, None))
+    seqs = page_table.size(0)
+    _int32(kv_len, "kv_len", (seqs,))
+    if q_start is not None:
+        _int32(q_start, "q_start", (seqs + 1,))
+    elif tokens != seqs:
+        _fail(f"without q_start there is one token per sequence: {tokens} tokens, {seqs} sequences")
+    return seqs
+
+
+def _caches(k_cache, v_cache):
+    code = _float(k_cache, "k_cache", 4)
+    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+        _fail(f"k_cache and v_cache differ: {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
+    _float(v_cache, "v_cache", 4)
+    return code
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _launch(fn, packed, device):
+    """Issues a call on the current stream of ``device``."""
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return _launch(fn, packed, device)
+    _nkb.check(fn(packed, torch.cuda.current_stream(device).cuda_stream))
+
+
+def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=None, cos=None, sin=None, pos_offset=0,
+                 q_out=None):
+    """Store the new tokens' ``k`` and ``v`` (tokens, kv_heads, head_dim) in their
+    sequences' pages, in place.  With ``cos`` / ``sin`` (positions, rot_dim / 2) the
+    first rot_dim dimensions of ``k``, and of ``q`` (tokens, q_heads, head_dim) when
+    given, are rotated (half split) by the token's position + ``pos_offset`` on the
+    way, in fp32.  Returns the rotated queries (``q_out``; may be ``q`` itself), or
+    None without ``q``.  A row whose page is not in the cache, or whose position is
+    outside the table, is not stored."""
+    device = _on_device(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, sin, q_out)
+    code = _float(k, "k", 3)
+    tokens, hkv, d = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype:
+        _fail(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    _float(v, "v", 3)
+    cache_code = _caches(k_cache, v_cache)
+    pages, page_size = k_cache.size(0), k_cache.size(1)
+    if k_cache.size(2) != hkv or k_cache.size(3) != d:
+        _fail(f"caches hold {k_cache.size(2)} heads of {k_cache.size(3)}, k has {hkv} of {d}")
+    seqs = _batch(page_table, kv_len, q_start, tokens)
+    rot = rows = stride = rope_code = 0
+    if (cos is None) != (sin is None):
+        _fail("cos and sin go together")
+    if cos is not None:
+        rope_code = _float(cos, "cos", 2)
+        if sin.shape != cos.shape or sin.dtype != cos.dtype or sin.stride() != cos.stride():
+            _fail("cos and sin differ in shape, type or strides")
+        rows, rot, stride = cos.size(0), 2 * cos.size(1), cos.stride(0)
+        if rot > d:
+            _fail(f"cos and sin rotate {rot} dimensions, head_dim is {d}")
+    hq = q_token = q_head = qo_token = qo_head = 0
+    if q is not None:
+        if _float(q, "q", 3) != code or q.size(0) != tokens or q.size(2) != d:
+            _fail(f"q {tuple(q.shape)} {q.dtype} does not go with k {tuple(k.shape)} {k.dtype}")
+        hq, q_token, q_head = q.size(1), q.stride(0), q.stride(1)
+        if q_out is None:
+            q_out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+        elif _float(q_out, "q_out", 3) != code or q_out.shape != q.shape:
+            _fail(f"q_out {tuple(q_out.shape)} {q_out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
+        qo_token, qo_head = q_out.stride(0), q_out.stride(1)
+    elif q_out is not None:
+        _fail("q_out without q")
+    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    packed = _APPEND.pack(
+        k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+        kv_len.data_ptr(), _ptr(q_start), _ptr(cos), _ptr(sin), code, cache_code, rope_code, tokens, seqs, hq, hkv, d, rot,
+        rows, stride, pos_offset, ks[0], ks[1], vs[0], vs[1], q_token, q_head, qo_token, qo_head, pages, page_size, kc[0],
+        kc[1], kc[2], vc[0], vc[1], vc[2], page_table.size(1), page_table.stride(0))
+    _launch(_nkb.lib().nkb_paged_append, packed, device)
+    return q_out
+
+
+def _attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, out, prefix_pages, prefix_len):
+    device = _on_device(q, k_cache, v_cache, page_table, kv_len, q_start, out, prefix_pages)
+    code = _float(q, "q", 3)
+    tokens, hq, d = q.shape
+    if _caches(k_cache, v_cache) != code:
+        raise TypeError(f"q is {q.dtype}, the caches are {k_cache.dtype}")
+    pages, page_size, hkv = k_cache.size(0), k_cache.size(1), k_cache.size(2)
+    if k_cache.size(3) != d or hkv == 0 or hq % hkv:
+        _fail(f"q {tuple(q.shape)} does not go with caches of {hkv} heads of {k_cache.size(3)}")
+    seqs = _batch(page_table, kv_len, q_start, tokens)
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+    elif _float(out, "out", 3) != code or out.shape != q.shape:
+        _fail(f"out {tuple(out.shape)} {out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
+    qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
+    head = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+            kv_len.data_ptr(), _ptr(q_start), _ptr(prefix_pages))
+    sizes = (code, tokens, seqs, hq, hkv, d, qs[0], qs[1], os_[0], os_[1], pages, page_size, kc[0], kc[1], kc[2], vc[0],
+             vc[1], vc[2], page_table.size(1), page_table.stride(0), window, sinks, prefix_len)
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    need, lib = ctypes.c_size_t(), _nkb.lib()
+    _nkb.check(lib.nkb_paged_attention_workspace(_ATTENTION.pack(*head, 0, *sizes, 0, scale), need))
+    room = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    _launch(lib.nkb_paged_attention, _ATTENTION.pack(*head, _ptr(room), *sizes, need.value, scale), device)
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, kv_len, q_start=None, window=0, sinks=0, scale=None, out=None):
+    """Attention of the new tokens' ``q`` (tokens, q_heads, head_dim) over their
+    sequences' cached keys up to their own position; with ``window`` > 0 only the last
+    ``window`` of them (the token itself among them) and the first ``sinks``.  ``scale``
+    defaults to 1 / sqrt(head_dim).  Returns ``out`` (tokens, q_heads, head_dim); a token
+    that sees no key gives zeros."""
+    return _attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, out, None, 0)
+
+
+def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, kv_len, q_start=None, scale=None,
+                     out=None):
+    """Attention of a batch whose sequences all begin with the same ``prefix_len``
+    tokens, held once in ``prefix_pages`` (int32 page ids) and read once for the batch;
+    ``page_table`` and ``kv_len`` describe what each sequence has after the prefix."""
+    if prefix_len < 0:
+        _fail("prefix_len must not be negative")
+    _int32(prefix_pages, "prefix_pages", (None,))
+    if prefix_len > prefix_pages.size(0) * k_cache.size(1):
+        _fail(f"prefix of {prefix_len} tokens needs more than {prefix_pages.size(0)} pages of {k_cache.size(1)}")
+    return _attention(q, k_cache, v_cache, page_table, kv_len, q_start, 0, 0, scale, out, prefix_pages, prefix_len)
+
+
+def sample_tokens(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """One token (int32) per row of ``logits`` (rows, vocab), drawn with the row's
+    ``u`` (fp32, in [0, 1)).  ``temperature``, ``top_p``, ``min_p`` (fp32) and ``top_k``
+    (int32) are one value per row, or None for 1, 1, 0 and 0 (off).  Filters apply in
+    the order temperature, top-k, top-p, min-p; a temperature of 0 takes the largest
+    logit.  A row without a finite logit or +inf gives -1."""
+    device = _on_device(logits, u, temperature, top_k, top_p, min_p, out)
+    code = _float(logits, "logits", 2)
+    rows, vocab = logits.shape
+    for t, name in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
+        if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != rows or not t.is_contiguous()):
+            _fail(f"{name}: expected a contiguous float32 tensor of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
+    if top_k is not None:
+        _int32(top_k, "top_k", (rows,))
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    else:
+        _int32(out, "out", (rows,))
+    packed = _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                          out.data_ptr(), code, rows, vocab, logits.stride(0))
+    _launch(_nkb.lib().nkb_sample_tokens, packed, device)
+    return out

@@ -113,6 +113,11 @@ def _declare(lib):
         "nkb_comm_reduce_scatter": [c_comm, vp, vp, sz, i32, vp],
         "nkb_comm_all_to_all": [c_comm, vp, vp, sz, i32, vp],
         "nkb_linear_attention_noalloc": [vp, vp, vp, vp, i64, i64, i64, i64, vp],
+        # argument structs, packed by the caller (runtime/serving.py)
+        "nkb_paged_append": [ctypes.c_char_p, vp],
+        "nkb_paged_attention": [ctypes.c_char_p, vp],
+        "nkb_paged_attention_workspace": [ctypes.c_char_p, ctypes.POINTER(sz)],
+        "nkb_sample_tokens": [ctypes.c_char_p, vp],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
