@@ -3,12 +3,10 @@
 //   out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j
 // over the keys j that the token at position p sees (j <= p, and with a window
 // w also j > p - w or j < sinks; all of the prefix).
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace nkb {
 namespace pattn {
-
-using Args = nkb_paged_attention_args;
 
 constexpr int WARPS = 4, MAX_D = 256;
 
@@ -101,19 +99,28 @@ int check_args(const Args &a) {
   return NKB_OK;
 }
 
-int workspace(const Args &a, size_t *bytes) {
+// One new token per sequence of a 16-bit type, rows of whole 16-byte pieces,
+// up to 128 dimensions: the split decode kernel.
+bool decode_form(const Args &a) {
+  return !a.q_start && !a.prefix_len && a.dtype != NKB_F32 && a.head_dim <= 128 && aligned16(a) &&
+         a.seqs * a.q_heads <= INT32_MAX;
+}
+
+int workspace(const Args &a, int device, size_t *bytes) {
   if (int s = check_args(a)) return s;
-  *bytes = 0;
+  *bytes = a.tokens && decode_form(a) ? decode_workspace(a, device) : 0;
   return NKB_OK;
 }
 
-int run(const Args &a, cudaStream_t st) {
+int run(const Args &a, int device, cudaStream_t st) {
   size_t need = 0;
-  if (int s = workspace(a, &need)) return s;
+  if (int s = workspace(a, device, &need)) return s;
   if (a.workspace_bytes < (int64_t)need || (need && !a.workspace))
     return fail(NKB_ERR_INVALID, "paged_attention: workspace of " + std::to_string(a.workspace_bytes) + " bytes, " +
                                      std::to_string(need) + " needed");
+  if (reinterpret_cast<uintptr_t>(a.workspace) & 15) return fail(NKB_ERR_INVALID, "paged_attention: unaligned workspace");
   if (a.tokens == 0) return NKB_OK;
+  if (decode_form(a)) return decode_run(a, st, device);
   paged::with_dtype(a.dtype, [&](auto t) {
     attn_any_kernel<decltype(t)><<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), WARPS * 32, 0, st>>>(a);
     return 0;
@@ -126,10 +133,14 @@ int run(const Args &a, cudaStream_t st) {
 
 extern "C" int nkb_paged_attention_workspace(const nkb_paged_attention_args *args, size_t *bytes) {
   if (!args || !bytes) return nkb::fail(NKB_ERR_INVALID, "NULL argument");
-  return nkb::pattn::workspace(*args, bytes);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return nkb::pattn::workspace(*args, dev, bytes);
 }
 
 extern "C" int nkb_paged_attention(const nkb_paged_attention_args *args, void *stream) {
   if (!args) return nkb::fail(NKB_ERR_INVALID, "args is NULL");
-  return nkb::pattn::run(*args, static_cast<cudaStream_t>(stream));
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return nkb::pattn::run(*args, dev, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,458 @@
+// Paged attention of one new token per sequence (bf16, fp16):
+//   out[b, h] = sum_j softmax_j(q[b, h] . k_j * scale) v_j
+// over the keys that the token sees, read once from their pages.
+//
+// The bound is HBM (4 G flop per 2-byte element of K and V for G query heads
+// per key head), so the keys of all sequences are cut into equal shares: the
+// sequences' key blocks, in (sequence, key head) order, form one run that the
+// resident CTAs split evenly whatever the lengths.  A CTA therefore holds the
+// end of one (sequence, key head), some whole ones, and the beginning of
+// another; what it holds whole it writes out, the rest goes to a workspace as
+// (max, sum, unnormalised output) for a second kernel to join.  Lengths are
+// read on the device: the grid depends on none of them.
+//
+// In a CTA the (up to 16) query heads of the key head are the rows of one m16
+// tile; each of four warps takes every fourth group of WN keys through its own
+// ring of stages filled by cp.async, scores and products on mma.sync m16n8k16
+// with fp32 accumulation, the running maximum and sum of the softmax in fp32.
+#include "mma_sync.cuh"
+#include "paged_attn.cuh"
+
+namespace nkb {
+namespace pattn {
+namespace {
+
+using mma::cp_async16;
+using mma::cp_commit;
+using mma::cp_wait;
+using mma::ldsm_x4;
+using mma::ldsm_x4_t;
+using mma::smem_addr;
+
+constexpr int THREADS = 128, WARPS = 4, ROWS = 16;
+
+template <int DP>
+struct Shape {
+  static constexpr int WN = DP == 128 ? 16 : 32;       // keys per warp and stage
+  static constexpr int BK = WARPS * WN;                // keys per block
+  static constexpr int TILE = WN * DP * 2;             // bytes of K (or V) per stage
+  static constexpr int STAGES = 3;
+  static constexpr int RING = STAGES * 2 * TILE;       // per warp
+  static constexpr int OPAD = DP + 4;                  // row stride of the join buffer (floats)
+  static constexpr int JOIN = WARPS * ROWS * (OPAD + 2) * 4;
+  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
+  static constexpr int SMEM = ROWS * DP * 2 + BODY;
+  static constexpr int SLOT = ROWS * (DP + 2);         // floats of one partial: outputs, then max and sum
+};
+
+struct Params {
+  Args a;
+  int groups;  // 16-row groups of query heads per key head
+  float scale_log2;
+  float *ws;
+  int ctas;
+  bool keep;  // write every result as a partial (a prefix is joined to it)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) { return mma::pack2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+template <class T>
+__device__ __forceinline__ void mma_tile(float *c, const uint32_t *a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_tile<__nv_bfloat16>(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  mma::mma16816(c, a, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma_tile<__half>(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ Visible visible_of(const Args &a, int b) {
+  return visible((int64_t)a.kv_len[b] - 1, a.table_width * a.page_size, a.window, a.sinks);
+}
+// key blocks of sequence b (one at least: a sequence without keys has a row of zeros to write)
+template <int BK>
+__device__ __forceinline__ int blocks_of(const Args &a, int b) {
+  return max(1, (visible_of(a, b).n + BK - 1) / BK);
+}
+
+// Sum of blocks_of over all sequences, and the first sequence whose blocks
+// before and in it reach past `f` units of `per` (its own included): found by
+// all threads of the block together.
+struct Found {
+  int64_t total;   // blocks of all sequences
+  int seq;         // the sequence
+  int64_t before;  // blocks of the sequences before it
+};
+template <int BK, class Want>
+__device__ __forceinline__ Found find(const Args &a, Want want) {
+  __shared__ int64_t s_warp[WARPS], s_before;
+  __shared__ int s_seq;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = (int)a.seqs;
+  Found r;
+  r.total = 0;
+  for (int base = 0; base < B; base += THREADS) {  // the sum
+    const int b = base + threadIdx.x;
+    int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) n += __shfl_xor_sync(0xffffffffu, n, w);
+    __syncthreads();
+    if (lane == 0) s_warp[warp] = n;
+    __syncthreads();
+    r.total += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+  }
+  int64_t done = 0;
+  for (int base = 0; base < B; base += THREADS) {  // the sequence
+    const int b = base + threadIdx.x;
+    const int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
+    int64_t p = n;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, p, w);
+      if (lane >= w) p += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = p;
+    __syncthreads();
+    int64_t first = done + p - n;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) first += s_warp[w];
+      done += s_warp[w];
+    }
+    if (b < B && want(r.total, b, first, n)) {
+      s_seq = b;
+      s_before = first;
+    }
+  }
+  __syncthreads();
+  r.seq = s_seq;
+  r.before = s_before;
+  return r;
+}
+
+// CTAs that share the blocks: none of them is left without one
+__device__ __forceinline__ int workers(int64_t total, int ctas) { return (int)min(total, (int64_t)ctas); }
+// first block of CTA c's share
+__device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) { return total * c / ctas; }
+// CTA whose share holds block f
+__device__ __forceinline__ int owner(int64_t total, int64_t f, int ctas) {
+  int c = (int)(f * ctas / total);
+  while (share(total, c + 1, ctas) <= f) ++c;
+  while (share(total, c, ctas) > f) --c;
+  return c;
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constant__ Params p) {
+  using S = Shape<DP>;
+  constexpr int WN = S::WN, NT = WN / 8, CH = DP / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *sQ = smem, *body = smem + ROWS * DP * 2;
+  const Args &a = p.a;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x;
+  const int heads = (int)a.kv_heads * p.groups;  // units per sequence
+  const int G = (int)(a.q_heads / a.kv_heads), D = (int)a.head_dim;
+  uint8_t *ring = body + warp * S::RING;
+
+  const Found at = find<S::BK>(a, [&](int64_t blocks, int, int64_t first, int64_t n) {
+    const int ctas = workers(blocks * heads, p.ctas);
+    const int64_t f = share(blocks * heads, min(c, ctas - 1), ctas);
+    return first * heads <= f && f < (first + n) * heads;
+  });
+  pdl_trigger();
+  const int64_t total = at.total * heads;
+  const int ctas = workers(total, p.ctas);
+  if (c >= ctas) return;
+  const int64_t f0 = share(total, c, ctas), f1 = share(total, c + 1, ctas);
+  int64_t f = f0, before = at.before * heads;  // `before`: blocks before sequence b
+  int b = at.seq;
+  while (f < f1) {
+    const Visible vis = visible_of(a, b);
+    const int nb = max(1, (vis.n + S::BK - 1) / S::BK);
+    const int unit = (int)((f - before) / nb), k0 = (int)((f - before) % nb);
+    const int k1 = (int)min((int64_t)nb, k0 + (f1 - f));
+    const int hk = unit / p.groups, h0 = hk * G + (unit % p.groups) * ROWS, rows = min(ROWS, (hk + 1) * G - h0);
+    const T *kc = static_cast<const T *>(a.k_cache) + hk * a.k_cache_head;
+    const T *vc = static_cast<const T *>(a.v_cache) + hk * a.v_cache_head;
+    const int32_t *table = a.page_table + b * a.table_stride;
+
+    __syncthreads();  // the join buffer and Q of the segment before are read
+    for (int i = threadIdx.x; i < ROWS * CH; i += THREADS) {
+      const int r = i / CH, ch = i % CH;
+      const bool ok = r < rows && ch * 8 < D;
+      cp_async16(smem_addr(sQ) + mma::swz(r, ch, DP * 2),
+                 static_cast<const T *>(a.q) + b * a.q_token + (ok ? (h0 + r) * a.q_head + ch * 8 : 0), ok);
+    }
+    cp_commit();
+
+    // page id (-1: none) and slot of this lane's key of block kb
+    auto locate = [&](int kb, int &page, int &slot) {
+      const int v = kb * S::BK + warp * WN + lane;
+      page = -1;
+      slot = 0;
+      if (lane < WN && kb < k1 && v < vis.n) {
+        const int key = vis.key(v), i = key / (int)a.page_size;
+        slot = key - i * (int)a.page_size;
+        page = table[i];
+        if (!paged::page_ok(page, a.pages)) page = -1;
+      }
+    };
+    auto load = [&](int stage, int page, int slot) {  // rows without a page are zeros
+      const uint32_t kd = smem_addr(ring + stage * 2 * S::TILE), vd = kd + S::TILE;
+#pragma unroll
+      for (int j = 0; j < WN * CH / 32; ++j) {
+        const int idx = j * 32 + lane, r = idx / CH, ch = idx % CH;
+        const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
+        const bool ok = pg >= 0 && ch * 8 < D;
+        const int64_t ko = ok ? pg * a.k_page + sl * a.k_slot + ch * 8 : 0;
+        const int64_t vo = ok ? pg * a.v_page + sl * a.v_slot + ch * 8 : 0;
+        cp_async16(kd + mma::swz(r, ch, DP * 2), kc + ko, ok);
+        cp_async16(vd + mma::swz(r, ch, DP * 2), vc + vo, ok);
+      }
+    };
+    int page, slot;
+    locate(k0, page, slot);
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; ++s) {
+      const int pg = page, sl = slot;
+      locate(k0 + s + 1, page, slot);
+      if (k0 + s < k1) load(s, pg, sl);
+      cp_commit();
+    }
+    cp_wait<S::STAGES - 1>();
+    __syncthreads();
+    uint32_t qf[DP / 16][4];
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      ldsm_x4(smem_addr(sQ) + mma::swz(lane % 16, kk * 2 + lane / 16, DP * 2), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+
+    float o[CH][4];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows lane / 4 and lane / 4 + 8, log2 units
+    int stage = 0;
+#pragma unroll 1
+    for (int kb = k0; kb < k1; ++kb) {
+      __syncwarp();  // every lane has read the stage that is filled next
+      {
+        const int pg = page, sl = slot, next = kb + S::STAGES - 1;
+        locate(next + 1, page, slot);
+        int fill = stage + S::STAGES - 1;
+        fill = fill >= S::STAGES ? fill - S::STAGES : fill;
+        if (next < k1) load(fill, pg, sl);
+        cp_commit();
+      }
+      cp_wait<S::STAGES - 1>();
+      __syncwarp();  // this block's rows, copied by every lane, are visible
+      const uint32_t kt = smem_addr(ring + stage * 2 * S::TILE), vt = kt + S::TILE;
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+      float s[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          uint32_t b0, b1, b2, b3;
+          const int r = j * 8 + (lane % 8) + (lane / 16) * 8;
+          ldsm_x4(kt + mma::swz(r, kk * 2 + (lane / 8) % 2, DP * 2), b0, b1, b2, b3);
+          mma_tile<T>(s[j], qf[kk], b0, b1);
+          mma_tile<T>(s[j + 1], qf[kk], b2, b3);
+        }
+      const int v0 = kb * S::BK + warp * WN;
+      float mx[2] = {m[0], m[1]};
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = v0 + j * 8 + (lane % 4) * 2 + (e & 1);
+          s[j][e] = v < vis.n ? s[j][e] * p.scale_log2 : -INFINITY;
+          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+        }
+      float alpha[2], sum[2] = {0.f, 0.f}, base[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        base[i] = mx[i] == -INFINITY ? 0.f : mx[i];  // a warp whose keys are all masked so far
+        alpha[i] = ex2(m[i] - base[i]);
+        m[i] = mx[i];
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][e] = ex2(s[j][e] - base[e >> 1]);
+          sum[e >> 1] += s[j][e];
+        }
+      l[0] = l[0] * alpha[0] + sum[0];
+      l[1] = l[1] * alpha[1] + sum[1];
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        o[j][0] *= alpha[0];
+        o[j][1] *= alpha[0];
+        o[j][2] *= alpha[1];
+        o[j][3] *= alpha[1];
+      }
+#pragma unroll
+      for (int kk = 0; kk < NT / 2; ++kk) {
+        // probabilities rounded to the cache's type, as the product's operand
+        const uint32_t pf[4] = {pack<T>(s[2 * kk][0], s[2 * kk][1]), pack<T>(s[2 * kk][2], s[2 * kk][3]),
+                                pack<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int j = 0; j < CH; j += 2) {
+          uint32_t b0, b1, b2, b3;
+          const int r = kk * 16 + (lane % 8) + ((lane / 8) % 2) * 8;
+          ldsm_x4_t(vt + mma::swz(r, j + lane / 16, DP * 2), b0, b1, b2, b3);
+          mma_tile<T>(o[j], pf, b0, b1);
+          mma_tile<T>(o[j + 1], pf, b2, b3);
+        }
+      }
+    }
+    // join the four warps
+    cp_wait<0>();
+    __syncthreads();
+    float *s_o = reinterpret_cast<float *>(body), *s_m = s_o + WARPS * ROWS * S::OPAD, *s_l = s_m + WARPS * ROWS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const int r = warp * ROWS + lane / 4 + i * 8;
+      if (lane % 4 == 0) {
+        s_m[r] = m[i];
+        s_l[r] = l[i];
+      }
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        *reinterpret_cast<float2 *>(s_o + r * S::OPAD + j * 8 + (lane % 4) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+    }
+    __syncthreads();
+    const bool whole = k0 == 0 && k1 == nb && !p.keep;
+    // the CTA's first segment has slot 2c, a later one that goes on in the next CTA 2c + 1
+    float *slot_ws = p.ws + (int64_t)(2 * c + (f != f0)) * S::SLOT;
+    for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
+      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * ROWS + r]);
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float mw = s_m[w * ROWS + r], g = mw == -INFINITY ? 0.f : ex2(mw - M);
+        const float4 y = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + r) * S::OPAD + d);
+        L += s_l[w * ROWS + r] * g;
+        x[0] += y.x * g;
+        x[1] += y.y * g;
+        x[2] += y.z * g;
+        x[3] += y.w * g;
+      }
+      if (whole) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        if (d < D)
+          *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + b * a.out_token + (h0 + r) * a.out_head + d) =
+              make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+      } else {
+        *reinterpret_cast<float4 *>(slot_ws + r * DP + d) = make_float4(x[0], x[1], x[2], x[3]);
+        if (d == 0) *reinterpret_cast<float2 *>(slot_ws + ROWS * DP + 2 * r) = make_float2(M, L);
+      }
+    }
+    f += k1 - k0;
+    if (f - before == (int64_t)nb * heads) {
+      before = f;
+      ++b;
+    }
+  }
+}
+
+// Joins the partials of one (sequence, 16-row group of heads).
+template <class T, int DP>
+__global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_constant__ Params p) {
+  using S = Shape<DP>;
+  const Args &a = p.a;
+  const int heads = (int)a.kv_heads * p.groups, b = blockIdx.x / heads, unit = blockIdx.x % heads;
+  const int G = (int)(a.q_heads / a.kv_heads), D = (int)a.head_dim;
+  const int hk = unit / p.groups, h0 = hk * G + (unit % p.groups) * ROWS, rows = min(ROWS, (hk + 1) * G - h0);
+  const Found at = find<S::BK>(a, [&](int64_t, int s, int64_t, int64_t) { return s == b; });
+  const int nb = blocks_of<S::BK>(a, b);
+  const int64_t total = at.total * heads, first = at.before * heads + (int64_t)unit * nb;
+  const int ctas = workers(total, p.ctas), c0 = owner(total, first, ctas), c1 = owner(total, first + nb - 1, ctas);
+  pdl_wait();  // in every block: the grid must not end before the one it follows
+  if (c0 == c1 && !p.keep) return;  // one CTA held it whole
+  const int s0 = 2 * c0 + (share(total, c0, ctas) != first), n = c1 - c0 + 1;
+  auto slot = [&](int i) { return p.ws + (int64_t)(i ? 2 * (c0 + i) : s0) * S::SLOT; };
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
+    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) M = fmaxf(M, __ldcg(slot(j) + ROWS * DP + 2 * r));
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(j) + ROWS * DP + 2 * r));
+      const float4 y = __ldcg(reinterpret_cast<const float4 *>(slot(j) + r * DP + d));
+      const float g = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      L += ml.y * g;
+      x[0] += y.x * g;
+      x[1] += y.y * g;
+      x[2] += y.z * g;
+      x[3] += y.w * g;
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (d < D)
+      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + b * a.out_token + (h0 + r) * a.out_head + d) =
+          make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+  }
+}
+
+int grid_ctas(int device) { return 2 * num_sms(device); }
+
+template <class T, int DP>
+int launch(Params &p, cudaStream_t st, int device) {
+  static ContextOnce attr;
+  if (int s = attr.run(device, []() -> int {
+        NKB_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::SMEM));
+        return NKB_OK;
+      }))
+    return s;
+  decode_kernel<T, DP><<<p.ctas, THREADS, Shape<DP>::SMEM, st>>>(p);
+  if (int s = launch_status("paged_decode")) return s;
+  const int64_t units = p.a.seqs * p.a.kv_heads * p.groups;
+  NKB_CUDA_TRY(launch_pdl(true, decode_join_kernel<T, DP>, dim3((unsigned)units), dim3(THREADS), 0, st, p));
+  return launch_status("paged_decode join");
+}
+
+}  // namespace
+
+size_t decode_workspace(const Args &a, int device) {
+  return (size_t)2 * grid_ctas(device) * (a.head_dim <= 64 ? Shape<64>::SLOT : Shape<128>::SLOT) * sizeof(float);
+}
+
+int decode_run(const Args &a, cudaStream_t st, int device) {
+  Params p;
+  p.a = a;
+  p.groups = (int)((a.q_heads / a.kv_heads + ROWS - 1) / ROWS);
+  p.scale_log2 = (float)(a.scale * 1.4426950408889634);
+  p.ws = static_cast<float *>(a.workspace);
+  p.ctas = grid_ctas(device);
+  p.keep = false;
+  if (a.dtype == NKB_BF16)
+    return a.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, st, device) : launch<__nv_bfloat16, 128>(p, st, device);
+  return a.head_dim <= 64 ? launch<__half, 64>(p, st, device) : launch<__half, 128>(p, st, device);
+}
+
+}  // namespace pattn
+}  // namespace nkb
