@@ -331,8 +331,9 @@ NKB_API int nkb_paged_append(const nkb_paged_append_args *args, void *stream);
  * what follows the prefix, all of the prefix is visible, and window must be 0.
  * Page ids outside the cache read as zero keys and values.  q, out and the
  * caches have one dtype; statistics and sums are fp32.  workspace: a device
- * array of nkb_paged_attention_workspace() bytes for this call alone (its
- * contents need not be kept or cleared). */
+ * array of nkb_paged_attention_workspace() bytes for this call alone, aligned to
+ * 16 bytes (its contents need not be kept or cleared); the bytes depend on the
+ * sizes and on whether q_start is given, not on the arrays. */
 typedef struct nkb_paged_attention_args {
   const void *q;
   void *out;

@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const __grid_const
   }
 }
 
-int check_args(const Args &a) {
+// what a call's sizes must be, without its arrays
+int check_sizes(const Args &a) {
   auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("paged_attention: ") + m); };
   if (int s = paged::check_cache("paged_attention", a.tokens, a.seqs, a.kv_heads, a.head_dim, a.pages, a.page_size,
                                  a.table_width, a.table_stride))
@@ -90,24 +91,30 @@ int check_args(const Args &a) {
     return fail(NKB_ERR_UNSUPPORTED, "paged_attention: q, out and caches must be float32, bfloat16 or float16");
   if (a.q_heads < 1 || a.q_heads % a.kv_heads || a.q_heads > 65535) return bad("q_heads must be a multiple of kv_heads");
   if (a.head_dim > MAX_D) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: head_dim above 256");
-  if (a.window < 0 || a.sinks < 0 || a.prefix_len < 0 || a.prefix_len > INT32_MAX) return bad("window, sinks and prefix_len must not be negative");
+  if (a.window < 0 || a.sinks < 0 || a.prefix_len < 0 || a.prefix_len > INT32_MAX)
+    return bad("window, sinks and prefix_len must not be negative");
   if (a.prefix_len && a.window) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: a window over a shared prefix");
-  if (a.prefix_len && !a.prefix_pages) return bad("a prefix needs its pages");
-  if (a.tokens && (!a.q || !a.out || !a.kv_len || (a.table_width && !a.page_table) || (a.pages && (!a.k_cache || !a.v_cache))))
-    return bad("NULL array");
   if (!a.q_start && a.tokens != a.seqs) return bad("without q_start there is one token per sequence");
   return NKB_OK;
 }
 
+int check_arrays(const Args &a) {
+  auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("paged_attention: ") + m); };
+  if (a.tokens && (!a.q || !a.out || !a.kv_len || (a.table_width && !a.page_table) || (a.pages && (!a.k_cache || !a.v_cache))))
+    return bad("NULL array");
+  if (a.tokens && a.prefix_len && !a.prefix_pages) return bad("a prefix needs its pages");
+  return NKB_OK;
+}
+
 // One new token per sequence of a 16-bit type, rows of whole 16-byte pieces,
-// up to 128 dimensions: the split decode kernel.
+// up to 128 dimensions: the split decode kernel.  (By the sizes; an unaligned
+// array then takes the form for any layout.)
 bool decode_form(const Args &a) {
-  return !a.q_start && !a.prefix_len && a.dtype != NKB_F32 && a.head_dim <= 128 && aligned16(a) &&
-         a.seqs * a.q_heads <= INT32_MAX;
+  return !a.q_start && !a.prefix_len && a.dtype != NKB_F32 && a.head_dim <= 128 && a.seqs * a.q_heads <= INT32_MAX;
 }
 
 int workspace(const Args &a, int device, size_t *bytes) {
-  if (int s = check_args(a)) return s;
+  if (int s = check_sizes(a)) return s;
   *bytes = a.tokens && decode_form(a) ? decode_workspace(a, device) : 0;
   return NKB_OK;
 }
@@ -115,12 +122,13 @@ int workspace(const Args &a, int device, size_t *bytes) {
 int run(const Args &a, int device, cudaStream_t st) {
   size_t need = 0;
   if (int s = workspace(a, device, &need)) return s;
+  if (int s = check_arrays(a)) return s;
   if (a.workspace_bytes < (int64_t)need || (need && !a.workspace))
     return fail(NKB_ERR_INVALID, "paged_attention: workspace of " + std::to_string(a.workspace_bytes) + " bytes, " +
                                      std::to_string(need) + " needed");
   if (reinterpret_cast<uintptr_t>(a.workspace) & 15) return fail(NKB_ERR_INVALID, "paged_attention: unaligned workspace");
   if (a.tokens == 0) return NKB_OK;
-  if (decode_form(a)) return decode_run(a, st, device);
+  if (decode_form(a) && aligned16(a)) return decode_run(a, st, device);
   paged::with_dtype(a.dtype, [&](auto t) {
     attn_any_kernel<decltype(t)><<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), WARPS * 32, 0, st>>>(a);
     return 0;

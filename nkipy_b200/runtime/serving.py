@@ -18,6 +18,7 @@ torch stream, so a call can be captured into a CUDA graph.
 """
 
 import ctypes
+import functools
 import math
 import struct
 
@@ -50,42 +51,49 @@ def _on_device(*tensors):
 
 
 def _float(t, name, ndim):
+    """The type code of a float tensor with ``ndim`` axes, the last one contiguous."""
     code = _CODES.get(t.dtype)
     if code is None:
         raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != ndim:
         _fail(f"{name}: expected {ndim} axes, got shape {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.size(-1) > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         _fail(f"{name}: the last axis must be contiguous")
     return code
 
 
-def _int32(t, name, shape):
+def _int32(t, name, *shape):
+    """Checks a contiguous int32 vector of the given length (None: any length)."""
     if t.dtype is not torch.int32:
         raise TypeError(f"{name}: expected int32, got {t.dtype}")
-    if t.dim() != len(shape) or any(n is not None and t.size(i) != n for i, n in enumerate(shape)):
-        _fail(f"{name}: expected shape {tuple('any' if n is None else n for n in shape)}, got {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.size(-1) > 1:
-        _fail(f"{name}: the last axis must be contiguous")
+    if t.dim() != 1 or (shape and t.shape[0] != shape[0]) or not t.is_contiguous():
+        _fail(f"{name}: expected a contiguous vector{f' of {shape[0]}' if shape else ''}, got shape {tuple(t.shape)}")
 
 
 def _batch(page_table, kv_len, q_start, tokens):
-    """Checks a call's page table and lengths; the number of sequences."""
-    _int32(page_table, "page_table", (None, None))
-    seqs = page_table.size(0)
-    _int32(kv_len, "kv_len", (seqs,))
+    """Checks a call's page table and lengths; sequences, table width and row stride."""
+    if page_table.dtype is not torch.int32:
+        raise TypeError(f"page_table: expected int32, got {page_table.dtype}")
+    if page_table.dim() != 2:
+        _fail(f"page_table: expected 2 axes, got shape {tuple(page_table.shape)}")
+    seqs, width = page_table.shape
+    stride = page_table.stride()
+    if stride[1] != 1 and width > 1:
+        _fail("page_table: the last axis must be contiguous")
+    _int32(kv_len, "kv_len", seqs)
     if q_start is not None:
-        _int32(q_start, "q_start", (seqs + 1,))
+        _int32(q_start, "q_start", seqs + 1)
     elif tokens != seqs:
         _fail(f"without q_start there is one token per sequence: {tokens} tokens, {seqs} sequences")
-    return seqs
+    return seqs, width, stride[0]
 
 
 def _caches(k_cache, v_cache):
     code = _float(k_cache, "k_cache", 4)
-    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+    if v_cache.dtype is not k_cache.dtype or v_cache.shape != k_cache.shape:
         _fail(f"k_cache and v_cache differ: {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
-    _float(v_cache, "v_cache", 4)
+    if v_cache.stride(-1) != 1 and v_cache.shape[-1] > 1:
+        _fail("v_cache: the last axis must be contiguous")
     return code
 
 
@@ -93,12 +101,24 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(device, *sizes):
+    """Workspace bytes of an attention call: by its sizes alone (positions in the struct as packed)."""
+    need = ctypes.c_size_t()
+    with torch.cuda.device(device):
+        _nkb.check(_nkb.lib().nkb_paged_attention_workspace(
+            _ATTENTION.pack(*([0] * 6), sizes[-1], *([0] * 2), *sizes[:-1], 0, 1.0), need))
+    return need.value
+
+
 def _launch(fn, packed, device):
     """Issues a call on the current stream of ``device``."""
     if torch.cuda.current_device() != device:
         with torch.cuda.device(device):
             return _launch(fn, packed, device)
-    _nkb.check(fn(packed, torch.cuda.current_stream(device).cuda_stream))
+    status = fn(packed, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _nkb.check(status)
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=None, cos=None, sin=None, pos_offset=0,
@@ -113,14 +133,14 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=Non
     device = _on_device(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, sin, q_out)
     code = _float(k, "k", 3)
     tokens, hkv, d = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
-        _fail(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
-    _float(v, "v", 3)
+    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    if v.shape != k.shape or v.dtype is not k.dtype or (vs[2] != 1 and d > 1):
+        _fail(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype} (strides {ks}, {vs})")
     cache_code = _caches(k_cache, v_cache)
-    pages, page_size = k_cache.size(0), k_cache.size(1)
-    if k_cache.size(2) != hkv or k_cache.size(3) != d:
-        _fail(f"caches hold {k_cache.size(2)} heads of {k_cache.size(3)}, k has {hkv} of {d}")
-    seqs = _batch(page_table, kv_len, q_start, tokens)
+    pages, page_size, heads, dim = k_cache.shape
+    if heads != hkv or dim != d:
+        _fail(f"caches hold {heads} heads of {dim}, k has {hkv} of {d}")
+    seqs, width, table_stride = _batch(page_table, kv_len, q_start, tokens)
     rot = rows = stride = rope_code = 0
     if (cos is None) != (sin is None):
         _fail("cos and sin go together")
@@ -128,27 +148,28 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=Non
         rope_code = _float(cos, "cos", 2)
         if sin.shape != cos.shape or sin.dtype != cos.dtype or sin.stride() != cos.stride():
             _fail("cos and sin differ in shape, type or strides")
-        rows, rot, stride = cos.size(0), 2 * cos.size(1), cos.stride(0)
+        rows, rot = cos.shape
+        rot, stride = 2 * rot, cos.stride(0)
         if rot > d:
             _fail(f"cos and sin rotate {rot} dimensions, head_dim is {d}")
     hq = q_token = q_head = qo_token = qo_head = 0
     if q is not None:
-        if _float(q, "q", 3) != code or q.size(0) != tokens or q.size(2) != d:
+        if _float(q, "q", 3) != code or q.shape[0] != tokens or q.shape[2] != d:
             _fail(f"q {tuple(q.shape)} {q.dtype} does not go with k {tuple(k.shape)} {k.dtype}")
-        hq, q_token, q_head = q.size(1), q.stride(0), q.stride(1)
+        hq = q.shape[1]
+        q_token, q_head, _ = q.stride()
         if q_out is None:
-            q_out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif _float(q_out, "q_out", 3) != code or q_out.shape != q.shape:
             _fail(f"q_out {tuple(q_out.shape)} {q_out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
-        qo_token, qo_head = q_out.stride(0), q_out.stride(1)
+        qo_token, qo_head, _ = q_out.stride()
     elif q_out is not None:
         _fail("q_out without q")
-    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
     packed = _APPEND.pack(
         k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
         kv_len.data_ptr(), _ptr(q_start), _ptr(cos), _ptr(sin), code, cache_code, rope_code, tokens, seqs, hq, hkv, d, rot,
         rows, stride, pos_offset, ks[0], ks[1], vs[0], vs[1], q_token, q_head, qo_token, qo_head, pages, page_size, kc[0],
-        kc[1], kc[2], vc[0], vc[1], vc[2], page_table.size(1), page_table.stride(0))
+        kc[1], kc[2], vc[0], vc[1], vc[2], width, table_stride)
     _launch(_nkb.lib().nkb_paged_append, packed, device)
     return q_out
 
@@ -159,24 +180,22 @@ def _attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, 
     tokens, hq, d = q.shape
     if _caches(k_cache, v_cache) != code:
         raise TypeError(f"q is {q.dtype}, the caches are {k_cache.dtype}")
-    pages, page_size, hkv = k_cache.size(0), k_cache.size(1), k_cache.size(2)
-    if k_cache.size(3) != d or hkv == 0 or hq % hkv:
-        _fail(f"q {tuple(q.shape)} does not go with caches of {hkv} heads of {k_cache.size(3)}")
-    seqs = _batch(page_table, kv_len, q_start, tokens)
+    pages, page_size, hkv, dim = k_cache.shape
+    if dim != d or hkv == 0 or hq % hkv:
+        _fail(f"q {tuple(q.shape)} does not go with caches of {hkv} heads of {dim}")
+    seqs, width, table_stride = _batch(page_table, kv_len, q_start, tokens)
     if out is None:
-        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif _float(out, "out", 3) != code or out.shape != q.shape:
         _fail(f"out {tuple(out.shape)} {out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
     qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
-    head = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-            kv_len.data_ptr(), _ptr(q_start), _ptr(prefix_pages))
     sizes = (code, tokens, seqs, hq, hkv, d, qs[0], qs[1], os_[0], os_[1], pages, page_size, kc[0], kc[1], kc[2], vc[0],
-             vc[1], vc[2], page_table.size(1), page_table.stride(0), window, sinks, prefix_len)
-    scale = 1.0 / math.sqrt(d) if scale is None else scale
-    need, lib = ctypes.c_size_t(), _nkb.lib()
-    _nkb.check(lib.nkb_paged_attention_workspace(_ATTENTION.pack(*head, 0, *sizes, 0, scale), need))
-    room = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    _launch(lib.nkb_paged_attention, _ATTENTION.pack(*head, _ptr(room), *sizes, need.value, scale), device)
+             vc[1], vc[2], width, table_stride, window, sinks, prefix_len)
+    need = _workspace(device, *sizes, q_start is not None)
+    room = q.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(_nkb.lib().nkb_paged_attention, _ATTENTION.pack(
+        q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(),
+        _ptr(q_start), _ptr(prefix_pages), _ptr(room), *sizes, need, 1.0 / math.sqrt(d) if scale is None else scale), device)
     return out
 
 
@@ -196,9 +215,9 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, 
     ``page_table`` and ``kv_len`` describe what each sequence has after the prefix."""
     if prefix_len < 0:
         _fail("prefix_len must not be negative")
-    _int32(prefix_pages, "prefix_pages", (None,))
-    if prefix_len > prefix_pages.size(0) * k_cache.size(1):
-        _fail(f"prefix of {prefix_len} tokens needs more than {prefix_pages.size(0)} pages of {k_cache.size(1)}")
+    _int32(prefix_pages, "prefix_pages")
+    if k_cache.dim() == 4 and prefix_len > prefix_pages.shape[0] * k_cache.shape[1]:
+        _fail(f"prefix of {prefix_len} tokens needs more than {prefix_pages.shape[0]} pages of {k_cache.shape[1]}")
     return _attention(q, k_cache, v_cache, page_table, kv_len, q_start, 0, 0, scale, out, prefix_pages, prefix_len)
 
 
@@ -215,11 +234,11 @@ def sample_tokens(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
         if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != rows or not t.is_contiguous()):
             _fail(f"{name}: expected a contiguous float32 tensor of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
     if top_k is not None:
-        _int32(top_k, "top_k", (rows,))
+        _int32(top_k, "top_k", rows)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = logits.new_empty(rows, dtype=torch.int32)
     else:
-        _int32(out, "out", (rows,))
+        _int32(out, "out", rows)
     packed = _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
                           out.data_ptr(), code, rows, vocab, logits.stride(0))
     _launch(_nkb.lib().nkb_sample_tokens, packed, device)
