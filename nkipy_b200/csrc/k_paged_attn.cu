@@ -113,9 +113,13 @@ bool decode_form(const Args &a) {
   return !a.q_start && !a.prefix_len && a.dtype != NKB_F32 && a.head_dim <= 128 && a.seqs * a.q_heads <= INT32_MAX;
 }
 
+// Tokens by q_start: the tensor-core tiles, for page sizes that a block of 128
+// keys is made of.
+bool several_form(const Args &a) { return a.q_start && !a.prefix_len && tile_form(a); }
+
 int workspace(const Args &a, int device, size_t *bytes) {
   if (int s = check_sizes(a)) return s;
-  *bytes = a.tokens && decode_form(a) ? decode_workspace(a, device) : 0;
+  *bytes = !a.tokens ? 0 : decode_form(a) ? decode_workspace(a, device) : several_form(a) ? tile_workspace(a, device) : 0;
   return NKB_OK;
 }
 
@@ -129,6 +133,7 @@ int run(const Args &a, int device, cudaStream_t st) {
   if (reinterpret_cast<uintptr_t>(a.workspace) & 15) return fail(NKB_ERR_INVALID, "paged_attention: unaligned workspace");
   if (a.tokens == 0) return NKB_OK;
   if (decode_form(a) && aligned16(a)) return decode_run(a, st, device);
+  if (several_form(a) && tile_strides(a)) return tile_run(a, st, device);
   paged::with_dtype(a.dtype, [&](auto t) {
     attn_any_kernel<decltype(t)><<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), WARPS * 32, 0, st>>>(a);
     return 0;

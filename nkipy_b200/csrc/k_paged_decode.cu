@@ -54,20 +54,6 @@ struct Params {
   bool keep;  // write every result as a partial (a prefix is joined to it)
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <class T>
-__device__ __forceinline__ uint32_t pack(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) { return mma::pack2(lo, hi); }
-template <>
-__device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t *>(&h);
-}
 template <class T>
 __device__ __forceinline__ void mma_tile(float *c, const uint32_t *a, uint32_t b0, uint32_t b1);
 template <>
@@ -143,18 +129,6 @@ __device__ __forceinline__ Found find(const Args &a, Want want) {
   r.seq = s_seq;
   r.before = s_before;
   return r;
-}
-
-// CTAs that share the blocks: none of them is left without one
-__device__ __forceinline__ int workers(int64_t total, int ctas) { return (int)min(total, (int64_t)ctas); }
-// first block of CTA c's share
-__device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) { return total * c / ctas; }
-// CTA whose share holds block f
-__device__ __forceinline__ int owner(int64_t total, int64_t f, int ctas) {
-  int c = (int)(f * ctas / total);
-  while (share(total, c + 1, ctas) <= f) ++c;
-  while (share(total, c, ctas) > f) --c;
-  return c;
 }
 
 template <class T, int DP>
@@ -342,9 +316,9 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
         *reinterpret_cast<float2 *>(s_o + r * S::OPAD + j * 8 + (lane % 4) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
     }
     __syncthreads();
-    const bool whole = k0 == 0 && k1 == nb && !p.keep;
-    // the CTA's first segment has slot 2c, a later one that goes on in the next CTA 2c + 1
-    float *slot_ws = p.ws + (int64_t)(2 * c + (f != f0)) * S::SLOT;
+    const bool all = k0 == 0 && k1 == nb, whole = all && !p.keep;
+    const int64_t at_slot = all ? 2 * p.ctas + (int64_t)b * heads + unit : 2 * c + (f != f0);
+    float *slot_ws = p.ws + at_slot * S::SLOT;
     for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       float M = -INFINITY, L = 0.f;
@@ -390,11 +364,11 @@ __global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_const
   const Found at = find<S::BK>(a, [&](int64_t, int s, int64_t, int64_t) { return s == b; });
   const int nb = blocks_of<S::BK>(a, b);
   const int64_t total = at.total * heads, first = at.before * heads + (int64_t)unit * nb;
-  const int ctas = workers(total, p.ctas), c0 = owner(total, first, ctas), c1 = owner(total, first + nb - 1, ctas);
+  const Parts parts = parts_of(total, first, nb, p.ctas, blockIdx.x);
   pdl_wait();  // in every block: the grid must not end before the one it follows
-  if (c0 == c1 && !p.keep) return;  // one CTA held it whole
-  const int s0 = 2 * c0 + (share(total, c0, ctas) != first), n = c1 - c0 + 1;
-  auto slot = [&](int i) { return p.ws + (int64_t)(i ? 2 * (c0 + i) : s0) * S::SLOT; };
+  if (parts.n == 1 && !p.keep) return;  // one CTA held it whole
+  const int n = parts.n;
+  auto slot = [&](int i) { return p.ws + (int64_t)parts.slot(i) * S::SLOT; };
   for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
     float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};

@@ -225,6 +225,9 @@ int nvls_read_and_clear_error(int *flag);
 int fa_read_and_clear_error(int *flag);
 int transpose_read_and_clear_error(int *flag);
 int waits_read_and_clear_error(int *flag);
+namespace pattn {
+int tile_read_and_clear_error(int *flag);
+}
 int wait_probe_launch(const uint32_t *counter, uint32_t target, cudaStream_t stream);
 }
 
@@ -239,7 +242,9 @@ extern "C" int nkb_device_error(int *flag) {
   if (int s = nkb::transpose_read_and_clear_error(&t)) return s;
   int w = 0;
   if (int s = nkb::waits_read_and_clear_error(&w)) return s;
-  *flag = g | l | n | f | t | w;
+  int p = 0;
+  if (int s = nkb::pattn::tile_read_and_clear_error(&p)) return s;
+  *flag = g | l | n | f | t | w | p;
   return NKB_OK;
 }
 
