@@ -110,16 +110,21 @@ int check_arrays(const Args &a) {
 // up to 128 dimensions: the split decode kernel.  (By the sizes; an unaligned
 // array then takes the form for any layout.)
 bool decode_form(const Args &a) {
-  return !a.q_start && !a.prefix_len && a.dtype != NKB_F32 && a.head_dim <= 128 && a.seqs * a.q_heads <= INT32_MAX;
+  return !a.q_start && a.dtype != NKB_F32 && a.head_dim <= 128 && a.seqs * a.q_heads <= INT32_MAX;
 }
 
 // Tokens by q_start: the tensor-core tiles, for page sizes that a block of 128
 // keys is made of.
-bool several_form(const Args &a) { return a.q_start && !a.prefix_len && tile_form(a); }
+bool several_form(const Args &a) { return a.q_start && tile_form(a); }
+// A shared prefix: its part on the tiles, the rest by either form.
+bool prefix_form(const Args &a) { return a.prefix_len > 0 && tile_form(a) && (a.q_start || decode_form(a)); }
 
 int workspace(const Args &a, int device, size_t *bytes) {
   if (int s = check_sizes(a)) return s;
-  *bytes = !a.tokens ? 0 : decode_form(a) ? decode_workspace(a, device) : several_form(a) ? tile_workspace(a, device) : 0;
+  if (!a.tokens) *bytes = 0;
+  else if (a.prefix_len) *bytes = prefix_form(a) ? prefix_workspace(a, device) : 0;
+  else if (decode_form(a)) *bytes = decode_workspace(a, device, false);
+  else *bytes = several_form(a) ? tile_workspace(a, device, true, false, false) : 0;
   return NKB_OK;
 }
 
@@ -132,8 +137,17 @@ int run(const Args &a, int device, cudaStream_t st) {
                                      std::to_string(need) + " needed");
   if (reinterpret_cast<uintptr_t>(a.workspace) & 15) return fail(NKB_ERR_INVALID, "paged_attention: unaligned workspace");
   if (a.tokens == 0) return NKB_OK;
-  if (decode_form(a) && aligned16(a)) return decode_run(a, st, device);
-  if (several_form(a) && tile_strides(a)) return tile_run(a, st, device);
+  if (a.prefix_len) {
+    if (prefix_form(a) && tile_strides(a)) return prefix_run(a, st, device);
+  } else if (decode_form(a) && aligned16(a)) {
+    single::Params p;
+    decode_params(a, device, a.workspace, false, &p);
+    return decode_launch(p, st, device, false);
+  } else if (several_form(a) && tile_strides(a)) {
+    several::Params p;
+    tile_params(a, device, a.workspace, true, false, false, &p);
+    return tile_launch(p, st, device);
+  }
   paged::with_dtype(a.dtype, [&](auto t) {
     attn_any_kernel<decltype(t)><<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), WARPS * 32, 0, st>>>(a);
     return 0;

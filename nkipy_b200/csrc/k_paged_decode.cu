@@ -29,30 +29,7 @@ using mma::ldsm_x4;
 using mma::ldsm_x4_t;
 using mma::smem_addr;
 
-constexpr int THREADS = 128, WARPS = 4, ROWS = 16;
-
-template <int DP>
-struct Shape {
-  static constexpr int WN = DP == 128 ? 16 : 32;       // keys per warp and stage
-  static constexpr int BK = WARPS * WN;                // keys per block
-  static constexpr int TILE = WN * DP * 2;             // bytes of K (or V) per stage
-  static constexpr int STAGES = 3;
-  static constexpr int RING = STAGES * 2 * TILE;       // per warp
-  static constexpr int OPAD = DP + 4;                  // row stride of the join buffer (floats)
-  static constexpr int JOIN = WARPS * ROWS * (OPAD + 2) * 4;
-  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
-  static constexpr int SMEM = ROWS * DP * 2 + BODY;
-  static constexpr int SLOT = ROWS * (DP + 2);         // floats of one partial: outputs, then max and sum
-};
-
-struct Params {
-  Args a;
-  int groups;  // 16-row groups of query heads per key head
-  float scale_log2;
-  float *ws;
-  int ctas;
-  bool keep;  // write every result as a partial (a prefix is joined to it)
-};
+using namespace single;
 
 template <class T>
 __device__ __forceinline__ void mma_tile(float *c, const uint32_t *a, uint32_t b0, uint32_t b1);
@@ -66,69 +43,6 @@ __device__ __forceinline__ void mma_tile<__half>(float *c, const uint32_t *a, ui
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ Visible visible_of(const Args &a, int b) {
-  return visible((int64_t)a.kv_len[b] - 1, a.table_width * a.page_size, a.window, a.sinks);
-}
-// key blocks of sequence b (one at least: a sequence without keys has a row of zeros to write)
-template <int BK>
-__device__ __forceinline__ int blocks_of(const Args &a, int b) {
-  return max(1, (visible_of(a, b).n + BK - 1) / BK);
-}
-
-// Sum of blocks_of over all sequences, and the first sequence whose blocks
-// before and in it reach past `f` units of `per` (its own included): found by
-// all threads of the block together.
-struct Found {
-  int64_t total;   // blocks of all sequences
-  int seq;         // the sequence
-  int64_t before;  // blocks of the sequences before it
-};
-template <int BK, class Want>
-__device__ __forceinline__ Found find(const Args &a, Want want) {
-  __shared__ int64_t s_warp[WARPS], s_before;
-  __shared__ int s_seq;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = (int)a.seqs;
-  Found r;
-  r.total = 0;
-  for (int base = 0; base < B; base += THREADS) {  // the sum
-    const int b = base + threadIdx.x;
-    int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) n += __shfl_xor_sync(0xffffffffu, n, w);
-    __syncthreads();
-    if (lane == 0) s_warp[warp] = n;
-    __syncthreads();
-    r.total += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
-  }
-  int64_t done = 0;
-  for (int base = 0; base < B; base += THREADS) {  // the sequence
-    const int b = base + threadIdx.x;
-    const int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
-    int64_t p = n;
-#pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, p, w);
-      if (lane >= w) p += x;
-    }
-    __syncthreads();
-    if (lane == 31) s_warp[warp] = p;
-    __syncthreads();
-    int64_t first = done + p - n;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) first += s_warp[w];
-      done += s_warp[w];
-    }
-    if (b < B && want(r.total, b, first, n)) {
-      s_seq = b;
-      s_before = first;
-    }
-  }
-  __syncthreads();
-  r.seq = s_seq;
-  r.before = s_before;
-  return r;
 }
 
 template <class T, int DP>
@@ -151,7 +65,10 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
   pdl_trigger();
   const int64_t total = at.total * heads;
   const int ctas = workers(total, p.ctas);
-  if (c >= ctas) return;
+  if (c >= ctas) {
+    pdl_wait();
+    return;
+  }
   const int64_t f0 = share(total, c, ctas), f1 = share(total, c + 1, ctas);
   int64_t f = f0, before = at.before * heads;  // `before`: blocks before sequence b
   int b = at.seq;
@@ -351,6 +268,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
       ++b;
     }
   }
+  pdl_wait();  // launched early, this grid must not end before the one it follows
 }
 
 // Joins the partials of one (sequence, 16-row group of heads).
@@ -395,15 +313,16 @@ __global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_const
 int grid_ctas(int device) { return 2 * num_sms(device); }
 
 template <class T, int DP>
-int launch(Params &p, cudaStream_t st, int device) {
+int launch(const Params &p, cudaStream_t st, int device, bool pdl) {
   static ContextOnce attr;
   if (int s = attr.run(device, []() -> int {
         NKB_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::SMEM));
         return NKB_OK;
       }))
     return s;
-  decode_kernel<T, DP><<<p.ctas, THREADS, Shape<DP>::SMEM, st>>>(p);
+  NKB_CUDA_TRY(launch_pdl(pdl, decode_kernel<T, DP>, dim3(p.ctas), dim3(THREADS), Shape<DP>::SMEM, st, p));
   if (int s = launch_status("paged_decode")) return s;
+  if (p.keep) return NKB_OK;
   const int64_t units = p.a.seqs * p.a.kv_heads * p.groups;
   NKB_CUDA_TRY(launch_pdl(true, decode_join_kernel<T, DP>, dim3((unsigned)units), dim3(THREADS), 0, st, p));
   return launch_status("paged_decode join");
@@ -411,21 +330,26 @@ int launch(Params &p, cudaStream_t st, int device) {
 
 }  // namespace
 
-size_t decode_workspace(const Args &a, int device) {
-  return (size_t)2 * grid_ctas(device) * (a.head_dim <= 64 ? Shape<64>::SLOT : Shape<128>::SLOT) * sizeof(float);
+size_t decode_workspace(const Args &a, int device, bool keep) {
+  const int64_t groups = (a.q_heads / a.kv_heads + ROWS - 1) / ROWS;
+  return (size_t)(2 * grid_ctas(device) + (keep ? a.seqs * a.kv_heads * groups : 0)) *
+         (a.head_dim <= 64 ? Shape<64>::SLOT : Shape<128>::SLOT) * sizeof(float);
 }
 
-int decode_run(const Args &a, cudaStream_t st, int device) {
-  Params p;
-  p.a = a;
-  p.groups = (int)((a.q_heads / a.kv_heads + ROWS - 1) / ROWS);
-  p.scale_log2 = (float)(a.scale * 1.4426950408889634);
-  p.ws = static_cast<float *>(a.workspace);
-  p.ctas = grid_ctas(device);
-  p.keep = false;
-  if (a.dtype == NKB_BF16)
-    return a.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, st, device) : launch<__nv_bfloat16, 128>(p, st, device);
-  return a.head_dim <= 64 ? launch<__half, 64>(p, st, device) : launch<__half, 128>(p, st, device);
+int decode_params(const Args &a, int device, void *workspace, bool keep, Params *p) {
+  p->a = a;
+  p->groups = (int)((a.q_heads / a.kv_heads + ROWS - 1) / ROWS);
+  p->scale_log2 = (float)(a.scale * 1.4426950408889634);
+  p->ws = static_cast<float *>(workspace);
+  p->ctas = grid_ctas(device);
+  p->keep = keep;
+  return NKB_OK;
+}
+
+int decode_launch(const Params &p, cudaStream_t st, int device, bool pdl) {
+  if (p.a.dtype == NKB_BF16)
+    return p.a.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, st, device, pdl) : launch<__nv_bfloat16, 128>(p, st, device, pdl);
+  return p.a.head_dim <= 64 ? launch<__half, 64>(p, st, device, pdl) : launch<__half, 128>(p, st, device, pdl);
 }
 
 }  // namespace pattn

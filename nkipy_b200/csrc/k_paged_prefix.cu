@@ -1,0 +1,121 @@
+// Paged attention of a batch whose sequences share their first prefix_len
+// tokens:
+//   out[t, h] = softmax over (prefix keys, own keys) times their values.
+// The prefix is attended once for all: the batch's tokens and the query heads
+// of a key head are the rows of the tensor-core tiles (k_paged_tile.cu), so its
+// keys and values are read once per 2 P tokens instead of once per sequence.
+// Each sequence's own keys take the form for single tokens or for several, and
+// both leave partials (max, sum, unnormalised output) that the kernel here
+// joins per token and head.
+#include "paged_attn.cuh"
+
+namespace nkb {
+namespace pattn {
+namespace {
+
+constexpr int THREADS = single::THREADS;
+
+struct Join {
+  const float *o, *ml;  // outputs of a row, and its (max, sum)
+};
+
+template <class T, int DP>
+__global__ void __launch_bounds__(THREADS)
+    prefix_join_kernel(const __grid_constant__ several::Params p, const __grid_constant__ single::Params s) {
+  using S = single::Shape<DP>;
+  constexpr int SLOT = several::slot_floats(DP), ML = 2 * several::BM * DP;
+  const Args &a = p.a;
+  const int t = blockIdx.x, hk = blockIdx.y, G = p.G, D = (int)a.head_dim, per = 2 * p.P;
+  single::Found at = {0, 0, 0};
+  if (!p.own) at = single::find<S::BK>(a, [&](int64_t, int b, int64_t, int64_t) { return b == t; });
+  pdl_wait();
+  const several::Walk walk(p, 0);
+  auto unit_parts = [&](int u, int &tok, int &seq) {  // of pair u
+    const several::Pair x = p.pairs[u];
+    const int64_t n = several::blocks_of(p, x).n;
+    tok = t - x.tok0;
+    seq = x.seq;
+    return parts_of(walk.total, p.head[1 + u] * a.kv_heads + hk * n, n, p.max_ctas, (int64_t)u * a.kv_heads + hk);
+  };
+  int ptok, otok = 0, seq = 0;
+  const Parts pre = unit_parts(t / per, ptok, seq);
+  Parts own;
+  int own_row_group = 0;
+  seq = 0;
+  if (p.own) {  // the pair of this token among the sequences' own
+    int lo = (int)((a.tokens + per - 1) / per), hi = (int)p.head[0] - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (p.pairs[mid].tok0 <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    own = unit_parts(lo, otok, seq);
+  }
+  const int heads = (int)a.kv_heads * s.groups;
+  for (int i = threadIdx.x; i < G * (DP / 4); i += THREADS) {
+    const int g = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (!p.own) {
+      const int unit = hk * s.groups + g / single::ROWS, nb = single::blocks_of<S::BK>(a, t);
+      own = parts_of(at.total * heads, at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
+    }
+    auto tile_part = [&](const Parts &x, int j, int tok) {
+      const float *slot = p.ws + (int64_t)x.slot(j) * SLOT;
+      const int row = tok / p.P * several::BM + tok % p.P * G + g;
+      return Join{slot + row * DP + d, slot + ML + 2 * row};
+    };
+    auto part = [&](int j) {
+      if (j < pre.n) return tile_part(pre, j, ptok);
+      if (p.own) return tile_part(own, j - pre.n, otok);
+      const float *slot = s.ws + (int64_t)own.slot(j - pre.n) * S::SLOT;
+      const int row = g % single::ROWS;
+      return Join{slot + row * DP + d, slot + single::ROWS * DP + 2 * row};
+    };
+    const int n = seq == -2 ? 0 : pre.n + own.n;  // a token of no sequence sees nothing
+    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < n; ++j) M = fmaxf(M, __ldcg(part(j).ml));
+    for (int j = 0; j < n; ++j) {
+      const Join q = part(j);
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q.ml));
+      const float4 y = __ldcg(reinterpret_cast<const float4 *>(q.o));
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      L += ml.y * f;
+      x[0] += y.x * f;
+      x[1] += y.y * f;
+      x[2] += y.z * f;
+      x[3] += y.w * f;
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (d < D)
+      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + t * a.out_token + (hk * G + g) * a.out_head + d) =
+          make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+  }
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t prefix_workspace(const Args &a, int device) {
+  const bool own = a.q_start != nullptr;
+  return up(tile_workspace(a, device, own, true, true)) + (own ? 0 : decode_workspace(a, device, true));
+}
+
+int prefix_run(const Args &a, cudaStream_t st, int device) {
+  const bool own = a.q_start != nullptr;
+  several::Params p;
+  single::Params s = {};
+  tile_params(a, device, a.workspace, own, true, true, &p);
+  decode_params(a, device, static_cast<char *>(a.workspace) + up(tile_workspace(a, device, own, true, true)), true, &s);
+  if (int e = tile_launch(p, st, device)) return e;
+  if (!own)
+    if (int e = decode_launch(s, st, device, true)) return e;
+  const dim3 grid((unsigned)a.tokens, (unsigned)a.kv_heads);
+  auto join = [&](auto kernel) { return launch_pdl(true, kernel, grid, dim3(THREADS), 0, st, p, s); };
+  const bool bf16 = a.dtype == NKB_BF16, small = a.head_dim <= 64;
+  NKB_CUDA_TRY(bf16 ? (small ? join(prefix_join_kernel<__nv_bfloat16, 64>) : join(prefix_join_kernel<__nv_bfloat16, 128>))
+                    : (small ? join(prefix_join_kernel<__half, 64>) : join(prefix_join_kernel<__half, 128>)));
+  return launch_status("paged prefix join");
+}
+
+}  // namespace pattn
+}  // namespace nkb

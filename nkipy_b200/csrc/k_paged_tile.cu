@@ -35,7 +35,8 @@ namespace {
 
 using namespace sm100;
 
-constexpr int BM = 128, BN = 128;
+using namespace several;
+
 constexpr int W_PROD = 8, W_MMA = 9, THREADS = 320;
 constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 columns, 128-byte swizzle
 constexpr uint32_t T_S = 0, T_O = 256, TMEM_COLS = 512;
@@ -48,57 +49,8 @@ struct Cfg {
   static constexpr int HALVES = DP / 64, TILE = HALVES * HALF, STAGES = DP == 128 ? 2 : 4;
   static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
   static constexpr int SMEM = 1024 + OFF_BAR + 256;
-  static constexpr int SLOT = 2 * BM * (DP + 2);  // floats of one partial: rows of both tiles, then (max, sum)
+  static constexpr int SLOT = slot_floats(DP);
 };
-
-// a pair: up to 2 P tokens of one sequence
-struct Pair {
-  int seq;  // -1: the shared prefix, -2: tokens of no sequence
-  int tok0, ntok, pos0;
-};
-
-struct Params {
-  Args a;
-  int G, P, page_shift, max_pairs, max_ctas;
-  int own, prefix;  // list the sequences' own keys / the prefix
-  int keep;         // write every unit as a partial
-  float scale_log2;
-  int64_t *head;   // number of pairs, then the pairs' first blocks (max_pairs + 1)
-  Pair *pairs;
-  int *seq_pairs;  // first pair of each sequence (scheduler only)
-  float *ws;
-};
-
-// The key blocks of a pair: `ns` from block 0 (first tokens), then [w0, w0 + n - ns).
-struct Blocks {
-  int end, low;  // keys below `end`, and from `low` (or below `sinks`) are seen by some row
-  int ns, w0, n;
-  __device__ __forceinline__ int block(int i) const { return i < ns ? i : w0 + i - ns; }
-};
-__device__ __forceinline__ Blocks blocks_of(const Params &p, const Pair &x) {
-  Blocks r;
-  if (x.seq < 0) {
-    r.end = x.seq == -1 ? (int)p.a.prefix_len : 0;
-    r.low = 0;
-  } else {
-    const int64_t cap = p.a.table_width * p.a.page_size;
-    r.end = (int)max((int64_t)0, min((int64_t)x.pos0 + x.ntok, cap));
-    r.low = p.a.window > 0 ? (int)min(max((int64_t)0, x.pos0 - p.a.window + 1), (int64_t)r.end) : 0;
-  }
-  const int sinks = (int)min(p.a.sinks, (int64_t)r.low);
-  r.w0 = r.low / BN;
-  r.ns = min((sinks + BN - 1) / BN, r.w0);
-  r.n = max(1, r.ns + (r.end + BN - 1) / BN - r.w0);
-  return r;
-}
-// blocks (from the first) that tile t of a pair needs
-__device__ __forceinline__ int tile_blocks(const Params &p, const Pair &x, const Blocks &k, int t) {
-  const int rows = min(x.ntok - t * p.P, p.P);
-  if (rows <= 0) return 0;
-  if (x.seq < 0) return x.seq == -1 ? k.n : 0;
-  const int end = (int)max((int64_t)0, min((int64_t)x.pos0 + t * p.P + rows, (int64_t)k.end));
-  return end == 0 ? 0 : k.ns + max(0, (end + BN - 1) / BN - k.w0);
-}
 
 // ---- the list of pairs ---------------------------------------------------------
 constexpr int SCHED = 1024;
@@ -125,10 +77,10 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *total) {
   return before + x - v;
 }
 
-// tokens of list entry i: the sequences, then the tokens before and after them
+// tokens of list entry i: those before the sequences, sequence i - 1, those after
 __device__ __forceinline__ void tokens_of(const Args &a, int i, int &first, int &n) {
   const int B = (int)a.seqs, T = (int)a.tokens;
-  const int lo = i < B ? a.q_start[i] : i == B ? 0 : a.q_start[B], hi = i < B ? a.q_start[i + 1] : i == B ? a.q_start[0] : T;
+  const int lo = i == 0 ? 0 : a.q_start[i - 1], hi = i > B ? T : a.q_start[i];
   first = max(0, min(lo, T));
   n = max(0, min(hi, T) - first);
 }
@@ -170,9 +122,9 @@ __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Pa
       const int off = (u - p.seq_pairs[lo]) * per;
       x.tok0 = first + off;
       x.ntok = max(0, min(per, n - off));
-      if (lo < B) {
-        x.seq = lo;
-        x.pos0 = a.kv_len[lo] - n + off;
+      if (lo >= 1 && lo <= B) {
+        x.seq = lo - 1;
+        x.pos0 = a.kv_len[lo - 1] - n + off;
       }
     }
     if (u < U) {
@@ -189,52 +141,6 @@ __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Pa
     p.head[1 + U] = blocks;
   }
 }
-
-// ---- segments: what a CTA's share holds of each unit -----------------------------
-struct Segment {
-  Pair x;
-  Blocks k;
-  int u, hk, k0, k1;  // pair, key head, blocks of it
-  bool all;           // the whole unit
-  int slot;           // of its partial
-};
-struct Walk {
-  const Params &p;
-  int64_t total, f, f0, f1;
-  int ctas, c;
-  __device__ __forceinline__ Walk(const Params &q, int cta) : p(q), c(cta) {
-    total = p.head[1 + p.head[0]] * p.a.kv_heads;
-    ctas = workers(total, p.max_ctas);
-    f0 = c < ctas ? share(total, c, ctas) : 0;
-    f1 = c < ctas ? share(total, c + 1, ctas) : 0;
-    f = f0;
-  }
-  // unit that holds block f
-  __device__ __forceinline__ void locate(int64_t at, Segment &s) const {
-    const int64_t row = at / p.a.kv_heads;  // pairs are kv_heads * n blocks long
-    int lo = 0, hi = (int)p.head[0] - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (p.head[1 + mid] <= row) lo = mid;
-      else hi = mid - 1;
-    }
-    s.u = lo;
-    s.x = p.pairs[lo];
-    s.k = blocks_of(p, s.x);
-    const int64_t in = at - p.head[1 + lo] * p.a.kv_heads;
-    s.hk = (int)(in / s.k.n);
-    s.k0 = (int)(in - (int64_t)s.hk * s.k.n);
-  }
-  __device__ __forceinline__ bool next(Segment &s) {
-    if (f >= f1) return false;
-    locate(f, s);
-    s.k1 = (int)min((int64_t)s.k.n, s.k0 + (f1 - f));
-    s.all = s.k0 == 0 && s.k1 == s.k.n;
-    s.slot = s.all ? 2 * p.max_ctas + s.u * (int)p.a.kv_heads + s.hk : 2 * c + (f != f0);
-    f += s.k1 - s.k0;
-    return true;
-  }
-};
 
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
   return mbar_wait(bar, parity, abort_flag, &g_tile_error);
@@ -673,29 +579,34 @@ bool tile_strides(const Args &a) {
          (a.pages == 1 || (a.k_page > 0 && a.v_page > 0)) && (a.q_heads == 1 || a.q_head > 0) && (a.tokens == 1 || a.q_token > 0);
 }
 
-size_t tile_workspace(const Args &a, int device) { return layout(a, num_sms(device), true, false, false).bytes; }
+size_t tile_workspace(const Args &a, int device, bool own, bool prefix, bool keep) {
+  return layout(a, num_sms(device), own, prefix, keep).bytes;
+}
 
-int tile_run(const Args &a, cudaStream_t st, int device) {
-  Params p;
-  p.a = a;
-  p.G = (int)(a.q_heads / a.kv_heads);
-  p.P = BM / p.G;
-  p.page_shift = log2_of(a.page_size);
-  p.max_ctas = num_sms(device);
-  p.own = 1;
-  p.prefix = 0;
-  p.keep = 0;
-  p.scale_log2 = (float)(a.scale * 1.4426950408889634);
-  const Layout x = layout(a, p.max_ctas, true, false, false);
-  p.max_pairs = x.max_pairs;
-  char *w = static_cast<char *>(a.workspace);
-  p.head = reinterpret_cast<int64_t *>(w);
-  p.pairs = reinterpret_cast<Pair *>(w + x.pairs);
-  p.seq_pairs = reinterpret_cast<int *>(w + x.seqs);
-  p.ws = reinterpret_cast<float *>(w + x.ws);
-  if (a.dtype == NKB_BF16)
-    return a.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, st, device) : launch<__nv_bfloat16, 128>(p, st, device);
-  return a.head_dim <= 64 ? launch<__half, 64>(p, st, device) : launch<__half, 128>(p, st, device);
+int tile_params(const Args &a, int device, void *workspace, bool own, bool prefix, bool keep, Params *p) {
+  p->a = a;
+  p->G = (int)(a.q_heads / a.kv_heads);
+  p->P = BM / p->G;
+  p->page_shift = log2_of(a.page_size);
+  p->max_ctas = num_sms(device);
+  p->own = own;
+  p->prefix = prefix;
+  p->keep = keep;
+  p->scale_log2 = (float)(a.scale * 1.4426950408889634);
+  const Layout x = layout(a, p->max_ctas, own, prefix, keep);
+  p->max_pairs = x.max_pairs;
+  char *w = static_cast<char *>(workspace);
+  p->head = reinterpret_cast<int64_t *>(w);
+  p->pairs = reinterpret_cast<Pair *>(w + x.pairs);
+  p->seq_pairs = reinterpret_cast<int *>(w + x.seqs);
+  p->ws = reinterpret_cast<float *>(w + x.ws);
+  return NKB_OK;
+}
+
+int tile_launch(const Params &p, cudaStream_t st, int device) {
+  if (p.a.dtype == NKB_BF16)
+    return p.a.head_dim <= 64 ? launch<__nv_bfloat16, 64>(p, st, device) : launch<__nv_bfloat16, 128>(p, st, device);
+  return p.a.head_dim <= 64 ? launch<__half, 64>(p, st, device) : launch<__half, 128>(p, st, device);
 }
 
 int tile_read_and_clear_error(int *flag) {

@@ -88,15 +88,220 @@ inline bool aligned16(const Args &a) {
   return true;
 }
 
-// single tokens (k_paged_decode.cu)
-size_t decode_workspace(const Args &a, int device);
-int decode_run(const Args &a, cudaStream_t st, int device);
+// ---- single tokens (k_paged_decode.cu) -------------------------------------
+namespace single {
 
-// several tokens per sequence (k_paged_tile.cu)
+constexpr int THREADS = 128, WARPS = 4, ROWS = 16;
+
+template <int DP>
+struct Shape {
+  static constexpr int WN = DP == 128 ? 16 : 32;       // keys per warp and stage
+  static constexpr int BK = WARPS * WN;                // keys per block
+  static constexpr int TILE = WN * DP * 2;             // bytes of K (or V) per stage
+  static constexpr int STAGES = 3;
+  static constexpr int RING = STAGES * 2 * TILE;       // per warp
+  static constexpr int OPAD = DP + 4;                  // row stride of the join buffer (floats)
+  static constexpr int JOIN = WARPS * ROWS * (OPAD + 2) * 4;
+  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
+  static constexpr int SMEM = ROWS * DP * 2 + BODY;
+  static constexpr int SLOT = ROWS * (DP + 2);         // floats of one partial: outputs, then max and sum
+};
+
+struct Params {
+  Args a;
+  int groups;  // 16-row groups of query heads per key head
+  float scale_log2;
+  float *ws;
+  int ctas;
+  bool keep;  // write every result as a partial (a prefix is joined to it)
+};
+
+__device__ __forceinline__ Visible visible_of(const Args &a, int b) {
+  return visible((int64_t)a.kv_len[b] - 1, a.table_width * a.page_size, a.window, a.sinks);
+}
+// key blocks of sequence b (one at least: a sequence without keys has a row of zeros to write)
+template <int BK>
+__device__ __forceinline__ int blocks_of(const Args &a, int b) {
+  return max(1, (visible_of(a, b).n + BK - 1) / BK);
+}
+
+// Sum of blocks_of over all sequences, and the first sequence whose blocks
+// before and in it reach past `f` units of `per` (its own included): found by
+// all threads of the block together.
+struct Found {
+  int64_t total;   // blocks of all sequences
+  int seq;         // the sequence
+  int64_t before;  // blocks of the sequences before it
+};
+template <int BK, class Want>
+__device__ __forceinline__ Found find(const Args &a, Want want) {
+  __shared__ int64_t s_warp[WARPS], s_before;
+  __shared__ int s_seq;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = (int)a.seqs;
+  Found r;
+  r.total = 0;
+  for (int base = 0; base < B; base += THREADS) {  // the sum
+    const int b = base + threadIdx.x;
+    int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) n += __shfl_xor_sync(0xffffffffu, n, w);
+    __syncthreads();
+    if (lane == 0) s_warp[warp] = n;
+    __syncthreads();
+    r.total += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+  }
+  int64_t done = 0;
+  for (int base = 0; base < B; base += THREADS) {  // the sequence
+    const int b = base + threadIdx.x;
+    const int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
+    int64_t p = n;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, p, w);
+      if (lane >= w) p += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = p;
+    __syncthreads();
+    int64_t first = done + p - n;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) first += s_warp[w];
+      done += s_warp[w];
+    }
+    if (b < B && want(r.total, b, first, n)) {
+      s_seq = b;
+      s_before = first;
+    }
+  }
+  __syncthreads();
+  r.seq = s_seq;
+  r.before = s_before;
+  return r;
+}
+
+}  // namespace single
+
+// `keep`: every result stays a partial in the workspace
+size_t decode_workspace(const Args &a, int device, bool keep);
+int decode_params(const Args &a, int device, void *workspace, bool keep, single::Params *p);
+int decode_launch(const single::Params &p, cudaStream_t st, int device, bool pdl);
+
+// ---- several tokens per sequence, a shared prefix (k_paged_tile.cu) ---------
+namespace several {
+
+constexpr int BM = 128, BN = 128;
+
+// a pair: up to 2 P tokens of one sequence
+struct Pair {
+  int seq;  // -1: the shared prefix, -2: tokens of no sequence
+  int tok0, ntok, pos0;
+};
+
+struct Params {
+  Args a;
+  int G, P, page_shift, max_pairs, max_ctas;
+  int own, prefix;  // list the sequences' own keys / the prefix
+  int keep;         // write every unit as a partial
+  float scale_log2;
+  int64_t *head;   // number of pairs, then the pairs' first blocks (max_pairs + 1)
+  Pair *pairs;
+  int *seq_pairs;  // first pair of each sequence (scheduler only)
+  float *ws;
+};
+
+// The key blocks of a pair: `ns` from block 0 (first tokens), then [w0, w0 + n - ns).
+struct Blocks {
+  int end, low;  // keys below `end`, and from `low` (or below `sinks`) are seen by some row
+  int ns, w0, n;
+  __device__ __forceinline__ int block(int i) const { return i < ns ? i : w0 + i - ns; }
+};
+__device__ __forceinline__ Blocks blocks_of(const Params &p, const Pair &x) {
+  Blocks r;
+  if (x.seq < 0) {
+    r.end = x.seq == -1 ? (int)p.a.prefix_len : 0;
+    r.low = 0;
+  } else {
+    const int64_t cap = p.a.table_width * p.a.page_size;
+    r.end = (int)max((int64_t)0, min((int64_t)x.pos0 + x.ntok, cap));
+    r.low = p.a.window > 0 ? (int)min(max((int64_t)0, x.pos0 - p.a.window + 1), (int64_t)r.end) : 0;
+  }
+  const int sinks = (int)min(p.a.sinks, (int64_t)r.low);
+  r.w0 = r.low / BN;
+  r.ns = min((sinks + BN - 1) / BN, r.w0);
+  r.n = max(1, r.ns + (r.end + BN - 1) / BN - r.w0);
+  return r;
+}
+// blocks (from the first) that tile t of a pair needs
+__device__ __forceinline__ int tile_blocks(const Params &p, const Pair &x, const Blocks &k, int t) {
+  const int rows = min(x.ntok - t * p.P, p.P);
+  if (rows <= 0) return 0;
+  if (x.seq < 0) return x.seq == -1 ? k.n : 0;
+  const int end = (int)max((int64_t)0, min((int64_t)x.pos0 + t * p.P + rows, (int64_t)k.end));
+  return end == 0 ? 0 : k.ns + max(0, (end + BN - 1) / BN - k.w0);
+}
+
+// ---- segments: what a CTA's share holds of each unit -----------------------------
+struct Segment {
+  Pair x;
+  Blocks k;
+  int u, hk, k0, k1;  // pair, key head, blocks of it
+  bool all;           // the whole unit
+  int slot;           // of its partial
+};
+struct Walk {
+  const Params &p;
+  int64_t total, f, f0, f1;
+  int ctas, c;
+  __device__ __forceinline__ Walk(const Params &q, int cta) : p(q), c(cta) {
+    total = p.head[1 + p.head[0]] * p.a.kv_heads;
+    ctas = workers(total, p.max_ctas);
+    f0 = c < ctas ? share(total, c, ctas) : 0;
+    f1 = c < ctas ? share(total, c + 1, ctas) : 0;
+    f = f0;
+  }
+  // unit that holds block f
+  __device__ __forceinline__ void locate(int64_t at, Segment &s) const {
+    const int64_t row = at / p.a.kv_heads;  // pairs are kv_heads * n blocks long
+    int lo = 0, hi = (int)p.head[0] - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (p.head[1 + mid] <= row) lo = mid;
+      else hi = mid - 1;
+    }
+    s.u = lo;
+    s.x = p.pairs[lo];
+    s.k = blocks_of(p, s.x);
+    const int64_t in = at - p.head[1 + lo] * p.a.kv_heads;
+    s.hk = (int)(in / s.k.n);
+    s.k0 = (int)(in - (int64_t)s.hk * s.k.n);
+  }
+  __device__ __forceinline__ bool next(Segment &s) {
+    if (f >= f1) return false;
+    locate(f, s);
+    s.k1 = (int)min((int64_t)s.k.n, s.k0 + (f1 - f));
+    s.all = s.k0 == 0 && s.k1 == s.k.n;
+    s.slot = s.all ? 2 * p.max_ctas + s.u * (int)p.a.kv_heads + s.hk : 2 * c + (f != f0);
+    f += s.k1 - s.k0;
+    return true;
+  }
+};
+
+// floats of one partial: the rows of both tiles, then their (max, sum)
+constexpr int slot_floats(int dp) { return 2 * BM * (dp + 2); }
+
+}  // namespace several
+
 bool tile_form(const Args &a);     // by the sizes
 bool tile_strides(const Args &a);  // whether TMA can describe the operands
-size_t tile_workspace(const Args &a, int device);
-int tile_run(const Args &a, cudaStream_t st, int device);
+// `own`: the sequences' own keys, `prefix`: the shared prefix's; `keep`: every
+// result stays a partial in the workspace
+size_t tile_workspace(const Args &a, int device, bool own, bool prefix, bool keep);
+int tile_params(const Args &a, int device, void *workspace, bool own, bool prefix, bool keep, several::Params *p);
+int tile_launch(const several::Params &p, cudaStream_t st, int device);
+
+// a shared prefix (k_paged_prefix.cu)
+size_t prefix_workspace(const Args &a, int device);
+int prefix_run(const Args &a, cudaStream_t st, int device);
 int tile_read_and_clear_error(int *flag);
 
 }  // namespace pattn
