@@ -3,6 +3,8 @@
 //   lo' = lo cos_p - hi sin_p,  hi' = lo sin_p + hi cos_p
 // for the two halves (lo, hi) of the first rot_dim dimensions at position p,
 // in fp32, rounded once to the stored type.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace nkb {
@@ -12,42 +14,47 @@ using Args = nkb_paged_append_args;
 
 constexpr int THREADS = 256;
 
-// One block per token: its rows (query heads, key heads, value heads), element
-// by element.
+// Where a token goes: its sequence, the row of the rotation tables, and the
+// offsets of its cache rows (-1: not stored).
+struct Place {
+  int seq;
+  int64_t rope, k, v;
+};
+__device__ __forceinline__ Place place_of(const Args &a, int t, int b) {
+  Place p = {b, 0, -1, -1};
+  if (b < 0) return p;
+  const int first = a.q_start ? a.q_start[b] : t, n = a.q_start ? a.q_start[b + 1] - first : 1;
+  const int64_t pos = (int64_t)a.kv_len[b] - n + (t - first);
+  if (pos >= 0 && pos < a.table_width * a.page_size) {
+    const int i = (int)pos / (int)a.page_size, slot = (int)pos - i * (int)a.page_size;
+    const int page = a.page_table[b * a.table_stride + i];
+    if (paged::page_ok(page, a.pages)) {
+      p.k = page * a.k_page + slot * a.k_slot;
+      p.v = page * a.v_page + slot * a.v_slot;
+    }
+  }
+  p.rope = max((int64_t)0, min(pos + a.pos_offset, a.rope_rows - 1)) * a.rope_stride;
+  return p;
+}
+
+// Any layout: one block per token, its rows (query heads, key heads, value
+// heads) element by element.
 template <class T, class C>
-__global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__ Args a) {
-  __shared__ int slot;
+__global__ void __launch_bounds__(THREADS) append_any_kernel(const __grid_constant__ Args a) {
+  __shared__ int found;
   const int t = blockIdx.x;
-  const int b = paged::block_find_seq(a.q_start, (int)a.seqs, t, &slot);
+  const Place at = place_of(a, t, paged::block_find_seq(a.q_start, (int)a.seqs, t, &found));
   const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
   T *qo = static_cast<T *>(a.q_out);
   C *kc = static_cast<C *>(a.k_cache), *vc = static_cast<C *>(a.v_cache);
   const int D = (int)a.head_dim, half = (int)a.rot_dim / 2;
-  int64_t pos = 0, cache_row_k = -1, cache_row_v = -1;
-  if (b >= 0) {
-    const int first = a.q_start ? a.q_start[b] : t, n = a.q_start ? a.q_start[b + 1] - first : 1;
-    pos = (int64_t)a.kv_len[b] - n + (t - first);
-    if (pos >= 0 && pos < a.table_width * a.page_size) {
-      const int page = a.page_table[b * a.table_stride + pos / a.page_size];
-      if (paged::page_ok(page, a.pages)) {
-        const int64_t s = pos % a.page_size;
-        cache_row_k = page * a.k_page + s * a.k_slot;
-        cache_row_v = page * a.v_page + s * a.v_slot;
-      }
-    }
-  }
-  int64_t row = pos + a.pos_offset;
-  row = row < 0 ? 0 : row >= a.rope_rows ? a.rope_rows - 1 : row;
-  auto angle = [&](const void *table, int i) {
-    return load_as_float(table, row * a.rope_stride + i, (int)a.rope_dtype);
-  };
   const int hq = a.q_out ? (int)a.q_heads : 0, hkv = (int)a.kv_heads;
   for (int i = threadIdx.x; i < (hq + 2 * hkv) * D; i += THREADS) {
     const int h = i / D, d = i % D;
     if (h >= hq + hkv) {
       const int hv = h - hq - hkv;
-      if (cache_row_v >= 0)
-        vc[cache_row_v + hv * a.v_cache_head + d] = paged::from_f32<C>(paged::to_f32(v[t * a.v_token + hv * a.v_head + d]));
+      if (at.v >= 0)
+        vc[at.v + hv * a.v_cache_head + d] = paged::from_f32<C>(paged::to_f32(v[t * a.v_token + hv * a.v_head + d]));
       continue;
     }
     const bool is_q = h < hq;
@@ -55,20 +62,142 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
     if (d >= half && d < 2 * half) continue;  // written with its partner
     float x = paged::to_f32(src[d]), y = 0.f;
     if (d < half) {
-      const float hi = paged::to_f32(src[d + half]), c = angle(a.cos, d), s = angle(a.sin, d);
+      const float hi = paged::to_f32(src[d + half]), c = load_as_float(a.cos, at.rope + d, (int)a.rope_dtype),
+                  s = load_as_float(a.sin, at.rope + d, (int)a.rope_dtype);
       y = x * s + hi * c;
       x = x * c - hi * s;
     }
     if (is_q) {
       T *dst = qo + t * a.q_out_token + h * a.q_out_head;
-      dst[d] = paged::from_f32<T>(b < 0 ? 0.f : x);
-      if (d < half) dst[d + half] = paged::from_f32<T>(b < 0 ? 0.f : y);
-    } else if (cache_row_k >= 0) {
-      C *dst = kc + cache_row_k + (h - hq) * a.k_cache_head;
+      dst[d] = paged::from_f32<T>(at.seq < 0 ? 0.f : x);
+      if (d < half) dst[d + half] = paged::from_f32<T>(at.seq < 0 ? 0.f : y);
+    } else if (at.k >= 0) {
+      C *dst = kc + at.k + (h - hq) * a.k_cache_head;
       dst[d] = paged::from_f32<C>(x);
       if (d < half) dst[d + half] = paged::from_f32<C>(y);
     }
   }
+}
+
+// Eight elements of a 16-byte piece (two pieces for fp32).
+template <class T>
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+  }
+  __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ void get(float *f) const {
+    const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = paged::to_f32(e[i]);
+  }
+  __device__ __forceinline__ void set(const float *f) {
+    T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = paged::from_f32<T>(f[i]);
+  }
+};
+
+// Rows of whole 16-byte pieces whose halves are whole pieces too: a row is
+// `pieces` pairs of eight elements (d, d + rot_dim / 2 of the rotated part, then
+// neighbouring pieces of the rest), one pair per thread and step.  Each byte is
+// moved once; a block takes one token, so its place is looked up once, while
+// the first rows are already on their way.
+template <class T, class C, class R>
+__global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__ Args a, int pieces, int unit) {
+  __shared__ int found;
+  const int t = blockIdx.x, half = (int)a.rot_dim / 2, D = (int)a.head_dim;
+  const int hq = a.q_out ? (int)a.q_heads : 0, hkv = (int)a.kv_heads, rows = hq + 2 * hkv;
+  const int step = THREADS / unit, c = threadIdx.x % unit, h0 = threadIdx.x / unit + blockIdx.y * step;
+  const bool live = c < pieces && h0 < rows;
+  const bool turns = c * 8 < half;
+  // the pair's elements: d0 .. d0 + 7 and d1 .. d1 + 7 (none past the row's end)
+  const int d0 = turns ? c * 8 : 2 * half + (c - half / 8) * 16, d1 = turns ? d0 + half : d0 + 8;
+  const bool two = d1 < D;
+  auto source = [&](int h) {
+    return h < hq ? static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head
+           : h < hq + hkv ? static_cast<const T *>(a.k) + t * a.k_token + (h - hq) * a.k_head
+                          : static_cast<const T *>(a.v) + t * a.v_token + (h - hq - hkv) * a.v_head;
+  };
+  Eight<T> lo, hi;
+  if (live) {
+    const T *src = source(h0);
+    lo.load(src + d0);
+    if (two) hi.load(src + d1);
+  }
+  const Place at = place_of(a, t, paged::block_find_seq(a.q_start, (int)a.seqs, t, &found));
+  float cs[8], sn[8];
+  if (live && turns) {
+    Eight<R> e;
+    e.load(static_cast<const R *>(a.cos) + at.rope + d0);
+    e.get(cs);
+    e.load(static_cast<const R *>(a.sin) + at.rope + d0);
+    e.get(sn);
+  }
+  for (int h = h0; live && h < rows;) {
+    float x[8], y[8];
+    lo.get(x);
+    hi.get(y);
+    const int now = h;
+    h += step * gridDim.y;
+    if (h < rows) {  // the next row is on its way
+      const T *src = source(h);
+      lo.load(src + d0);
+      if (two) hi.load(src + d1);
+    }
+    if (turns && now < hq + hkv) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = x[i], q = y[i];
+        x[i] = p * cs[i] - q * sn[i];
+        y[i] = p * sn[i] + q * cs[i];
+      }
+    }
+    if (now < hq) {
+      if (at.seq < 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+      }
+      Eight<T> o;
+      T *dst = static_cast<T *>(a.q_out) + t * a.q_out_token + now * a.q_out_head;
+      o.set(x);
+      o.store(dst + d0);
+      o.set(y);
+      if (two) o.store(dst + d1);
+    } else {
+      const bool is_k = now < hq + hkv;
+      const int64_t row = is_k ? at.k : at.v;
+      if (row < 0) continue;
+      C *dst = is_k ? static_cast<C *>(a.k_cache) + row + (now - hq) * a.k_cache_head
+                    : static_cast<C *>(a.v_cache) + row + (now - hq - hkv) * a.v_cache_head;
+      Eight<C> o;
+      o.set(x);
+      o.store(dst + d0);
+      o.set(y);
+      if (two) o.store(dst + d1);
+    }
+  }
+}
+
+// Whether every row starts at a 16-byte boundary and is made of whole pieces,
+// the rotated halves too.
+bool pieces_form(const Args &a) {
+  const int64_t ts = dtype_size((int)a.dtype), cs = dtype_size((int)a.cache_dtype), rs = dtype_size((int)a.rope_dtype);
+  auto whole = [](int64_t stride, int64_t size) { return stride >= 0 && stride * size % 16 == 0; };
+  for (int64_t s : {a.k_token, a.k_head, a.v_token, a.v_head, a.q_token, a.q_head, a.q_out_token, a.q_out_head})
+    if (!whole(s, ts)) return false;
+  for (int64_t s : {a.k_page, a.k_slot, a.k_cache_head, a.v_page, a.v_slot, a.v_cache_head})
+    if (!whole(s, cs)) return false;
+  if (a.rot_dim && !whole(a.rope_stride, rs)) return false;
+  uintptr_t p = 0;
+  for (const void *x : {a.k, a.v, a.q, (const void *)a.q_out, (const void *)a.k_cache, (const void *)a.v_cache, a.cos, a.sin})
+    p |= reinterpret_cast<uintptr_t>(x);
+  return p % 16 == 0 && a.head_dim % 8 == 0 && a.rot_dim % 16 == 0 && a.head_dim <= 16 * THREADS;
 }
 
 int check_args(const Args &a) {
@@ -89,13 +218,32 @@ int check_args(const Args &a) {
   return NKB_OK;
 }
 
-int run(const Args &a, cudaStream_t st) {
+int run(const Args &a, cudaStream_t st, int device) {
   if (int s = check_args(a)) return s;
   if (a.tokens == 0) return NKB_OK;
+  if (!pieces_form(a)) {
+    paged::with_dtype(a.dtype, [&](auto t) {
+      return paged::with_dtype(a.cache_dtype, [&](auto c) {
+        append_any_kernel<decltype(t), decltype(c)><<<(unsigned)a.tokens, THREADS, 0, st>>>(a);
+        return 0;
+      });
+    });
+    return launch_status("paged_append");
+  }
+  // pairs of pieces per row, and the threads that a row takes: the next power of two
+  const int pieces = (int)(a.rot_dim / 16 + (a.head_dim - a.rot_dim + 15) / 16);
+  int unit = 1;
+  while (unit < pieces) unit *= 2;
+  // a few tokens spread their rows over more blocks
+  const int rows = (int)((a.q_out ? a.q_heads : 0) + 2 * a.kv_heads), step = THREADS / unit;
+  const int64_t want = (2 * num_sms(device) + a.tokens - 1) / a.tokens;
+  const unsigned split = (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + step - 1) / step, want));
   paged::with_dtype(a.dtype, [&](auto t) {
     return paged::with_dtype(a.cache_dtype, [&](auto c) {
-      append_kernel<decltype(t), decltype(c)><<<(unsigned)a.tokens, THREADS, 0, st>>>(a);
-      return 0;
+      return paged::with_dtype(a.rot_dim ? a.rope_dtype : NKB_F32, [&](auto r) {
+        append_kernel<decltype(t), decltype(c), decltype(r)><<<dim3((unsigned)a.tokens, split), THREADS, 0, st>>>(a, pieces, unit);
+        return 0;
+      });
     });
   });
   return launch_status("paged_append");
@@ -106,5 +254,7 @@ int run(const Args &a, cudaStream_t st) {
 
 extern "C" int nkb_paged_append(const nkb_paged_append_args *args, void *stream) {
   if (!args) return nkb::fail(NKB_ERR_INVALID, "args is NULL");
-  return nkb::append::run(*args, static_cast<cudaStream_t>(stream));
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return nkb::append::run(*args, static_cast<cudaStream_t>(stream), dev);
 }
