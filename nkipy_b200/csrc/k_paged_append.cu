@@ -249,7 +249,23 @@ int run(const Args &a, cudaStream_t st, int device) {
   return launch_status("paged_append");
 }
 
+// "paged_append": the pointers of nkb_paged_append_args that are given; ints a
+// mask of them and the struct's integers
+int check(const Step &s) {
+  Args a;
+  if (int e = paged::step_args(s, nullptr, 11, 30, "paged_append", &a)) return e;
+  return check_args(a);
+}
+int launch(const LaunchArgs &l) {
+  Args a;
+  if (int e = paged::step_args(*l.step, l.ptrs, 11, 30, "paged_append", &a)) return e;
+  return run(a, l.stream, l.device);
+}
+
 }  // namespace append
+
+NKB_REGISTER_KERNEL("paged_append", append::launch, append::check);
+
 }  // namespace nkb
 
 extern "C" int nkb_paged_append(const nkb_paged_append_args *args, void *stream) {

@@ -155,7 +155,24 @@ int run(const Args &a, int device, cudaStream_t st) {
   return launch_status("paged_attention");
 }
 
+// "paged_attention": the pointers of nkb_paged_attention_args that are given;
+// ints a mask of them and the struct's integers; floats scale
+int check(const Step &s) {
+  Args a;
+  if (int e = paged::step_args(s, nullptr, 9, 24, "paged_attention", &a)) return e;
+  if (int e = check_sizes(a)) return e;
+  return check_arrays(a);
+}
+int launch(const LaunchArgs &l) {
+  Args a;
+  if (int e = paged::step_args(*l.step, l.ptrs, 9, 24, "paged_attention", &a)) return e;
+  return run(a, l.device, l.stream);
+}
+
 }  // namespace pattn
+
+NKB_REGISTER_KERNEL("paged_attention", pattn::launch, pattn::check);
+
 }  // namespace nkb
 
 extern "C" int nkb_paged_attention_workspace(const nkb_paged_attention_args *args, size_t *bytes) {

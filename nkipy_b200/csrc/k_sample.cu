@@ -25,7 +25,7 @@
 
 #include <type_traits>
 
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace nkb {
 namespace sample {
@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(THREADS) long_row_kernel(const __grid_constant
 }
 
 
-int run(const Args &a, cudaStream_t st, int device) {
+int check_args(const Args &a) {
   auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("sample_tokens: ") + m); };
   if (a.rows < 0 || a.rows > INT32_MAX / MAX_C || a.vocab < 1) return bad("rows or vocab out of range");
   if (a.dtype != NKB_F32 && a.dtype != NKB_BF16 && a.dtype != NKB_F16)
@@ -734,6 +734,11 @@ int run(const Args &a, cudaStream_t st, int device) {
   if (a.vocab > MAX_VOCAB) return fail(NKB_ERR_UNSUPPORTED, "sample_tokens: more than 2^21 entries");
   if (a.rows && (!a.logits || !a.u || !a.tokens)) return bad("NULL array");
   if (a.rows > 1 && a.row_stride < a.vocab) return bad("rows overlap");
+  return NKB_OK;
+}
+
+int run(const Args &a, cudaStream_t st, int device) {
+  if (int s = check_args(a)) return s;
   if (a.rows == 0) return NKB_OK;
   int slice = 0;
   if (const int C = cluster_for(a, &slice)) {
@@ -745,7 +750,23 @@ int run(const Args &a, cudaStream_t st, int device) {
   return launch_status("sample_tokens");
 }
 
+// "sample_tokens": the pointers of nkb_sample_args that are given; ints a mask of
+// them and the struct's integers
+int check(const Step &s) {
+  Args a;
+  if (int e = paged::step_args(s, nullptr, 7, 4, "sample_tokens", &a)) return e;
+  return check_args(a);
+}
+int launch(const LaunchArgs &l) {
+  Args a;
+  if (int e = paged::step_args(*l.step, l.ptrs, 7, 4, "sample_tokens", &a)) return e;
+  return run(a, l.stream, l.device);
+}
+
 }  // namespace sample
+
+NKB_REGISTER_KERNEL("sample_tokens", sample::launch, sample::check);
+
 }  // namespace nkb
 
 extern "C" int nkb_sample_tokens(const nkb_sample_args *args, void *stream) {

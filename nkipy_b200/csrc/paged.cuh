@@ -2,6 +2,8 @@
 // has, and where a position's row lies in the pages.
 #pragma once
 
+#include <cstring>
+
 #include "common.cuh"
 
 namespace nkb {
@@ -54,6 +56,36 @@ int with_dtype(int64_t dt, F &&f) {
   if (dt == NKB_F32) return f(float{});
   if (dt == NKB_BF16) return f(__nv_bfloat16{});
   return f(__half{});
+}
+
+// The argument struct of a plan step: its pointers first, then 8-byte integers
+// (and doubles, from the step's floats).  ints[0] has a bit for each pointer
+// that is given, in order; ptrs is NULL while a plan is checked.
+template <class A>
+int step_args(const Step &s, void *const *ptrs, int n_ptrs, int n_ints, const char *what, A *a) {
+  static_assert(sizeof(void *) == 8 && sizeof(int64_t) == 8, "8-byte fields");
+  const int n_floats = (int)(sizeof(A) / 8) - n_ptrs - n_ints;
+  auto bad = [&]() { return fail(NKB_ERR_PLAN, std::string(what) + ": bad parameters"); };
+  if ((int)s.ints.size() != n_ints + 1 || (int)s.floats.size() != n_floats) return bad();
+  if (s.ints[0] < 0 || s.ints[0] >> n_ptrs) return bad();
+  char *at = reinterpret_cast<char *>(a);
+  size_t next = 0;
+  for (int i = 0; i < n_ptrs; ++i) {
+    void *p = nullptr;
+    if (s.ints[0] >> i & 1) {
+      if (next >= s.buf_ids.size()) return bad();
+      p = ptrs ? ptrs[next] : reinterpret_cast<void *>(16);  // any that is not NULL and aligned
+      ++next;
+    }
+    memcpy(at + 8 * i, &p, 8);
+  }
+  if (next != s.buf_ids.size()) return bad();
+  for (int i = 0; i < n_ints; ++i) memcpy(at + 8 * (n_ptrs + i), &s.ints[1 + i], 8);
+  for (int i = 0; i < n_floats; ++i) {
+    const double f = s.floats[i];
+    memcpy(at + 8 * (n_ptrs + n_ints + i), &f, 8);
+  }
+  return NKB_OK;
 }
 
 // What every call on a paged cache requires of its sizes (names for messages).

@@ -1211,6 +1211,96 @@ class Lowering:
         self.step("topk_rows", bufs, ints, note=f"{rows}x{cols} k={k}")
         self.tuples[op.id] = (vals, idx)
 
+    # ------------------------------------------------------------ serving
+    def rows_view(self, t) -> V.View:
+        """A view of ``t`` whose last axis is contiguous and that repeats no element: the
+        serving kernels take every other stride."""
+        v = self.materialize(self.get(t), dense=False)
+        inner = v.shape[-1] <= 1 or v.strides[-1] == 1
+        return v if inner and all(s > 0 for s, n in zip(v.strides, v.shape) if n > 1) else self.materialize(v, dense=True, out=self.tmp_view(v.shape, v.dtype))
+
+    def serving_step(self, kernel, op, order, views, ints, floats=(), note=""):
+        """A step whose buffers are the given arrays in the order of the C argument
+        struct; the first int has a bit for each that is given."""
+        bufs, mask = [], 0
+        for i, name in enumerate(order):
+            v = views.get(name)
+            if v is not None:
+                mask |= 1 << i
+                bufs.append(self.bref(v))
+        self.step(kernel, bufs, [mask] + list(ints), floats, note=note)
+
+    @staticmethod
+    def _strides(v, axes):
+        """Element strides of a view's leading ``axes`` axes (a size-1 axis has the dense one)."""
+        dense = V.dense_strides(v.shape)
+        return [int(v.strides[i]) if v.shape[i] > 1 else int(dense[i]) for i in range(axes)]
+
+    def op_paged_append(self, op):
+        """``paged-append``: one ``paged_append`` launch writing into the caches in place."""
+        t = dict(zip(op.attributes["operands"], op.operands))
+        views = {n: self.rows_view(x) for n, x in t.items() if n not in ("k_cache", "v_cache", "page_table", "kv_len", "q_start")}
+        for n in ("page_table", "kv_len", "q_start"):
+            if n in t:
+                views[n] = self.materialize(self.get(t[n]), dense=True)
+        views["k_cache"] = self.mutable_base(t["k_cache"], op)
+        views["v_cache"] = self.mutable_base(t["v_cache"], op)
+        k, kc = views["k"], views["k_cache"]
+        tokens, hkv, d = k.shape
+        q, cos = views.get("q"), views.get("cos")
+        if q is not None:
+            views["q_out"] = self.tmp_view(q.shape, q.dtype)
+        if cos is not None and self._strides(cos, 1) != self._strides(views["sin"], 1):
+            views["cos"], views["sin"] = (self.materialize(views[n], out=self.tmp_view(views[n].shape, views[n].dtype)) for n in ("cos", "sin"))
+            cos = views["cos"]
+        ints = [E.dt_code(k.dtype), E.dt_code(kc.dtype), E.dt_code(cos.dtype) if cos is not None else 0, tokens,
+                views["page_table"].shape[0], q.shape[1] if q is not None else 0, hkv, d,
+                2 * cos.shape[1] if cos is not None else 0, cos.shape[0] if cos is not None else 0,
+                self._strides(cos, 1)[0] if cos is not None else 0, op.attributes["pos_offset"]]
+        ints += self._strides(k, 2) + self._strides(views["v"], 2)
+        ints += self._strides(q, 2) + self._strides(views["q_out"], 2) if q is not None else [0] * 4
+        ints += [kc.shape[0], kc.shape[1]] + self._strides(kc, 3) + self._strides(views["v_cache"], 3)
+        ints += [views["page_table"].shape[1], views["page_table"].shape[1]]
+        order = ["k", "v", "q", "q_out", "k_cache", "v_cache", "page_table", "kv_len", "q_start", "cos", "sin"]
+        self.serving_step("paged_append", op, order, views, ints, note=f"{tokens} tokens, {hkv} x {d}")
+        self.tuples[op.id] = (kc, views["v_cache"], views.get("q_out"))
+
+    def op_paged_attention(self, op):
+        """``paged-attention``: one ``paged_attention`` launch (its workspace a plan buffer)."""
+        from nkipy_b200.runtime.serving import attention_workspace
+
+        t = dict(zip(op.attributes["operands"], op.operands))
+        views = {n: self.rows_view(t[n]) for n in ("q", "k_cache", "v_cache")}
+        for n in ("page_table", "kv_len", "q_start", "prefix_pages"):
+            if n in t:
+                views[n] = self.materialize(self.get(t[n]), dense=True)
+        q, kc = views["q"], views["k_cache"]
+        out = views["out"] = self.tmp_view(q.shape, q.dtype)
+        tokens, hq, d = q.shape
+        a = op.attributes
+        ints = [E.dt_code(q.dtype), tokens, views["page_table"].shape[0], hq, kc.shape[2], d]
+        ints += self._strides(q, 2) + self._strides(out, 2) + [kc.shape[0], kc.shape[1]]
+        ints += self._strides(kc, 3) + self._strides(views["v_cache"], 3)
+        ints += [views["page_table"].shape[1], views["page_table"].shape[1], a["window"], a["sinks"], a["prefix_len"]]
+        need = attention_workspace(ints, "q_start" in t)
+        if need:
+            views["workspace"] = V.View(self.new_buf("tmp", -1, need), 0, (need,), (1,), np.dtype(np.uint8))
+        order = ["q", "out", "k_cache", "v_cache", "page_table", "kv_len", "q_start", "prefix_pages", "workspace"]
+        self.serving_step("paged_attention", op, order, views, ints + [need], [a["scale"]],
+                          note=f"{tokens} tokens, {hq}/{kc.shape[2]} x {d} window={a['window']} prefix={a['prefix_len']}")
+        self.vals[("o", op.id)] = out
+
+    def op_sample_tokens(self, op):
+        """``sample-tokens``: one ``sample_tokens`` launch."""
+        t = dict(zip(op.attributes["operands"], op.operands))
+        views = {n: self.materialize(self.get(x), dense=True) for n, x in t.items() if n != "logits"}
+        x = views["logits"] = self.rows_view(t["logits"])
+        out = views["tokens"] = self.tmp_view(op.result_shape, op.result_dtype)
+        order = ["logits", "u", "temperature", "top_k", "top_p", "min_p", "tokens"]
+        self.serving_step("sample_tokens", op, order, views, [E.dt_code(x.dtype), x.shape[0], x.shape[1]] + self._strides(x, 1),
+                          note=f"{x.shape[0]} x {x.shape[1]}")
+        self.vals[("o", op.id)] = out
+
     def op_get_tuple_element(self, op):
         src = op.operands[0].source_op
         if src is None or src.id not in self.tuples:

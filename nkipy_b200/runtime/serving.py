@@ -102,13 +102,18 @@ def _ptr(t):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace(device, *sizes):
-    """Workspace bytes of an attention call: by its sizes alone (positions in the struct as packed)."""
+def _workspace(tokens_by_start, *sizes):
     need = ctypes.c_size_t()
-    with torch.cuda.device(device):
-        _nkb.check(_nkb.lib().nkb_paged_attention_workspace(
-            _ATTENTION.pack(*([0] * 6), sizes[-1], *([0] * 2), *sizes[:-1], 0, 1.0), need))
+    _nkb.check(_nkb.lib().nkb_paged_attention_workspace(
+        _ATTENTION.pack(*([0] * 6), int(tokens_by_start), 0, 0, *sizes, 0, 1.0), need))
     return need.value
+
+
+def attention_workspace(sizes, tokens_by_start) -> int:
+    """Workspace bytes of an attention call: ``sizes`` are the integers of
+    ``nkb_paged_attention_args`` up to ``prefix_len``, ``tokens_by_start`` whether
+    ``q_start`` is given."""
+    return _workspace(bool(tokens_by_start), *(int(n) for n in sizes))
 
 
 def _launch(fn, packed, device):
@@ -191,7 +196,7 @@ def _attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, 
     qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
     sizes = (code, tokens, seqs, hq, hkv, d, qs[0], qs[1], os_[0], os_[1], pages, page_size, kc[0], kc[1], kc[2], vc[0],
              vc[1], vc[2], width, table_stride, window, sinks, prefix_len)
-    need = _workspace(device, *sizes, q_start is not None)
+    need = _workspace(q_start is not None, *sizes)
     room = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(_nkb.lib().nkb_paged_attention, _ATTENTION.pack(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(),

@@ -301,6 +301,46 @@ def greedy_sampling_kernel(h, norm_weight, lm_head_weight, max_batch_size=1, nor
     return final_next_id
 
 
+# ---------------------------------------------------------------------------
+# 7. A serving step over a paged KV cache
+# ---------------------------------------------------------------------------
+def paged_step_kernel(
+    x, norm_weight, qkv_weight, o_weight, head_weight, cache_k, cache_v, page_table, kv_len, cos, sin, u, temperature,
+    top_k, top_p, min_p, q_start=None, last=None, prefix_pages=None, prefix_len=0, n_heads=4, n_kv_heads=2, window=0,
+    sinks=0, eps=1e-6,
+):
+    """One served step of an attention block and its sampling head over ragged
+    sequences in pages: RMSNorm, QKV projection, keys and queries rotated and the
+    new rows appended (the caches are mutated in place), attention through the
+    page table (all keys, a window with first tokens, or a shared prefix),
+    o-projection with the residual, logits and the drawn tokens.  ``x`` holds the
+    new tokens of all sequences, (tokens, hidden); with ``q_start`` a prompt chunk
+    per sequence, and ``last`` (sequences,) the index of each one's last token,
+    the only ones that draw.  Where a prefix is shared, ``kv_len`` counts what
+    follows it and positions go on after it."""
+    from nkipy_b200.core import tensor_apis
+
+    tokens = x.shape[0]
+    d = cache_k.shape[3]
+    h = qk_rmsnorm(x, norm_weight, eps)
+    q, k, v = np.split((h @ qkv_weight).astype(x.dtype), [n_heads * d, (n_heads + n_kv_heads) * d], axis=-1)
+    q = q.reshape(tokens, n_heads, d)
+    k = k.reshape(tokens, n_kv_heads, d)
+    v = v.reshape(tokens, n_kv_heads, d)
+    q = tensor_apis.paged_append(k, v, cache_k, cache_v, page_table, kv_len, q_start=q_start, q=q, cos=cos, sin=sin,
+                                 pos_offset=prefix_len)
+    if prefix_len:
+        attn = tensor_apis.prefix_attention(q, cache_k, cache_v, prefix_pages, prefix_len, page_table, kv_len,
+                                            q_start=q_start)
+    else:
+        attn = tensor_apis.paged_attention(q, cache_k, cache_v, page_table, kv_len, q_start=q_start, window=window,
+                                           sinks=sinks)
+    y = x + attn.reshape(tokens, n_heads * d) @ o_weight
+    if last is not None:
+        y = np.take(y, last, axis=0)
+    return tensor_apis.sample_tokens((y @ head_weight).astype(x.dtype), u, temperature, top_k, top_p, min_p)
+
+
 def rope_tables(seq_len, head_dim, theta=500000.0):
     """cos/sin tables (S, head_dim/2), as ``qwen3_embedding/kernels/rope.py:4-31``."""
     inv_freq = 1.0 / (theta ** (np.arange(0, head_dim, 2, dtype=np.float32) / head_dim))
