@@ -18,13 +18,17 @@
 //   9      one thread issues the products, in the order S_A(0) S_B(0), then per
 //          block PV_A(c) S_A(c+1) PV_B(c) S_B(c+1), so one tile's softmax
 //          overlaps the other's products; it owns the TMEM;
+//   10     walks the CTA's share and hands its segments to the others through a
+//          small ring, ahead of them;
 //   0-3, 4-7  softmax of tile A and of tile B, one thread per row: scores from
 //          TMEM, mask, running maximum (raised only when it grows by more than
 //          2^8, O is then scaled in TMEM), exp2, P as 16-bit pairs over the
-//          scores; at a segment's end O / l to memory, or the partial.
+//          scores, handed over in two halves; at a segment's end O / l to
+//          memory, or the partial.
 // Keys that no row of the CTA sees may hold anything (another sequence's rows,
-// infinities, NaN): their scores are replaced, and their V rows are set to zero
-// in shared memory before the product that would multiply them by zero.
+// infinities, NaN): their scores are replaced; pages of which no key is seen are
+// not read (TMA fills zeros), and the unseen V rows of the others are set to
+// zero in shared memory before the product that would multiply them by zero.
 // TMEM: S_A S_B O_A O_B, 128 columns each.  Every wait is bounded.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
@@ -37,7 +41,11 @@ using namespace sm100;
 
 using namespace several;
 
-constexpr int W_PROD = 8, W_MMA = 9, THREADS = 320;
+constexpr int W_PROD = 8, W_MMA = 9, W_WALK = 10, THREADS = 384;
+// registers: 168 a thread at launch, moved from the last four warps to the
+// softmax warps (8 x 208 + 4 x 88 = 12 x 168)
+constexpr int REGS_SOFTMAX = 208, REGS_REST = 88;
+constexpr int RING = 4;  // segments
 constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 columns, 128-byte swizzle
 constexpr uint32_t T_S = 0, T_O = 256, TMEM_COLS = 512;
 constexpr float RESCALE = 8.f;  // log2 headroom before the running maximum is raised
@@ -48,7 +56,8 @@ template <int DP>
 struct Cfg {
   static constexpr int HALVES = DP / 64, TILE = HALVES * HALF, STAGES = DP == 128 ? 2 : 4;
   static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
-  static constexpr int SMEM = 1024 + OFF_BAR + 256;
+  static constexpr int OFF_ITEMS = OFF_BAR + 320;
+  static constexpr int SMEM = 1024 + OFF_ITEMS + RING * 64;
   static constexpr int SLOT = slot_floats(DP);
 };
 
@@ -148,11 +157,6 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
 __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
   return __all_sync(0xffffffffu, wait(bar, parity, abort_flag));
 }
-__device__ __forceinline__ uint64_t desc_k(uint32_t base, int kk) {
-  return smem_desc(base + (kk >> 2) * HALF + (kk & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int kk) { return smem_desc(base + kk * 2048, HALF, 1024); }
-
 // instruction descriptor, kind::f16, fp32 accumulator: both operands bf16 or both fp16
 template <class T>
 __device__ __forceinline__ constexpr uint32_t idesc(int M, int N, int b_mn_major) {
@@ -160,6 +164,52 @@ __device__ __forceinline__ constexpr uint32_t idesc(int M, int N, int b_mn_major
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
 }
+
+// A segment as the roles need it.
+struct Item {
+  int seq, tok0, ntok, pos0, hk;
+  int end, low, ns, w0;  // Blocks
+  int k0, n;             // first block, number of blocks; n = 0: the share is done
+  int nb[2];             // blocks that each tile needs
+  int final, slot;
+};
+
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two fp32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// Descriptors whose address part moves by a constant.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ explicit Desc(uint64_t d) : lo((uint32_t)d), hi((uint32_t)(d >> 32)) {}
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo + (bytes >> 4)), "r"(hi));
+    return r;
+  }
+};
 
 template <class T, int DP>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -170,10 +220,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
-  uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_ready = bars + 4, *o_done = bars + 6,
-           *o_free = bars + 8, *k_full = bars + 10, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+  uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_half = bars + 4, *p_ready = bars + 6,
+           *o_done = bars + 8, *o_free = bars + 10, *i_full = bars + 12, *i_empty = i_full + RING, *k_full = i_empty + RING,
+           *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_empty + ST);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  Item *ring = reinterpret_cast<Item *>(smem + C::OFF_ITEMS);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Args &a = p.a;
 
@@ -182,9 +234,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], BM);
       mbar_init(&p_ready[t], BM);
       mbar_init(&o_done[t], 1);
       mbar_init(&o_free[t], BM);
+    }
+    for (int s = 0; s < RING; ++s) {
+      mbar_init(&i_full[s], 1);
+      mbar_init(&i_empty[s], 10);  // producer, issuer, eight softmax warps
     }
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
@@ -207,96 +264,142 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();
-  Walk walk(p, blockIdx.x);
-  Segment s;
   bool ok = true;
+  uint32_t items = 0;  // segments taken so far
+  // the next segment, from the ring (whole warps, or one thread for the issuer)
+  auto take = [&](Item &x, bool whole_warp) {
+    const int i = items % RING;
+    ok = whole_warp ? wait_warp(&i_full[i], (items / RING) & 1, abort_flag) : wait(&i_full[i], (items / RING) & 1, abort_flag);
+    if (!ok) return false;
+    x = ring[i];
+    if (whole_warp) __syncwarp();
+    if (!whole_warp || lane == 0) mbar_arrive(&i_empty[i]);
+    ++items;
+    return x.n > 0;
+  };
+  auto block_of = [](const Item &x, int i) { return i < x.ns ? i : x.w0 + i - x.ns; };
 
-  if (warp == W_PROD) {
-    // ---------------- TMA producer ----------------
-    const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
-    uint32_t segs = 0, blk = 0;
-    while (ok && walk.next(s)) {
-      const int32_t *table = s.x.seq < 0 ? a.prefix_pages : a.page_table + s.x.seq * a.table_stride;
-      // page of this lane's part of block i; one past the cache (zeros) where there is none
-      auto page_of = [&](int i) {
-        const int64_t key = (int64_t)s.k.block(i) * BN + lane * box;
-        int id = -1;
-        if (i < s.k1 && lane < npb && key < s.k.end) id = table[key >> p.page_shift];
-        return paged::page_ok(id, a.pages) ? id : (int)a.pages;
-      };
-      int next = page_of(s.k0);
-      if (!wait_warp(q_empty, (segs & 1) ^ 1, abort_flag)) break;
-      if (lane == 0) {
-        const int tiles = s.x.ntok > p.P ? 2 : 1;
-        mbar_expect_tx(q_full, tiles * C::HALVES * 128 * p.G * p.P);
-        for (int t = 0; t < tiles; ++t)
-          for (int j = 0; j < C::HALVES; ++j)
-            tma_load_4d(smem + t * C::TILE + j * HALF, &mq, q_full, j * 64, 0, s.hk, s.x.tok0 + t * p.P);
-      }
-      ++segs;
-      for (int i = s.k0; i < s.k1; ++i, ++blk) {
-        const int st = blk % ST, page = next;
-        const uint32_t par = ((blk / ST) & 1) ^ 1;
-        const int slot = (s.k.block(i) * BN + lane * box) & (ps - 1);
-        next = page_of(i + 1);
-        uint8_t *kt = smem + C::OFF_K + st * C::TILE + lane * box * 128, *vt = smem + C::OFF_V + st * C::TILE + lane * box * 128;
-        if (!(ok = wait_warp(&k_empty[st], par, abort_flag))) break;
-        if (lane == 0) mbar_expect_tx(&k_full[st], C::TILE);
+  if (warp >= W_PROD) {
+    regs_dec<REGS_REST>();
+    if (warp == W_WALK) {
+      // ---------------- segments of this CTA's share ----------------
+      Walk walk(p, blockIdx.x);
+      Segment s;
+      while (true) {
+        const bool more = walk.next(s, lane);
+        const int i = items % RING;
+        if (!wait_warp(&i_empty[i], ((items / RING) & 1) ^ 1, abort_flag)) break;
+        if (lane == 0) {
+          Item x;
+          x.n = 0;
+          if (more) {
+            x = {s.x.seq, s.x.tok0, s.x.ntok, s.x.pos0, s.hk, s.k.end, s.k.low, s.k.ns, s.k.w0, s.k0, s.k1 - s.k0, {0, 0},
+                 s.all && !p.keep, s.slot};
+            for (int t = 0; t < 2; ++t) x.nb[t] = max(0, min(x.n, tile_blocks(p, s.x, s.k, t) - s.k0));
+          }
+          ring[i] = x;
+          mbar_arrive(&i_full[i]);
+        }
         __syncwarp();
-        if (lane < npb)
-          for (int j = 0; j < C::HALVES; ++j) tma_load_4d(kt + j * HALF, &mk, &k_full[st], j * 64, slot, s.hk, page);
-        if (!(ok = wait_warp(&v_empty[st], par, abort_flag))) break;
-        if (lane == 0) mbar_expect_tx(&v_full[st], C::TILE);
-        __syncwarp();
-        if (lane < npb)
-          for (int j = 0; j < C::HALVES; ++j) tma_load_4d(vt + j * HALF, &mv, &v_full[st], j * 64, slot, s.hk, page);
+        ++items;
+        if (!more) break;
       }
-    }
-  } else if (warp == W_MMA) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    } else if (warp == W_PROD) {
+      // ---------------- TMA producer ----------------
+      const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
+      uint32_t segs = 0, blk = 0;
+      Item x;
+      while (ok && take(x, true)) {
+        const int32_t *table = x.seq < 0 ? a.prefix_pages : a.page_table + x.seq * a.table_stride;
+        const int sinks = (int)min(a.sinks, (int64_t)x.end);
+        // page of this lane's part of block i; one past the cache (zeros) where no key of it is seen
+        auto page_of = [&](int i) {
+          const int64_t key = (int64_t)block_of(x, i) * BN + lane * box;
+          int id = -1;
+          if (i < x.k0 + x.n && lane < npb && key < x.end && (key + box > x.low || key < sinks)) id = table[key >> p.page_shift];
+          return paged::page_ok(id, a.pages) ? id : (int)a.pages;
+        };
+        int next = page_of(x.k0);
+        if (!(ok = wait_warp(q_empty, (segs & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          const int tiles = x.ntok > p.P ? 2 : 1;
+          mbar_expect_tx(q_full, tiles * C::HALVES * 128 * p.G * p.P);
+          for (int t = 0; t < tiles; ++t)
+            for (int j = 0; j < C::HALVES; ++j)
+              tma_load_4d(smem + t * C::TILE + j * HALF, &mq, q_full, j * 64, 0, x.hk, x.tok0 + t * p.P);
+        }
+        ++segs;
+        for (int i = x.k0; i < x.k0 + x.n; ++i, ++blk) {
+          const int st = blk % ST, page = next;
+          const uint32_t par = ((blk / ST) & 1) ^ 1;
+          const int slot = (block_of(x, i) * BN + lane * box) & (ps - 1);
+          next = page_of(i + 1);
+          uint8_t *kt = smem + C::OFF_K + st * C::TILE + lane * box * 128, *vt = smem + C::OFF_V + st * C::TILE + lane * box * 128;
+          if (!(ok = wait_warp(&k_empty[st], par, abort_flag))) break;
+          if (lane == 0) mbar_expect_tx(&k_full[st], C::TILE);
+          __syncwarp();
+          if (lane < npb)
+            for (int j = 0; j < C::HALVES; ++j) tma_load_4d(kt + j * HALF, &mk, &k_full[st], j * 64, slot, x.hk, page);
+          if (!(ok = wait_warp(&v_empty[st], par, abort_flag))) break;
+          if (lane == 0) mbar_expect_tx(&v_full[st], C::TILE);
+          __syncwarp();
+          if (lane < npb)
+            for (int j = 0; j < C::HALVES; ++j) tma_load_4d(vt + j * HALF, &mv, &v_full[st], j * 64, slot, x.hk, page);
+        }
+      }
+    } else if (warp == W_MMA && lane == 0) {
+      // ---------------- MMA issuer ----------------
       constexpr uint32_t ID_S = idesc<T>(128, BN, 0), ID_O = idesc<T>(128, DP, 1);
-      const uint32_t qs = smem_u32(smem), ks = smem_u32(smem + C::OFF_K), vs = smem_u32(smem + C::OFF_V);
+      const Desc dq(smem_desc(smem_u32(smem), 16, 1024)), dk(smem_desc(smem_u32(smem + C::OFF_K), 16, 1024)),
+          dv(smem_desc(smem_u32(smem + C::OFF_V), HALF, 1024));
       uint32_t segs = 0, blk = 0, cnt[2] = {0, 0}, outs[2] = {0, 0};
-      while (ok && walk.next(s)) {
-        const int n = s.k1 - s.k0;
-        int nb[2];
-        for (int t = 0; t < 2; ++t) nb[t] = max(0, min(n, tile_blocks(p, s.x, s.k, t) - s.k0));
+      Item x;
+      while (ok && take(x, false)) {
+        const int n = x.n;
         auto qk = [&](int t, int c) {  // S_t = Q_t K_c^T
-          const uint32_t kt = ks + ((blk + c) % ST) * C::TILE, qt = qs + t * C::TILE;
+          const Desc k(dk.at(((blk + c) % ST) * C::TILE)), q(dq.at(t * C::TILE));
 #pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) umma_f16(tmem + T_S + t * 128, desc_k(qt, kk), desc_k(kt, kk), ID_S, kk > 0);
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
+            umma_f16(tmem + T_S + t * 128, q.at(off), k.at(off), ID_S, kk > 0);
+          }
           umma_commit(&s_full[t]);
         };
-        auto pv = [&](int t, int c) {  // O_t += P_t V_c
-          const uint32_t vt = vs + ((blk + c) % ST) * C::TILE;
+        auto pv = [&](int t, int c, int half) {  // O_t += P_t V_c, 64 keys of the block
+          const Desc v(dv.at(((blk + c) % ST) * C::TILE));
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_f16_ts(tmem + T_O + t * 128, tmem + T_S + t * 128 + kk * 8, desc_mn(vt, kk), ID_O, (c > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&o_done[t]);
+          for (int kk = 0; kk < BN / 32; ++kk) {
+            const int k = half * (BN / 32) + kk;
+            umma_f16_ts(tmem + T_O + t * 128, tmem + T_S + t * 128 + k * 8, v.at(k * 2048), ID_O, (c > 0 || k > 0) ? 1u : 0u);
+          }
         };
         auto k_wait = [&](int c) { return wait(&k_full[(blk + c) % ST], ((blk + c) / ST) & 1, abort_flag); };
         if (!(ok = wait(q_full, segs & 1, abort_flag) && k_wait(0))) break;
         ++segs;
         tc_fence_after();
         for (int t = 0; t < 2; ++t)
-          if (nb[t] > 0) qk(t, 0);
+          if (x.nb[t] > 0) qk(t, 0);
         umma_commit(&k_empty[blk % ST]);
         if (n == 1) umma_commit(q_empty);
         for (int c = 0; ok && c < n; ++c) {
           const bool more = c + 1 < n;
           if (!(ok = wait(&v_full[(blk + c) % ST], ((blk + c) / ST) & 1, abort_flag) && (!more || k_wait(c + 1)))) break;
+#pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (c < nb[t]) {
-              // P of block c is written; before a segment's first product, O of the segment before is read
-              if (!(ok = wait(&p_ready[t], cnt[t] & 1, abort_flag) &&
+            if (c < x.nb[t]) {
+              // half of P of block c is written; before a segment's first product, O of the segment before is read
+              if (!(ok = wait(&p_half[t], cnt[t] & 1, abort_flag) &&
                          (c > 0 || outs[t] == 0 || wait(&o_free[t], (outs[t] - 1) & 1, abort_flag))))
                 break;
               tc_fence_after();
-              pv(t, c);
+              pv(t, c, 0);
+              if (!(ok = wait(&p_ready[t], cnt[t] & 1, abort_flag))) break;
+              tc_fence_after();
+              pv(t, c, 1);
+              umma_commit(&o_done[t]);
               ++cnt[t];
             }
-            if (c + 1 < nb[t]) qk(t, c + 1);
+            if (c + 1 < x.nb[t]) qk(t, c + 1);
           }
           if (!ok) break;
           if (more) {
@@ -306,33 +409,36 @@ __global__ void __launch_bounds__(THREADS, 1)
           umma_commit(&v_empty[(blk + c) % ST]);
         }
         blk += n;
-        for (int t = 0; t < 2; ++t) outs[t] += nb[t] > 0;
+        for (int t = 0; t < 2; ++t) outs[t] += x.nb[t] > 0;
       }
     }
   } else {
     // ---------------- softmax and results: tile t, row r ----------------
+    regs_inc<REGS_SOFTMAX>();
     const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t rows = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_col = rows + T_S + t * 128, o_col = rows + T_O + t * 128;
     const int g = r % p.G, tok = t * p.P + r / p.G;  // query head in the group, token in the pair
+    const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2);
     uint32_t blk = 0, cnt = 0;
-    while (ok && walk.next(s)) {
-      const int n = s.k1 - s.k0, nb = max(0, min(n, tile_blocks(p, s.x, s.k, t) - s.k0));
-      const bool row_ok = r < p.P * p.G && tok < s.x.ntok;
+    Item x;
+    while (ok && take(x, true)) {
+      const int nb = x.nb[t];
+      const bool row_ok = r < p.P * p.G && tok < x.ntok;
       // keys that the row sees: [lo, hi), and below `first`
       int hi = 0, lo = 0, first = 0;
       if (row_ok) {
-        const int64_t pos = (int64_t)s.x.pos0 + tok;
-        hi = s.x.seq < 0 ? s.k.end : (int)max((int64_t)0, min(pos + 1, (int64_t)s.k.end));
-        if (s.x.seq >= 0 && a.window > 0) {
+        const int64_t pos = (int64_t)x.pos0 + tok;
+        hi = x.seq < 0 ? x.end : (int)max((int64_t)0, min(pos + 1, (int64_t)x.end));
+        if (x.seq >= 0 && a.window > 0) {
           lo = (int)min(max((int64_t)0, pos - a.window + 1), (int64_t)hi);
           first = (int)min(a.sinks, (int64_t)hi);
         }
       }
-      const int all_lo = s.k.low, all_first = (int)min(a.sinks, (int64_t)s.k.end);
+      const int all_first = (int)min(a.sinks, (int64_t)x.end);
       float m = -INFINITY, l = 0.f;  // running (possibly stale) maximum in log2 units, and sum
       for (int c = 0; c < nb; ++c, ++cnt) {
-        const int key0 = s.k.block(s.k0 + c) * BN;
+        const int key0 = block_of(x, x.k0 + c) * BN;
         if (!(ok = wait_warp(&s_full[t], cnt & 1, abort_flag))) break;
         tc_fence_after();
         uint32_t v[128];
@@ -340,28 +446,40 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int i = 0; i < 4; ++i) tmem_ld32_nw(s_col + i * 32, v + i * 32);
         tmem_ld_wait();
         if (__any_sync(0xffffffffu, key0 + BN > hi || (key0 < lo && key0 + BN > first))) {
+          // a bit per key: below hi, and from lo or below first
           const int h = hi - key0, w = lo - key0, f = first - key0;
+          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (j >= h || (j < w && j >= f)) v[j] = 0xff800000u;
-        }
-        if (key0 + BN > s.k.end || (key0 < all_lo && key0 + BN > all_first)) {
-          // rows of V that no token of the pair sees: zeros
-          const uint32_t b = blk + c;
-          if (!(ok = wait_warp(&v_full[b % ST], (b / ST) & 1, abort_flag))) break;
-          const int key = key0 + r;
-          if (key >= s.k.end || (key < all_lo && key >= all_first)) {
-            uint8_t *row = smem + C::OFF_V + (b % ST) * C::TILE + r * 128;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bits = below(h - 32 * i) & (~below(w - 32 * i) | below(f - 32 * i));
 #pragma unroll
-            for (int j = 0; j < C::HALVES; ++j)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(row + j * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < 32; ++j)
+              if (!(bits >> j & 1)) v[32 * i + j] = 0xff800000u;
           }
-          fence_proxy_async_smem();
+        }
+        if (key0 + BN > x.end || (key0 < x.low && key0 + BN > all_first)) {
+          // rows of V that no token of the pair sees: zeros
+          const int key = key0 + r;
+          const bool unseen = key >= x.end || (key < x.low && key >= all_first);
+          if (__any_sync(0xffffffffu, unseen)) {
+            const uint32_t b = blk + c;
+            if (!(ok = wait_warp(&v_full[b % ST], (b / ST) & 1, abort_flag))) break;
+            if (unseen) {
+              uint8_t *row = smem + C::OFF_V + (b % ST) * C::TILE + r * 128;
+#pragma unroll
+              for (int j = 0; j < C::HALVES; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(row + j * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 128; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(v[j]));
+        for (int j = 0; j < 128; j += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mx4[i] = max3(mx4[i], __uint_as_float(v[j + 2 * i]), __uint_as_float(v[j + 2 * i + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         mx = mx == -INFINITY ? -INFINITY : mx * p.scale_log2;
         const bool raise = mx > m + RESCALE;
@@ -385,32 +503,40 @@ __global__ void __launch_bounds__(THREADS, 1)
           m = m_new;
         }
         const float mm = m == -INFINITY ? 0.f : m;
-        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t base2 = pair2(-mm, -mm);
+        uint64_t l2[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 128; j += 2) {
-          const float e0 = ex2(fmaf(__uint_as_float(v[j]), p.scale_log2, -mm));
-          const float e1 = ex2(fmaf(__uint_as_float(v[j + 1]), p.scale_log2, -mm));
-          l4[(j >> 1) & 3] += e0 + e1;
-          v[j / 2] = pack<T>(e0, e1);
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int j = half * 64; j < half * 64 + 64; j += 2) {
+            float e0, e1;
+            unpair2(fma2(pair2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, base2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            l2[(j >> 1) & 1] = add2(l2[(j >> 1) & 1], pair2(e0, e1));
+            v[j / 2] = pack<T>(e0, e1);
+          }
+          tmem_st16(s_col + half * 32, v + half * 32);
+          tmem_st16(s_col + half * 32 + 16, v + half * 32 + 16);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(half ? &p_ready[t] : &p_half[t]);
         }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_st16(s_col + i * 16, v + i * 16);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_ready[t]);
+        float s0, s1, s2, s3;
+        unpair2(l2[0], s0, s1);
+        unpair2(l2[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
       }
       if (!ok) break;
-      blk += n;
+      blk += x.n;
       if (nb > 0) {
         if (!(ok = wait_warp(&o_done[t], (cnt - 1) & 1, abort_flag))) break;
         tc_fence_after();
       }
-      const bool final = s.all && !p.keep;
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int D = (int)a.head_dim, token = s.x.tok0 + tok;
-      T *dst = static_cast<T *>(a.out) + token * a.out_token + (s.hk * p.G + g) * a.out_head;
-      float *part = p.ws + (int64_t)s.slot * C::SLOT;
+      const int D = (int)a.head_dim, token = x.tok0 + tok;
+      T *dst = static_cast<T *>(a.out) + token * a.out_token + (x.hk * p.G + g) * a.out_head;
+      float *part = p.ws + (int64_t)x.slot * C::SLOT;
 #pragma unroll 1
       for (int i = 0; i < DP / 32; ++i) {
         uint32_t o[32];
@@ -421,7 +547,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0;
         }
-        if (row_ok && final) {
+        if (row_ok && x.final) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 w;
@@ -437,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             *reinterpret_cast<uint4 *>(part + (t * BM + r) * DP + i * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
       }
-      if (row_ok && !final) *reinterpret_cast<float2 *>(part + 2 * BM * DP + 2 * (t * BM + r)) = make_float2(m, l);
+      if (row_ok && !x.final) *reinterpret_cast<float2 *>(part + 2 * BM * DP + 2 * (t * BM + r)) = make_float2(m, l);
       __syncwarp();
       if (nb > 0) {
         tc_fence_before();
@@ -474,7 +600,7 @@ __global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ 
   if (c >= walk.ctas) return;
   const int64_t cut = share(walk.total, c, walk.ctas);
   Segment s;
-  walk.locate(cut, s);
+  walk.locate(cut, s, threadIdx.x % 32);
   const int64_t first = cut - s.k0;
   if (s.k0 == 0) return;  // the share begins with the unit
   const Parts parts = parts_of(walk.total, first, s.k.n, p.max_ctas, 0);

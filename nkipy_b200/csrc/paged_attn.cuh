@@ -259,25 +259,39 @@ struct Walk {
     f1 = c < ctas ? share(total, c + 1, ctas) : 0;
     f = f0;
   }
-  // unit that holds block f
-  __device__ __forceinline__ void locate(int64_t at, Segment &s) const {
+  // unit that holds block `at`: a whole warp looks, 32 pivots at a time
+  __device__ __forceinline__ void locate(int64_t at, Segment &s, int lane) const {
     const int64_t row = at / p.a.kv_heads;  // pairs are kv_heads * n blocks long
-    int lo = 0, hi = (int)p.head[0] - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (p.head[1 + mid] <= row) lo = mid;
-      else hi = mid - 1;
+    int lo = 0, n = (int)p.head[0];
+    while (n > 1) {
+      const int step = (n + 31) / 32, i = lane * step;
+      const uint32_t m = __ballot_sync(0xffffffffu, i < n && p.head[1 + lo + min(i, n - 1)] <= row);
+      const int last = 31 - __clz(m | 1u);
+      lo += last * step;
+      n = min(step, n - last * step);
     }
-    s.u = lo;
-    s.x = p.pairs[lo];
-    s.k = blocks_of(p, s.x);
-    const int64_t in = at - p.head[1 + lo] * p.a.kv_heads;
-    s.hk = (int)(in / s.k.n);
-    s.k0 = (int)(in - (int64_t)s.hk * s.k.n);
+    set(lo, s);
+    const int in = (int)(at - p.head[1 + lo] * p.a.kv_heads);
+    s.hk = in / s.k.n;
+    s.k0 = in - s.hk * s.k.n;
   }
-  __device__ __forceinline__ bool next(Segment &s) {
+  __device__ __forceinline__ void set(int u, Segment &s) const {
+    s.u = u;
+    s.x = p.pairs[u];
+    s.k = blocks_of(p, s.x);
+  }
+  // the next segment of the share (a whole warp)
+  __device__ __forceinline__ bool next(Segment &s, int lane) {
     if (f >= f1) return false;
-    locate(f, s);
+    if (f == f0) {
+      locate(f, s, lane);
+    } else {  // a unit ended with the segment before
+      s.k0 = 0;
+      if (++s.hk == (int)p.a.kv_heads) {
+        s.hk = 0;
+        set(s.u + 1, s);
+      }
+    }
     s.k1 = (int)min((int64_t)s.k.n, s.k0 + (f1 - f));
     s.all = s.k0 == 0 && s.k1 == s.k.n;
     s.slot = s.all ? 2 * p.max_ctas + s.u * (int)p.a.kv_heads + s.hk : 2 * c + (f != f0);
