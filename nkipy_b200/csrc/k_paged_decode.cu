@@ -285,28 +285,15 @@ __global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_const
   const Parts parts = parts_of(total, first, nb, p.ctas, blockIdx.x);
   pdl_wait();  // in every block: the grid must not end before the one it follows
   if (parts.n == 1 && !p.keep) return;  // one CTA held it whole
-  const int n = parts.n;
-  auto slot = [&](int i) { return p.ws + (int64_t)parts.slot(i) * S::SLOT; };
   for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) M = fmaxf(M, __ldcg(slot(j) + ROWS * DP + 2 * r));
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(j) + ROWS * DP + 2 * r));
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(slot(j) + r * DP + d));
-      const float g = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L += ml.y * g;
-      x[0] += y.x * g;
-      x[1] += y.y * g;
-      x[2] += y.z * g;
-      x[3] += y.w * g;
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    if (d < D)
-      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + b * a.out_token + (h0 + r) * a.out_head + d) =
-          make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+    if (d >= D) continue;
+    Joined x;
+    x.add(parts.n, [&](int j) {
+      const float *slot = p.ws + (int64_t)parts.slot(j) * S::SLOT;
+      return Partial{slot + r * DP + d, slot + ROWS * DP + 2 * r};
+    });
+    x.store(static_cast<T *>(a.out) + b * a.out_token + (h0 + r) * a.out_head + d);
   }
 }
 

@@ -15,10 +15,6 @@ namespace {
 
 constexpr int THREADS = single::THREADS;
 
-struct Join {
-  const float *o, *ml;  // outputs of a row, and its (max, sum)
-};
-
 template <class T, int DP>
 __global__ void __launch_bounds__(THREADS)
     prefix_join_kernel(const __grid_constant__ several::Params p, const __grid_constant__ single::Params s) {
@@ -35,12 +31,11 @@ __global__ void __launch_bounds__(THREADS)
     const int64_t n = several::blocks_of(p, x).n;
     tok = t - x.tok0;
     seq = x.seq;
-    return parts_of(walk.total, p.head[1 + u] * a.kv_heads + hk * n, n, p.max_ctas, (int64_t)u * a.kv_heads + hk);
+    return walk.parts(u, hk, n);
   };
   int ptok, otok = 0, seq = 0;
   const Parts pre = unit_parts(t / per, ptok, seq);
   Parts own;
-  int own_row_group = 0;
   seq = 0;
   if (p.own) {  // the pair of this token among the sequences' own
     int lo = (int)((a.tokens + per - 1) / per), hi = (int)p.head[0] - 1;
@@ -61,33 +56,21 @@ __global__ void __launch_bounds__(THREADS)
     auto tile_part = [&](const Parts &x, int j, int tok) {
       const float *slot = p.ws + (int64_t)x.slot(j) * SLOT;
       const int row = tok / p.P * several::BM + tok % p.P * G + g;
-      return Join{slot + row * DP + d, slot + ML + 2 * row};
+      return Partial{slot + row * DP + d, slot + ML + 2 * row};
     };
-    auto part = [&](int j) {
-      if (j < pre.n) return tile_part(pre, j, ptok);
-      if (p.own) return tile_part(own, j - pre.n, otok);
-      const float *slot = s.ws + (int64_t)own.slot(j - pre.n) * S::SLOT;
-      const int row = g % single::ROWS;
-      return Join{slot + row * DP + d, slot + single::ROWS * DP + 2 * row};
-    };
-    const int n = seq == -2 ? 0 : pre.n + own.n;  // a token of no sequence sees nothing
-    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < n; ++j) M = fmaxf(M, __ldcg(part(j).ml));
-    for (int j = 0; j < n; ++j) {
-      const Join q = part(j);
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q.ml));
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(q.o));
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L += ml.y * f;
-      x[0] += y.x * f;
-      x[1] += y.y * f;
-      x[2] += y.z * f;
-      x[3] += y.w * f;
+    if (d >= D) continue;
+    Joined x;
+    if (seq != -2) {  // (a token of no sequence sees nothing)
+      x.add(pre.n, [&](int j) { return tile_part(pre, j, ptok); });
+      if (p.own) x.add(own.n, [&](int j) { return tile_part(own, j, otok); });
+      else
+        x.add(own.n, [&](int j) {
+          const float *slot = s.ws + (int64_t)own.slot(j) * S::SLOT;
+          const int row = g % single::ROWS;
+          return Partial{slot + row * DP + d, slot + single::ROWS * DP + 2 * row};
+        });
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    if (d < D)
-      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + t * a.out_token + (hk * G + g) * a.out_head + d) =
-          make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+    x.store(static_cast<T *>(a.out) + t * a.out_token + (hk * G + g) * a.out_head + d);
   }
 }
 

@@ -12,24 +12,24 @@
 // share's end is joined from partials by a second kernel.  Lengths are read on
 // the device: a small kernel lists the pairs first.
 //
-// Warps of a CTA:
-//   8      producer: TMA loads of Q (both tiles) and, page by page, of K and V
-//          into rings of stages that are released separately;
-//   9      one thread issues the products, in the order S_A(0) S_B(0), then per
-//          block PV_A(c) S_A(c+1) PV_B(c) S_B(c+1), so one tile's softmax
-//          overlaps the other's products; it owns the TMEM;
-//   10     walks the CTA's share and hands its segments to the others through a
-//          small ring, ahead of them;
+// A block is taken in two halves of 64 keys, each with its own score buffer, so
+// that the scores of the next half are there when a softmax ends: the softmax
+// warps wait for no product of their own half.  Warps of a CTA:
+//   8      walks the CTA's share, hands its segments to the others through a small
+//          ring, and produces: TMA loads of Q (both tiles) and, page by page, of
+//          K and V into rings of stages that are released separately;
+//   9, 10  one thread each issues the products of tile A and of tile B: S(0)
+//          S(1), then per half PV(h) S(h + 2); warp 9 owns the TMEM;
+//   11     sees to V: rows that no token of the pair sees become zeros;
 //   0-3, 4-7  softmax of tile A and of tile B, one thread per row: scores from
 //          TMEM, mask, running maximum (raised only when it grows by more than
 //          2^8, O is then scaled in TMEM), exp2, P as 16-bit pairs over the
-//          scores, handed over in two halves; at a segment's end O / l to
-//          memory, or the partial.
+//          scores; at a segment's end O / l to memory, or the partial.
 // Keys that no row of the CTA sees may hold anything (another sequence's rows,
 // infinities, NaN): their scores are replaced; pages of which no key is seen are
 // not read (TMA fills zeros), and the unseen V rows of the others are set to
 // zero in shared memory before the product that would multiply them by zero.
-// TMEM: S_A S_B O_A O_B, 128 columns each.  Every wait is bounded.
+// TMEM: two score buffers of 64 columns and O of up to 128 for each tile.  Every wait is bounded.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 
@@ -41,10 +41,8 @@ using namespace sm100;
 
 using namespace several;
 
-constexpr int W_PROD = 8, W_MMA = 9, W_WALK = 10, THREADS = 384;
-// registers: 168 a thread at launch, moved from the last four warps to the
-// softmax warps (8 x 208 + 4 x 88 = 12 x 168)
-constexpr int REGS_SOFTMAX = 208, REGS_REST = 88;
+constexpr int BH = 64;  // keys of a half
+constexpr int W_PROD = 8, W_MMA = 9, W_FIX = 11, THREADS = 384;
 constexpr int RING = 4;  // segments
 constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 columns, 128-byte swizzle
 constexpr uint32_t T_S = 0, T_O = 256, TMEM_COLS = 512;
@@ -56,7 +54,7 @@ template <int DP>
 struct Cfg {
   static constexpr int HALVES = DP / 64, TILE = HALVES * HALF, STAGES = DP == 128 ? 2 : 4;
   static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
-  static constexpr int OFF_ITEMS = OFF_BAR + 320;
+  static constexpr int OFF_ITEMS = OFF_BAR + 448;
   static constexpr int SMEM = 1024 + OFF_ITEMS + RING * 64;
   static constexpr int SLOT = slot_floats(DP);
 };
@@ -77,13 +75,15 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *total) {
   __syncthreads();
   if (lane == 31) s[warp] = x;
   __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int w = 0; w < SCHED / 32; ++w) {
-    if (w < warp) before += s[w];
-    all += s[w];
+  int64_t y = s[lane];  // the warps' sums, scanned by every warp
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const int64_t z = __shfl_up_sync(0xffffffffu, y, w);
+    if (lane >= w) y += z;
   }
-  *total = all;
-  return before + x - v;
+  *total = __shfl_sync(0xffffffffu, y, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
+  return (warp ? before : 0) + x - v;
 }
 
 // tokens of list entry i: those before the sequences, sequence i - 1, those after
@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Pa
     blocks += all;
   }
   if (threadIdx.x == 0) {
+    *p.next = p.max_ctas;  // the CTAs' first units are their own numbers
     p.head[0] = U;
     p.head[1 + U] = blocks;
   }
@@ -170,14 +171,9 @@ struct Item {
   int seq, tok0, ntok, pos0, hk;
   int end, low, ns, w0;  // Blocks
   int k0, n;             // first block, number of blocks; n = 0: the share is done
-  int nb[2];             // blocks that each tile needs
+  int nb_a, nb_b;        // blocks that each tile needs
   int final, slot;
 };
-
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Two fp32 values as one operand of the packed instructions.
 __device__ __forceinline__ uint64_t pair2(float lo, float hi) {
@@ -198,7 +194,54 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^y for two values on the FMA pipe: y = n + r with |r| <= 1/2, 2^r by its
+// minimax polynomial (least squares reweighted to an even relative error: 7.5e-5
+// for degree 3, 2.7e-6 for degree 4, a tenth of the rounding of P to bf16 and to
+// fp16), n added to the exponent.  y below -126 gives 2^-126.
+template <class T>
+__device__ __forceinline__ void exp2_poly(uint64_t y2, float &e0, float &e1) {
+  constexpr bool fine = std::is_same<T, __half>::value;
+  float y0, y1, t0, t1;
+  unpair2(y2, y0, y1);
+  y2 = pair2(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
+  const uint64_t t2 = add2(y2, pair2(12582912.f, 12582912.f));           // 1.5 * 2^23: n in the low bits
+  const uint64_t r2 = add2(y2, fma2(add2(t2, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), 0));
+  auto c = [](float x) { return pair2(x, x); };
+  uint64_t q;
+  if (fine) {
+    q = fma2(c(9.570101276040077e-3f), r2, c(5.591786280274391e-2f));
+    q = fma2(q, r2, c(0.240247443318367f));
+    q = fma2(q, r2, c(0.6931217908859253f));
+    q = fma2(q, r2, c(0.9999992847442627f));
+  } else {
+    q = fma2(c(5.51716610789299e-2f), r2, c(0.2426111400127411f));
+    q = fma2(q, r2, c(0.6932609677314758f));
+    q = fma2(q, r2, c(0.9999280571937561f));
+  }
+  unpair2(t2, t0, t1);
+  unpair2(q, e0, e1);
+  e0 = __int_as_float(__float_as_int(e0) + (__float_as_int(t0) << 23));
+  e1 = __int_as_float(__float_as_int(e1) + (__float_as_int(t1) << 23));
+}
+
+// 32 bytes of one row (a whole sector), or two halves where they are only
+// aligned to 16
+__device__ __forceinline__ void store32(void *p, const uint32_t *v, bool wide) {
+  if (wide)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  else {
+    static_cast<uint4 *>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    static_cast<uint4 *>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
 
 // Descriptors whose address part moves by a constant.
 struct Desc {
@@ -220,10 +263,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
-  uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_half = bars + 4, *p_ready = bars + 6,
-           *o_done = bars + 8, *o_free = bars + 10, *i_full = bars + 12, *i_empty = i_full + RING, *k_full = i_empty + RING,
-           *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_empty + ST);
+  // [tile][score buffer] where a tile has two
+  uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_ready = bars + 6, *o_done = bars + 10,
+           *o_free = bars + 14, *i_full = bars + 16, *i_empty = i_full + RING, *k_full = i_empty + RING,
+           *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *v_ready = v_empty + ST;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_ready + ST);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   Item *ring = reinterpret_cast<Item *>(smem + C::OFF_ITEMS);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -231,23 +275,25 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);  // both issuers
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], BM);
-      mbar_init(&p_ready[t], BM);
-      mbar_init(&o_done[t], 1);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&s_full[2 * t + j], 1);
+        mbar_init(&p_ready[2 * t + j], BM);
+        mbar_init(&o_done[2 * t + j], 1);
+      }
       mbar_init(&o_free[t], BM);
     }
     for (int s = 0; s < RING; ++s) {
       mbar_init(&i_full[s], 1);
-      mbar_init(&i_empty[s], 10);  // producer, issuer, eight softmax warps
+      mbar_init(&i_empty[s], 11);  // two issuers, V's warp, eight softmax warps
     }
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
+      mbar_init(&v_ready[s], 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -266,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_trigger();
   bool ok = true;
   uint32_t items = 0;  // segments taken so far
-  // the next segment, from the ring (whole warps, or one thread for the issuer)
+  // the next segment, from the ring (whole warps, or one thread for an issuer)
   auto take = [&](Item &x, bool whole_warp) {
     const int i = items % RING;
     ok = whole_warp ? wait_warp(&i_full[i], (items / RING) & 1, abort_flag) : wait(&i_full[i], (items / RING) & 1, abort_flag);
@@ -280,36 +326,30 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto block_of = [](const Item &x, int i) { return i < x.ns ? i : x.w0 + i - x.ns; };
 
   if (warp >= W_PROD) {
-    regs_dec<REGS_REST>();
-    if (warp == W_WALK) {
-      // ---------------- segments of this CTA's share ----------------
+    if (warp == W_PROD) {
+      // ---------------- segments of this CTA's share, TMA producer ----------------
+      const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
+      uint32_t segs = 0, blk = 0;
       Walk walk(p, blockIdx.x);
       Segment s;
-      while (true) {
+      while (ok) {
         const bool more = walk.next(s, lane);
-        const int i = items % RING;
-        if (!wait_warp(&i_empty[i], ((items / RING) & 1) ^ 1, abort_flag)) break;
+        const int slot_i = items % RING;
+        if (!(ok = wait_warp(&i_empty[slot_i], ((items / RING) & 1) ^ 1, abort_flag))) break;
+        Item x = {};
+        if (more) {
+          x = {s.x.seq, s.x.tok0, s.x.ntok, s.x.pos0, s.hk, s.k.end, s.k.low, s.k.ns, s.k.w0, s.k0, s.k1 - s.k0, 0, 0,
+               s.all && !p.keep, s.slot};
+          x.nb_a = max(0, min(x.n, tile_blocks(p, s.x, s.k, 0) - s.k0));
+          x.nb_b = max(0, min(x.n, tile_blocks(p, s.x, s.k, 1) - s.k0));
+        }
         if (lane == 0) {
-          Item x;
-          x.n = 0;
-          if (more) {
-            x = {s.x.seq, s.x.tok0, s.x.ntok, s.x.pos0, s.hk, s.k.end, s.k.low, s.k.ns, s.k.w0, s.k0, s.k1 - s.k0, {0, 0},
-                 s.all && !p.keep, s.slot};
-            for (int t = 0; t < 2; ++t) x.nb[t] = max(0, min(x.n, tile_blocks(p, s.x, s.k, t) - s.k0));
-          }
-          ring[i] = x;
-          mbar_arrive(&i_full[i]);
+          ring[slot_i] = x;
+          mbar_arrive(&i_full[slot_i]);
         }
         __syncwarp();
         ++items;
         if (!more) break;
-      }
-    } else if (warp == W_PROD) {
-      // ---------------- TMA producer ----------------
-      const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
-      uint32_t segs = 0, blk = 0;
-      Item x;
-      while (ok && take(x, true)) {
         const int32_t *table = x.seq < 0 ? a.prefix_pages : a.page_table + x.seq * a.table_stride;
         const int sinks = (int)min(a.sinks, (int64_t)x.end);
         // page of this lane's part of block i; one past the cache (zeros) where no key of it is seen
@@ -347,74 +387,102 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int j = 0; j < C::HALVES; ++j) tma_load_4d(vt + j * HALF, &mv, &v_full[st], j * 64, slot, x.hk, page);
         }
       }
-    } else if (warp == W_MMA && lane == 0) {
-      // ---------------- MMA issuer ----------------
-      constexpr uint32_t ID_S = idesc<T>(128, BN, 0), ID_O = idesc<T>(128, DP, 1);
-      const Desc dq(smem_desc(smem_u32(smem), 16, 1024)), dk(smem_desc(smem_u32(smem + C::OFF_K), 16, 1024)),
+    } else if (warp == W_FIX) {
+      // ---------------- V rows that no token of the pair sees ----------------
+      uint32_t blk = 0;
+      Item x;
+      while (ok && take(x, true)) {
+        const int sinks = (int)min(a.sinks, (int64_t)x.end);
+        for (int i = x.k0; i < x.k0 + x.n; ++i, ++blk) {
+          const int st = blk % ST, key0 = block_of(x, i) * BN;
+          if (!(ok = wait_warp(&v_full[st], (blk / ST) & 1, abort_flag))) break;
+          if (key0 + BN > x.end || (key0 < x.low && key0 + BN > sinks)) {
+            // four rows at a time, eight lanes on the 128 bytes of a row
+            for (int r = lane / 8; r < BN; r += 4) {
+              const int key = key0 + r;
+              if (key < x.end && (key >= x.low || key < sinks)) continue;
+              uint8_t *row = smem + C::OFF_V + st * C::TILE + r * 128 + lane % 8 * 16;
+#pragma unroll
+              for (int j = 0; j < C::HALVES; ++j) *reinterpret_cast<uint4 *>(row + j * HALF) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&v_ready[st]);
+        }
+      }
+    } else if (lane == 0) {
+      // ---------------- MMA issuer of tile t ----------------
+      constexpr uint32_t ID_S = idesc<T>(128, BH, 0), ID_O = idesc<T>(128, DP, 1);
+      const int t = warp - W_MMA;
+      const Desc dq(smem_desc(smem_u32(smem + t * C::TILE), 16, 1024)), dk(smem_desc(smem_u32(smem + C::OFF_K), 16, 1024)),
           dv(smem_desc(smem_u32(smem + C::OFF_V), HALF, 1024));
-      uint32_t segs = 0, blk = 0, cnt[2] = {0, 0}, outs[2] = {0, 0};
+      const uint32_t ts = tmem + T_S + t * 128, to = tmem + T_O + t * 128;
+      uint32_t segs = 0, blk = 0, cnt = 0, outs = 0;
       Item x;
       while (ok && take(x, false)) {
-        const int n = x.n;
-        auto qk = [&](int t, int c) {  // S_t = Q_t K_c^T
-          const Desc k(dk.at(((blk + c) % ST) * C::TILE)), q(dq.at(t * C::TILE));
+        const int n = x.n, nb = t ? x.nb_b : x.nb_a;
+        auto stage = [&](int c) { return (blk + c) % ST; };
+        auto full = [&](uint64_t *bar, int c) { return wait(&bar[stage(c)], ((blk + c) / ST) & 1, abort_flag); };
+        auto qk = [&](int c, int j) {  // S = Q K^T of half j of block c
+          const Desc k(dk.at(stage(c) * C::TILE + j * BH * 128));
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-            umma_f16(tmem + T_S + t * 128, q.at(off), k.at(off), ID_S, kk > 0);
+            umma_f16(ts + j * BH, dq.at(off), k.at(off), ID_S, kk > 0);
           }
-          umma_commit(&s_full[t]);
+          umma_commit(&s_full[2 * t + j]);
         };
-        auto pv = [&](int t, int c, int half) {  // O_t += P_t V_c, 64 keys of the block
-          const Desc v(dv.at(((blk + c) % ST) * C::TILE));
+        auto pv = [&](int c, int j) {  // O += P V
+          const Desc v(dv.at(stage(c) * C::TILE + j * BH * 128));
 #pragma unroll
-          for (int kk = 0; kk < BN / 32; ++kk) {
-            const int k = half * (BN / 32) + kk;
-            umma_f16_ts(tmem + T_O + t * 128, tmem + T_S + t * 128 + k * 8, v.at(k * 2048), ID_O, (c > 0 || k > 0) ? 1u : 0u);
-          }
+          for (int kk = 0; kk < BH / 16; ++kk)
+            umma_f16_ts(to, ts + j * BH + kk * 8, v.at(kk * 2048), ID_O, (c > 0 || j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&o_done[2 * t + j]);
         };
-        auto k_wait = [&](int c) { return wait(&k_full[(blk + c) % ST], ((blk + c) / ST) & 1, abort_flag); };
-        if (!(ok = wait(q_full, segs & 1, abort_flag) && k_wait(0))) break;
+        if (!(ok = wait(q_full, segs & 1, abort_flag) && full(k_full, 0))) break;
         ++segs;
         tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (x.nb[t] > 0) qk(t, 0);
-        umma_commit(&k_empty[blk % ST]);
+        if (nb > 0) {
+          qk(0, 0);
+          qk(0, 1);
+        }
+        umma_commit(&k_empty[stage(0)]);
         if (n == 1) umma_commit(q_empty);
-        for (int c = 0; ok && c < n; ++c) {
-          const bool more = c + 1 < n;
-          if (!(ok = wait(&v_full[(blk + c) % ST], ((blk + c) / ST) & 1, abort_flag) && (!more || k_wait(c + 1)))) break;
+        for (int c = 0; c < n; ++c) {
+          // a block that this tile does not need is waited for all the same: its stages are released in order
+          if (!(ok = full(v_ready, c))) break;
+          if (c < nb) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (c < x.nb[t]) {
-              // half of P of block c is written; before a segment's first product, O of the segment before is read
-              if (!(ok = wait(&p_half[t], cnt[t] & 1, abort_flag) &&
-                         (c > 0 || outs[t] == 0 || wait(&o_free[t], (outs[t] - 1) & 1, abort_flag))))
+            for (int j = 0; j < 2; ++j) {
+              // P of the half is written; before a segment's first product, O of the segment before is read
+              if (!(ok = wait(&p_ready[2 * t + j], cnt & 1, abort_flag) &&
+                         (c > 0 || j > 0 || outs == 0 || wait(&o_free[t], (outs - 1) & 1, abort_flag))))
                 break;
               tc_fence_after();
-              pv(t, c, 0);
-              if (!(ok = wait(&p_ready[t], cnt[t] & 1, abort_flag))) break;
-              tc_fence_after();
-              pv(t, c, 1);
-              umma_commit(&o_done[t]);
-              ++cnt[t];
+              pv(c, j);
+              if (c + 1 < nb) {
+                if (j == 0 && !(ok = full(k_full, c + 1))) break;
+                tc_fence_after();
+                qk(c + 1, j);
+              }
             }
-            if (c + 1 < x.nb[t]) qk(t, c + 1);
+            if (!ok) break;
+            ++cnt;
           }
-          if (!ok) break;
-          if (more) {
-            umma_commit(&k_empty[(blk + c + 1) % ST]);
+          umma_commit(&v_empty[stage(c)]);
+          if (c + 1 < n) {
+            if (c + 1 >= nb && !(ok = full(k_full, c + 1))) break;
+            umma_commit(&k_empty[stage(c + 1)]);
             if (c + 2 == n) umma_commit(q_empty);
           }
-          umma_commit(&v_empty[(blk + c) % ST]);
         }
         blk += n;
-        for (int t = 0; t < 2; ++t) outs[t] += x.nb[t] > 0;
+        outs += nb > 0;
       }
     }
   } else {
     // ---------------- softmax and results: tile t, row r ----------------
-    regs_inc<REGS_SOFTMAX>();
     const int t = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t rows = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_col = rows + T_S + t * 128, o_col = rows + T_O + t * 128;
@@ -423,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t blk = 0, cnt = 0;
     Item x;
     while (ok && take(x, true)) {
-      const int nb = x.nb[t];
+      const int nb = t ? x.nb_b : x.nb_a;
       const bool row_ok = r < p.P * p.G && tok < x.ntok;
       // keys that the row sees: [lo, hi), and below `first`
       int hi = 0, lo = 0, first = 0;
@@ -435,66 +503,55 @@ __global__ void __launch_bounds__(THREADS, 1)
           first = (int)min(a.sinks, (int64_t)hi);
         }
       }
-      const int all_first = (int)min(a.sinks, (int64_t)x.end);
       float m = -INFINITY, l = 0.f;  // running (possibly stale) maximum in log2 units, and sum
-      for (int c = 0; c < nb; ++c, ++cnt) {
-        const int key0 = block_of(x, x.k0 + c) * BN;
-        if (!(ok = wait_warp(&s_full[t], cnt & 1, abort_flag))) break;
+      for (int h = 0; h < 2 * nb; ++h, ++cnt) {
+        const int c = h >> 1, j = h & 1, key0 = block_of(x, x.k0 + c) * BN + j * BH;
+        const uint32_t sc = s_col + j * BH;
+        // the scores, and the product of the half before last: every phase of o_done is waited for in turn, so
+        // that the parity of a later wait (below) cannot be that of an older phase
+        if (!(ok = wait_warp(&s_full[2 * t + j], (cnt >> 1) & 1, abort_flag) &&
+                   (h < 2 || wait_warp(&o_done[2 * t + j], ((cnt >> 1) - 1) & 1, abort_flag))))
+          break;
         tc_fence_after();
-        uint32_t v[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_nw(s_col + i * 32, v + i * 32);
+        uint32_t v[BH];
+        tmem_ld32_nw(sc, v);
+        tmem_ld32_nw(sc + 32, v + 32);
         tmem_ld_wait();
-        if (__any_sync(0xffffffffu, key0 + BN > hi || (key0 < lo && key0 + BN > first))) {
+        const bool masked = __any_sync(0xffffffffu, key0 + BH > hi || (key0 < lo && key0 + BH > first));
+        if (masked) {
           // a bit per key: below hi, and from lo or below first
-          const int h = hi - key0, w = lo - key0, f = first - key0;
+          const int hk = hi - key0, w = lo - key0, f = first - key0;
           auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t bits = below(h - 32 * i) & (~below(w - 32 * i) | below(f - 32 * i));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t bits = below(hk - 32 * i) & (~below(w - 32 * i) | below(f - 32 * i));
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!(bits >> j & 1)) v[32 * i + j] = 0xff800000u;
-          }
-        }
-        if (key0 + BN > x.end || (key0 < x.low && key0 + BN > all_first)) {
-          // rows of V that no token of the pair sees: zeros
-          const int key = key0 + r;
-          const bool unseen = key >= x.end || (key < x.low && key >= all_first);
-          if (__any_sync(0xffffffffu, unseen)) {
-            const uint32_t b = blk + c;
-            if (!(ok = wait_warp(&v_full[b % ST], (b / ST) & 1, abort_flag))) break;
-            if (unseen) {
-              uint8_t *row = smem + C::OFF_V + (b % ST) * C::TILE + r * 128;
-#pragma unroll
-              for (int j = 0; j < C::HALVES; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(row + j * HALF + i * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
+            for (int e = 0; e < 32; ++e)
+              if (!(bits >> e & 1)) v[32 * i + e] = 0xff800000u;
           }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 128; j += 8)
+        for (int e = 0; e < BH; e += 8)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            mx4[i] = max3(mx4[i], __uint_as_float(v[j + 2 * i]), __uint_as_float(v[j + 2 * i + 1]));
+            mx4[i] = max3(mx4[i], __uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         mx = mx == -INFINITY ? -INFINITY : mx * p.scale_log2;
         const bool raise = mx > m + RESCALE;
         if (__any_sync(0xffffffffu, raise)) {
           const float m_new = raise ? mx : m;
           const float alpha = m == -INFINITY ? 0.f : raise ? ex2(m - m_new) : 1.f;
-          if (c > 0) {
-            if (!(ok = wait_warp(&o_done[t], (cnt - 1) & 1, abort_flag))) break;
+          // (rows that have seen no key so far have O = 0 already)
+          if (h > 0 && __any_sync(0xffffffffu, raise && m > -INFINITY)) {
+            if (!(ok = wait_warp(&o_done[2 * t + (j ^ 1)], ((cnt - 1) >> 1) & 1, abort_flag))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < DP / 16; ++i) {
               uint32_t o[16];
               tmem_ld16(o_col + i * 16, o);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
               tmem_st16(o_col + i * 16, o);
             }
             tmem_st_wait();
@@ -505,69 +562,71 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float mm = m == -INFINITY ? 0.f : m;
         const uint64_t base2 = pair2(-mm, -mm);
         uint64_t l2[2] = {0, 0};
+        // of every eight pairs, `POLY` on the FMA pipe: the special-function unit alone would take 64 x 8 cycles a warp
+        auto exps = [&](auto poly) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int j = half * 64; j < half * 64 + 64; j += 2) {
+          for (int e = 0; e < BH; e += 2) {
             float e0, e1;
-            unpair2(fma2(pair2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, base2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            l2[(j >> 1) & 1] = add2(l2[(j >> 1) & 1], pair2(e0, e1));
-            v[j / 2] = pack<T>(e0, e1);
+            const uint64_t y2 = fma2(pair2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, base2);
+            if (decltype(poly)::value && ((e >> 1) & 7) % 3 == 1) {
+              exp2_poly<T>(y2, e0, e1);
+            } else {
+              unpair2(y2, e0, e1);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+            }
+            l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], pair2(e0, e1));
+            v[e / 2] = pack<T>(e0, e1);
           }
-          tmem_st16(s_col + half * 32, v + half * 32);
-          tmem_st16(s_col + half * 32 + 16, v + half * 32 + 16);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(half ? &p_ready[t] : &p_half[t]);
-        }
+        };
+        if (masked) exps(std::false_type{});  // masked scores have to become zeros exactly
+        else exps(std::true_type{});
+        tmem_st16(sc, v);
+        tmem_st16(sc + 16, v + 16);
         float s0, s1, s2, s3;
         unpair2(l2[0], s0, s1);
         unpair2(l2[1], s2, s3);
         l += (s0 + s1) + (s2 + s3);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[2 * t + j]);
       }
       if (!ok) break;
       blk += x.n;
       if (nb > 0) {
-        if (!(ok = wait_warp(&o_done[t], (cnt - 1) & 1, abort_flag))) break;
+        const uint32_t last = ((cnt >> 1) - 1) & 1;
+        if (!(ok = wait_warp(&o_done[2 * t], last, abort_flag) && wait_warp(&o_done[2 * t + 1], last, abort_flag))) break;
         tc_fence_after();
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int D = (int)a.head_dim, token = x.tok0 + tok;
-      T *dst = static_cast<T *>(a.out) + token * a.out_token + (x.hk * p.G + g) * a.out_head;
-      float *part = p.ws + (int64_t)x.slot * C::SLOT;
-#pragma unroll 1
-      for (int i = 0; i < DP / 32; ++i) {
-        uint32_t o[32];
-        __syncwarp();  // the warp reads TMEM together
-        if (nb > 0) {
-          tmem_ld32(o_col + i * 32, o);
-        } else {
+      uint32_t o[DP];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0;
-        }
-        if (row_ok && x.final) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 w;
-            w.x = pack<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
-            w.y = pack<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-            w.z = pack<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
-            w.w = pack<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
-            if (i * 32 + j < D) *reinterpret_cast<uint4 *>(dst + i * 32 + j) = w;
-          }
-        } else if (row_ok) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4 *>(part + (t * BM + r) * DP + i * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-        }
-      }
-      if (row_ok && !x.final) *reinterpret_cast<float2 *>(part + 2 * BM * DP + 2 * (t * BM + r)) = make_float2(m, l);
-      __syncwarp();
+      for (int i = 0; i < DP; ++i) o[i] = 0;
       if (nb > 0) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) tmem_ld32_nw(o_col + i * 32, o + i * 32);
+        tmem_ld_wait();
         tc_fence_before();
-        mbar_arrive(&o_free[t]);
+        mbar_arrive(&o_free[t]);  // the next segment's products may go on
+      }
+      if (!row_ok) continue;
+      const int D = (int)a.head_dim;
+      if (x.final) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        T *dst = static_cast<T *>(a.out) + (x.tok0 + tok) * a.out_token + (x.hk * p.G + g) * a.out_head;
+#pragma unroll
+        for (int i = 0; i < DP; i += 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = pack<T>(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+          if (i + 16 <= D) store32(dst + i, w, p.wide);
+          else if (i < D) *reinterpret_cast<uint4 *>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+        float *part = p.ws + (int64_t)x.slot * C::SLOT;
+#pragma unroll
+        for (int i = 0; i < DP; i += 8) store32(part + (t * BM + r) * DP + i, o + i, true);
+        *reinterpret_cast<float2 *>(part + 2 * BM * DP + 2 * (t * BM + r)) = make_float2(m, l);
       }
     }
   }
@@ -587,45 +646,37 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// Joins the partials of the units that a share's end cuts: block (c, y) looks at
-// the unit cut by the beginning of CTA c's share, and takes 32 of its rows if
-// that is the unit's first cut.
+// Joins the partials of the units that a share's end cuts: an item (c, y) is the
+// unit cut by the beginning of CTA c's share, if that is the unit's first cut,
+// and 32 of its rows.
+constexpr int JOIN = 256;
 template <class T, int DP>
-__global__ void __launch_bounds__(256) tile_join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(JOIN) tile_join_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP>;
+  constexpr int PARTS = 2 * BM / 32;
   pdl_wait();
   const Args &a = p.a;
   const Walk walk(p, 0);
-  const int c = blockIdx.x + 1;
-  if (c >= walk.ctas) return;
-  const int64_t cut = share(walk.total, c, walk.ctas);
-  Segment s;
-  walk.locate(cut, s, threadIdx.x % 32);
-  const int64_t first = cut - s.k0;
-  if (s.k0 == 0) return;  // the share begins with the unit
-  const Parts parts = parts_of(walk.total, first, s.k.n, p.max_ctas, 0);
-  if (parts.c0 != c - 1) return;
-  const int D = (int)a.head_dim;
-  for (int i = threadIdx.x; i < 32 * (DP / 4); i += 256) {
-    const int row = blockIdx.y * 32 + i / (DP / 4), d = i % (DP / 4) * 4, t = row / BM, r = row % BM;
-    const int g = r % p.G, tok = t * p.P + r / p.G;
-    if (r >= p.P * p.G || tok >= s.x.ntok || d >= D) continue;
-    auto slot = [&](int j) { return p.ws + (int64_t)parts.slot(j) * C::SLOT; };
-    float M = -INFINITY, L = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < parts.n; ++j) M = fmaxf(M, __ldcg(slot(j) + 2 * BM * DP + 2 * row));
-    for (int j = 0; j < parts.n; ++j) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(j) + 2 * BM * DP + 2 * row));
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(slot(j) + row * DP + d));
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L += ml.y * f;
-      x[0] += y.x * f;
-      x[1] += y.y * f;
-      x[2] += y.z * f;
-      x[3] += y.w * f;
+  if (walk.whole) return;
+  for (int item = blockIdx.x; item < (walk.ctas - 1) * PARTS; item += gridDim.x) {
+    const int c = item / PARTS + 1;
+    const int64_t cut = share(walk.total, c, walk.ctas);
+    Segment s;
+    walk.locate(cut, s, threadIdx.x % 32);
+    if (s.k0 == 0) continue;  // the share begins with the unit
+    const Parts parts = parts_of(walk.total, cut - s.k0, s.k.n, p.max_ctas, 0);
+    if (parts.c0 != c - 1) continue;
+    for (int i = threadIdx.x; i < 32 * (DP / 4); i += JOIN) {
+      const int row = item % PARTS * 32 + i / (DP / 4), d = i % (DP / 4) * 4, t = row / BM, r = row % BM;
+      const int g = r % p.G, tok = t * p.P + r / p.G;
+      if (r >= p.P * p.G || tok >= s.x.ntok || d >= (int)a.head_dim) continue;
+      Joined x;
+      x.add(parts.n, [&](int j) {
+        const float *slot = p.ws + (int64_t)parts.slot(j) * C::SLOT;
+        return Partial{slot + row * DP + d, slot + 2 * BM * DP + 2 * row};
+      });
+      x.store(static_cast<T *>(a.out) + (s.x.tok0 + tok) * a.out_token + (s.hk * p.G + g) * a.out_head + d);
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + (s.x.tok0 + tok) * a.out_token + (s.hk * p.G + g) * a.out_head + d) =
-        make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
   }
 }
 
@@ -637,7 +688,7 @@ int log2_of(int64_t x) {
 
 // workspace: head | pairs | seq_pairs | partial slots
 struct Layout {
-  size_t pairs, seqs, ws, bytes;
+  size_t next, pairs, seqs, ws, bytes;
   int max_pairs;
 };
 Layout layout(const Args &a, int max_ctas, bool own, bool prefix, bool keep) {
@@ -646,7 +697,8 @@ Layout layout(const Args &a, int max_ctas, bool own, bool prefix, bool keep) {
   // every sequence, and the tokens before and after them, may end in a part of a pair
   x.max_pairs = (int)((prefix ? (T + per - 1) / per : 0) + (own ? T / per + a.seqs + 2 : 0));
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  x.pairs = up(((size_t)x.max_pairs + 2) * 8);
+  x.next = ((size_t)x.max_pairs + 2) * 8;
+  x.pairs = up(x.next + 8);
   x.seqs = x.pairs + up((size_t)x.max_pairs * sizeof(Pair));
   x.ws = x.seqs + up((size_t)(own ? a.seqs + 2 : 0) * 4);
   const size_t slot = (a.head_dim <= 64 ? Cfg<64>::SLOT : Cfg<128>::SLOT) * sizeof(float);
@@ -687,7 +739,7 @@ int launch(const Params &p, cudaStream_t st, int device) {
   NKB_CUDA_TRY(launch_pdl(true, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
   if (int s = launch_status("paged_tile")) return s;
   if (p.keep || p.max_ctas < 2) return NKB_OK;
-  NKB_CUDA_TRY(launch_pdl(true, tile_join_kernel<T, DP>, dim3(p.max_ctas - 1, 2 * BM / 32), dim3(256), 0, st, p));
+  NKB_CUDA_TRY(launch_pdl(true, tile_join_kernel<T, DP>, dim3(4 * p.max_ctas), dim3(JOIN), 0, st, p));
   return launch_status("paged_tile join");
 }
 
@@ -719,10 +771,12 @@ int tile_params(const Args &a, int device, void *workspace, bool own, bool prefi
   p->prefix = prefix;
   p->keep = keep;
   p->scale_log2 = (float)(a.scale * 1.4426950408889634);
+  p->wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
   const Layout x = layout(a, p->max_ctas, own, prefix, keep);
   p->max_pairs = x.max_pairs;
   char *w = static_cast<char *>(workspace);
   p->head = reinterpret_cast<int64_t *>(w);
+  p->next = reinterpret_cast<int *>(w + x.next);
   p->pairs = reinterpret_cast<Pair *>(w + x.pairs);
   p->seq_pairs = reinterpret_cast<int *>(w + x.seqs);
   p->ws = reinterpret_cast<float *>(w + x.ws);

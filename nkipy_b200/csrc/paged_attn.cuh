@@ -56,6 +56,10 @@ __device__ __forceinline__ Parts parts_of(int64_t total, int64_t first, int64_t 
   return p;
 }
 
+// One partial of a row: where its four outputs and its (max, sum) lie.
+struct Partial {
+  const float *o, *ml;
+};
 // 2^x on the special-function unit (relative error about 2^-22; -inf -> 0)
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -75,6 +79,49 @@ __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&h);
 }
+
+// Four outputs of a row, joined from partials that are read eight at a time.
+struct Joined {
+  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  template <class At>
+  __device__ __forceinline__ void add(int n, At at) {
+    constexpr int U = 8;
+    for (int j0 = 0; j0 < n; j0 += U) {
+      float2 ml[U];
+      float4 y[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const Partial q = at(min(j0 + j, n - 1));
+        ml[j] = __ldcg(reinterpret_cast<const float2 *>(q.ml));
+        y[j] = __ldcg(reinterpret_cast<const float4 *>(q.o));
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < U; ++j) top = fmaxf(top, ml[j].x);
+      if (top == -INFINITY) continue;  // nothing seen so far
+      const float f = ex2(m - top);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= f;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const float g = j0 + j < n ? ex2(ml[j].x - top) : 0.f;
+        if (g == 0.f) continue;  // a part that saw nothing has nothing written for it to scale
+        l += ml[j].y * g;
+        x[0] += y[j].x * g;
+        x[1] += y[j].y * g;
+        x[2] += y[j].z * g;
+        x[3] += y[j].w * g;
+      }
+      m = top;
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void store(T *p) const {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
+  }
+};
 
 // rows of 16-byte pieces: every stride and base that a vector or TMA access needs
 inline bool aligned16(const Args &a) {
@@ -202,8 +249,10 @@ struct Params {
   int G, P, page_shift, max_pairs, max_ctas;
   int own, prefix;  // list the sequences' own keys / the prefix
   int keep;         // write every unit as a partial
+  int wide;         // rows of out start at 32-byte boundaries
   float scale_log2;
   int64_t *head;   // number of pairs, then the pairs' first blocks (max_pairs + 1)
+  int *next;       // the next unit that no CTA has, where whole units are handed out
   Pair *pairs;
   int *seq_pairs;  // first pair of each sequence (scheduler only)
   float *ws;
@@ -248,16 +297,30 @@ struct Segment {
   bool all;           // the whole unit
   int slot;           // of its partial
 };
+// Where there are many units a CTA takes whole ones, the last pairs first (under
+// a causal mask the longest), the next when it has done one: no partial is
+// written, and the CTAs end within a unit of one another.  With few, their
+// blocks are shared evenly.
+constexpr int WHOLE = 4;  // units per CTA from which they stay whole
 struct Walk {
   const Params &p;
   int64_t total, f, f0, f1;
-  int ctas, c;
+  int ctas, c, units;
+  bool whole;
   __device__ __forceinline__ Walk(const Params &q, int cta) : p(q), c(cta) {
-    total = p.head[1 + p.head[0]] * p.a.kv_heads;
+    const int pairs = (int)p.head[0];
+    total = p.head[1 + pairs] * p.a.kv_heads;
+    units = pairs * (int)p.a.kv_heads;
+    whole = units >= WHOLE * p.max_ctas;
     ctas = workers(total, p.max_ctas);
     f0 = c < ctas ? share(total, c, ctas) : 0;
     f1 = c < ctas ? share(total, c + 1, ctas) : 0;
     f = f0;
+  }
+  __device__ __forceinline__ Parts parts(int u, int hk, int64_t n) const {
+    const int unit = u * (int)p.a.kv_heads + hk;
+    if (whole) return Parts{1, 0, 2 * p.max_ctas + unit};
+    return parts_of(total, p.head[1 + u] * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
   }
   // unit that holds block `at`: a whole warp looks, 32 pivots at a time
   __device__ __forceinline__ void locate(int64_t at, Segment &s, int lane) const {
@@ -282,6 +345,21 @@ struct Walk {
   }
   // the next segment of the share (a whole warp)
   __device__ __forceinline__ bool next(Segment &s, int lane) {
+    if (whole) {
+      int i = c;
+      if (f != f0 && lane == 0) i = atomicAdd(p.next, 1);
+      i = __shfl_sync(0xffffffffu, i, 0);
+      ++f;
+      if (i >= units) return false;
+      i = units - 1 - i;
+      set(i / (int)p.a.kv_heads, s);
+      s.hk = i % (int)p.a.kv_heads;
+      s.k0 = 0;
+      s.k1 = s.k.n;
+      s.all = true;
+      s.slot = 2 * p.max_ctas + i;
+      return true;
+    }
     if (f >= f1) return false;
     if (f == f0) {
       locate(f, s, lane);
