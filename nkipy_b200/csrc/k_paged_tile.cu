@@ -18,7 +18,7 @@
 //   8      walks the CTA's share, hands its segments to the others through a small
 //          ring, and produces: TMA loads of Q (both tiles) and, page by page, of
 //          K and V into rings of stages that are released separately;
-//   9, 10  one thread each issues the products of tile A and of tile B: S(0)
+//   9, 10  issue the products of tile A and of tile B: S(0)
 //          S(1), then per half PV(h) S(h + 2); warp 9 owns the TMEM;
 //   11     sees to V: rows that no token of the pair sees become zeros;
 //   0-3, 4-7  softmax of tile A and of tile B, one thread per row: scores from
@@ -166,6 +166,31 @@ __device__ __forceinline__ constexpr uint32_t idesc(int M, int N, int b_mn_major
          ((uint32_t)(M >> 4) << 24);
 }
 
+// Products and commits of a whole warp, issued by its elected lane: the warp
+// stays converged and the descriptors warp-uniform, so that no operand has to be
+// moved out of a diverged thread's registers (in an `if (lane == 0)` an issue
+// took about 100 cycles, which bounded the kernel).
+__device__ __forceinline__ void warp_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void warp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n elect.sync _|q, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
 // A segment as the roles need it.
 struct Item {
   int seq, tok0, ntok, pos0, hk;
@@ -211,7 +236,7 @@ __device__ __forceinline__ void exp2_poly(uint64_t y2, float &e0, float &e1) {
   unpair2(y2, y0, y1);
   y2 = pair2(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
   const uint64_t t2 = add2(y2, pair2(12582912.f, 12582912.f));           // 1.5 * 2^23: n in the low bits
-  const uint64_t r2 = add2(y2, fma2(add2(t2, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), 0));
+  const uint64_t r2 = fma2(add2(t2, pair2(-12582912.f, -12582912.f)), pair2(-1.f, -1.f), y2);
   auto c = [](float x) { return pair2(x, x); };
   uint64_t q;
   if (fine) {
@@ -266,8 +291,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   // [tile][score buffer] where a tile has two
   uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_ready = bars + 6, *o_done = bars + 10,
            *o_free = bars + 14, *i_full = bars + 16, *i_empty = i_full + RING, *k_full = i_empty + RING,
-           *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *v_ready = v_empty + ST;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_ready + ST);
+           *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *v_ready = v_empty + ST,
+           *b_go = v_ready + ST;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(b_go + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   Item *ring = reinterpret_cast<Item *>(smem + C::OFF_ITEMS);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -276,6 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 2);  // both issuers
+    mbar_init(b_go, 1);
     for (int t = 0; t < 2; ++t) {
       for (int j = 0; j < 2; ++j) {
         mbar_init(&s_full[2 * t + j], 1);
@@ -312,14 +339,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_trigger();
   bool ok = true;
   uint32_t items = 0;  // segments taken so far
-  // the next segment, from the ring (whole warps, or one thread for an issuer)
-  auto take = [&](Item &x, bool whole_warp) {
+  // the next segment, from the ring (a whole warp)
+  auto take = [&](Item &x) {
     const int i = items % RING;
-    ok = whole_warp ? wait_warp(&i_full[i], (items / RING) & 1, abort_flag) : wait(&i_full[i], (items / RING) & 1, abort_flag);
-    if (!ok) return false;
+    if (!(ok = wait_warp(&i_full[i], (items / RING) & 1, abort_flag))) return false;
     x = ring[i];
-    if (whole_warp) __syncwarp();
-    if (!whole_warp || lane == 0) mbar_arrive(&i_empty[i]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[i]);
     ++items;
     return x.n > 0;
   };
@@ -391,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------- V rows that no token of the pair sees ----------------
       uint32_t blk = 0;
       Item x;
-      while (ok && take(x, true)) {
+      while (ok && take(x)) {
         const int sinks = (int)min(a.sinks, (int64_t)x.end);
         for (int i = x.k0; i < x.k0 + x.n; ++i, ++blk) {
           const int st = blk % ST, key0 = block_of(x, i) * BN;
@@ -411,44 +437,47 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) mbar_arrive(&v_ready[st]);
         }
       }
-    } else if (lane == 0) {
+    } else {
       // ---------------- MMA issuer of tile t ----------------
       constexpr uint32_t ID_S = idesc<T>(128, BH, 0), ID_O = idesc<T>(128, DP, 1);
-      const int t = warp - W_MMA;
+      const int t = __shfl_sync(0xffffffffu, warp, 0) - W_MMA;
       const Desc dq(smem_desc(smem_u32(smem + t * C::TILE), 16, 1024)), dk(smem_desc(smem_u32(smem + C::OFF_K), 16, 1024)),
           dv(smem_desc(smem_u32(smem + C::OFF_V), HALF, 1024));
       const uint32_t ts = tmem + T_S + t * 128, to = tmem + T_O + t * 128;
       uint32_t segs = 0, blk = 0, cnt = 0, outs = 0;
       Item x;
-      while (ok && take(x, false)) {
-        const int n = x.n, nb = t ? x.nb_b : x.nb_a;
+      while (ok && take(x)) {
+        const int n = __shfl_sync(0xffffffffu, x.n, 0), nb = __shfl_sync(0xffffffffu, t ? x.nb_b : x.nb_a, 0);
+        // tile B begins when the softmax of A has done its first half: in step, both would want the special-function
+        // units at one time and the tensor cores at another.  (A cannot be a segment ahead: Q is shared.)
+        if (t == 1 && !(ok = wait_warp(b_go, segs & 1, abort_flag))) break;
         auto stage = [&](int c) { return (blk + c) % ST; };
-        auto full = [&](uint64_t *bar, int c) { return wait(&bar[stage(c)], ((blk + c) / ST) & 1, abort_flag); };
+        auto full = [&](uint64_t *bar, int c) { return wait_warp(&bar[stage(c)], ((blk + c) / ST) & 1, abort_flag); };
         auto qk = [&](int c, int j) {  // S = Q K^T of half j of block c
           const Desc k(dk.at(stage(c) * C::TILE + j * BH * 128));
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk) {
             const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-            umma_f16(ts + j * BH, dq.at(off), k.at(off), ID_S, kk > 0);
+            warp_mma(ts + j * BH, dq.at(off), k.at(off), ID_S, kk > 0);
           }
-          umma_commit(&s_full[2 * t + j]);
+          warp_commit(&s_full[2 * t + j]);
         };
         auto pv = [&](int c, int j) {  // O += P V
           const Desc v(dv.at(stage(c) * C::TILE + j * BH * 128));
 #pragma unroll
           for (int kk = 0; kk < BH / 16; ++kk)
-            umma_f16_ts(to, ts + j * BH + kk * 8, v.at(kk * 2048), ID_O, (c > 0 || j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&o_done[2 * t + j]);
+            warp_mma_ts(to, ts + j * BH + kk * 8, v.at(kk * 2048), ID_O, (c > 0 || j > 0 || kk > 0) ? 1u : 0u);
+          warp_commit(&o_done[2 * t + j]);
         };
-        if (!(ok = wait(q_full, segs & 1, abort_flag) && full(k_full, 0))) break;
+        if (!(ok = wait_warp(q_full, segs & 1, abort_flag) && full(k_full, 0))) break;
         ++segs;
         tc_fence_after();
         if (nb > 0) {
           qk(0, 0);
           qk(0, 1);
         }
-        umma_commit(&k_empty[stage(0)]);
-        if (n == 1) umma_commit(q_empty);
+        warp_commit(&k_empty[stage(0)]);
+        if (n == 1) warp_commit(q_empty);
         for (int c = 0; c < n; ++c) {
           // a block that this tile does not need is waited for all the same: its stages are released in order
           if (!(ok = full(v_ready, c))) break;
@@ -456,8 +485,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               // P of the half is written; before a segment's first product, O of the segment before is read
-              if (!(ok = wait(&p_ready[2 * t + j], cnt & 1, abort_flag) &&
-                         (c > 0 || j > 0 || outs == 0 || wait(&o_free[t], (outs - 1) & 1, abort_flag))))
+              if (!(ok = wait_warp(&p_ready[2 * t + j], cnt & 1, abort_flag) &&
+                         (c > 0 || j > 0 || outs == 0 || wait_warp(&o_free[t], (outs - 1) & 1, abort_flag))))
                 break;
               tc_fence_after();
               pv(c, j);
@@ -470,11 +499,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!ok) break;
             ++cnt;
           }
-          umma_commit(&v_empty[stage(c)]);
+          warp_commit(&v_empty[stage(c)]);
           if (c + 1 < n) {
             if (c + 1 >= nb && !(ok = full(k_full, c + 1))) break;
-            umma_commit(&k_empty[stage(c + 1)]);
-            if (c + 2 == n) umma_commit(q_empty);
+            warp_commit(&k_empty[stage(c + 1)]);
+            if (c + 2 == n) warp_commit(q_empty);
           }
         }
         blk += n;
@@ -490,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2);
     uint32_t blk = 0, cnt = 0;
     Item x;
-    while (ok && take(x, true)) {
+    while (ok && take(x)) {
       const int nb = t ? x.nb_b : x.nb_a;
       const bool row_ok = r < p.P * p.G && tok < x.ntok;
       // keys that the row sees: [lo, hi), and below `first`
@@ -503,21 +532,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           first = (int)min(a.sinks, (int64_t)hi);
         }
       }
+      // halves that need no mask: from the last row's first key to the first row's last one
+      const int plain_lo = __reduce_max_sync(0xffffffffu, lo), plain_hi = __reduce_min_sync(0xffffffffu, hi);
       float m = -INFINITY, l = 0.f;  // running (possibly stale) maximum in log2 units, and sum
       for (int h = 0; h < 2 * nb; ++h, ++cnt) {
         const int c = h >> 1, j = h & 1, key0 = block_of(x, x.k0 + c) * BN + j * BH;
         const uint32_t sc = s_col + j * BH;
         // the scores, and the product of the half before last: every phase of o_done is waited for in turn, so
         // that the parity of a later wait (below) cannot be that of an older phase
-        if (!(ok = wait_warp(&s_full[2 * t + j], (cnt >> 1) & 1, abort_flag) &&
-                   (h < 2 || wait_warp(&o_done[2 * t + j], ((cnt >> 1) - 1) & 1, abort_flag))))
-          break;
+        ok = wait(&s_full[2 * t + j], (cnt >> 1) & 1, abort_flag) &&
+             (h < 2 || wait(&o_done[2 * t + j], ((cnt >> 1) - 1) & 1, abort_flag));
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         uint32_t v[BH];
         tmem_ld32_nw(sc, v);
         tmem_ld32_nw(sc + 32, v + 32);
         tmem_ld_wait();
-        const bool masked = __any_sync(0xffffffffu, key0 + BH > hi || (key0 < lo && key0 + BH > first));
+        const bool masked = key0 < plain_lo || key0 + BH > plain_hi;
         if (masked) {
           // a bit per key: below hi, and from lo or below first
           const int hk = hi - key0, w = lo - key0, f = first - key0;
@@ -590,9 +621,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_ready[2 * t + j]);
+        if (h == 0 && warp == 0 && lane == 0) mbar_arrive(b_go);
       }
       if (!ok) break;
       blk += x.n;
+      if (nb == 0 && warp == 0 && lane == 0) mbar_arrive(b_go);
       if (nb > 0) {
         const uint32_t last = ((cnt >> 1) - 1) & 1;
         if (!(ok = wait_warp(&o_done[2 * t], last, abort_flag) && wait_warp(&o_done[2 * t + 1], last, abort_flag))) break;
