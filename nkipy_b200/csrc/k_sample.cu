@@ -8,18 +8,19 @@
 // above the complement of the index, so equal logits rank by index and the
 // kept set is "rank word >= threshold", with e >= min_p.
 //
-// A cluster of up to 8 CTAs holds a row in its shared memory: the logits are
-// read from memory once.  What bounds the kernel is then the instructions per
-// element and the cluster's meetings (three without filters on the order,
-// seven with both), so that elements which cannot matter are dropped by one
-// comparison with a cut: the lowest logit with a nonzero weight, and for top-k
-// a bound from the threads' own maxima.
+// A cluster of 8 CTAs holds a row in its shared memory: the logits are read from
+// memory once.  What bounds the kernel is then the instructions per element and
+// the cluster's meetings, so that elements which cannot matter are dropped by
+// one comparison with a cut: the lowest logit with a nonzero weight, and for
+// top-k a bound from the threads' own maxima.
 //   1  logits to shared memory, each thread's maxima; the row's maximum
-//   2  top-k / top-p: histogram of counts and weights over bins linear in
+//   2  top-k of up to FAST_K: what passes the bound (some 8 k elements) goes to
+//      one CTA, which sorts it and does the rest alone; otherwise
+//   3  top-k / top-p: histogram of counts and weights over bins linear in
 //      (max - x) / temperature; summed over the cluster, every CTA gets it
-//   3  the elements of the bin that the threshold falls in go to every CTA,
+//   4  the elements of the bin that the threshold falls in go to every CTA,
 //      which finds the threshold among them (narrowing by rank word)
-//   4  kept weight per warp, contiguous in the row; the warp in which the
+//   5  kept weight per warp, contiguous in the row; the warp in which the
 //      running sum passes u times the total walks its part
 #include <cooperative_groups.h>
 
@@ -69,18 +70,20 @@ constexpr int NT = 512, NW = NT / 32;
 constexpr int NB = 1024;    // bins
 constexpr int CAP = 1024;   // elements of a bin that a CTA takes
 constexpr int FEW = 96;     // elements that are ranked one against another
-constexpr int MAX_C = 8;
+constexpr int C = 8;        // CTAs of a cluster
+constexpr int FAST_K = 100; // top-k that one CTA sorts: C * FAST_K candidates are expected, CAP fit
 constexpr int MAX_SLICE = 65528;  // weights' 16-bit halves sum to less than 2^32
 constexpr float SPAN = 22.25f;    // e^-SPAN < 2^-32
 
 struct Shared {
   u64 list[2][CAP], lw[2][CAP];  // rank words and weights of the threshold bin: top-k's, top-p's
   u64 gm[NB];                    // weights per bin, whole row
-  u64 sums[MAX_C], red[NW], red2[NW], few[FEW], few_w[FEW];
+  u64 sums[C], red[NW], red2[NW], few[FEW], few_w[FEW];
   uint32_t hc[NB], hl[NB], hh[NB];  // this CTA's bins: counts, low and high halves of the weights
   uint32_t gc[NB];                  // counts per bin, whole row
   uint32_t nc[NB], nl[NB], nh[NB];  // narrowing
-  float maxima[MAX_C];
+  float maxima[C];
+  int counts[C], n_fast;
   u64 out_a, out_b, out_c;
   int n_list, bin;
 };
@@ -100,11 +103,22 @@ __device__ V reduce(V v, Op op, V *shared) {  // over the block, to every thread
 }
 
 // Lowest key in (-inf, inf] that `yes` holds for, where it holds for `top` and
-// for every key above one it holds for: 32 pivots at a time, by one warp.
+// for every key above one it holds for: by one warp, first the 32 keys around a
+// guess, then 32 pivots at a time.
 template <class Yes>
-__device__ uint32_t lowest_key(uint32_t top, Yes yes) {
+__device__ uint32_t lowest_key(uint32_t top, float guess, Yes yes) {
   uint32_t lo = KEY_NEG_INF, hi = top;  // not at lo, at hi
   const int lane = threadIdx.x & 31;
+  {
+    const uint32_t g = key_of(guess);
+    const uint32_t base = g > KEY_NEG_INF + 16 && g < top ? g - 16 : KEY_NEG_INF;
+    const uint32_t at = min(base + 1 + lane, hi);
+    const uint32_t m = __ballot_sync(0xffffffffu, yes(of_key(at)));
+    const int f = __ffs(m) - 1;
+    if (f > 0) return min(base + 1 + f, hi);
+    if (f == 0) hi = min(base + 1, hi);
+    else lo = base + 32;
+  }
   while (hi - lo > 1) {
     const uint32_t step = (hi - lo - 1) / 32 + 1;
     const uint32_t off = step * (lane + 1), at = off < hi - lo ? lo + off : hi;
@@ -151,14 +165,80 @@ __device__ int crossing(Shared &s, u64 target, Get get, u64 *before) {
   return s.bin;
 }
 
+// The rest of a row whose n candidates (rank words, at most CAP) hold its k
+// largest elements, by one CTA.
+__device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, int n, int k, float p, uint32_t key_pmin) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  u64 *list = s.list[0];
+  int N = 64;
+  while (N < n) N *= 2;
+  for (int i = n + tid; i < N; i += NT) list[i] = 0;
+  __syncthreads();
+  // bitonic, largest first; a warp keeps the 64 elements of its short strides to itself
+  for (int size = 2; size <= N; size *= 2)
+    for (int stride = size / 2; stride; stride /= 2) {
+      if (tid < N / 2) {
+        const int i = 2 * tid - (tid & (stride - 1)), j = i + stride;
+        const u64 x = list[i], y = list[j];
+        if ((x < y) == ((i & size) == 0)) {
+          list[i] = y;
+          list[j] = x;
+        }
+      }
+      // the next stride's elements are this warp's own while it is at most 32
+      if (stride > 1 && stride <= 32) __syncwarp();
+      else __syncthreads();
+    }
+  const int m = min(k, n);
+  static_assert(FAST_K <= 128, "four warps hold the k largest");
+  u64 w = 0, sum = 0;
+  uint32_t key = 0;
+  if (tid < 128) {
+    if (tid < m) {
+      key = (uint32_t)(list[tid] >> IDX_BITS);
+      w = Row::w(f.e(of_key(key)));
+    }
+    sum = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += y;
+    }
+    if (lane == 31) s.red[warp] = sum;
+  }
+  __syncthreads();
+  if (tid < 128) {
+    for (int i = 0; i < warp; ++i) sum += s.red[i];
+    const u64 W = s.red[0] + s.red[1] + s.red[2] + s.red[3];
+    const double want = (double)p * (double)W;
+    const u64 T = p < 1.f ? (want >= 1.0 ? (u64)want : 1) : ~0ull;
+    const bool keep = tid < m && sum - w < T && key >= key_pmin;
+    s.lw[0][tid] = keep ? w : 0;
+  }
+  __syncthreads();
+  if (tid < 128) {
+    const u64 own = s.lw[0][tid];
+    u64 total = 0, upto = 0;  // of all, and of those up to this one in index order
+    for (int i = 0; i < m; ++i) {
+      const u64 x = s.lw[0][i];
+      total += x;
+      if (tid < m && (list[i] & (MAX_VOCAB - 1)) >= (list[tid] & (MAX_VOCAB - 1))) upto += x;
+    }
+    const float u = a.u[r];
+    u64 at = (u64)((double)(u > 0.f ? u : 0.f) * (double)total);
+    at = at < total ? at : total - 1;
+    if (own && upto > at && upto - own <= at) a.tokens[r] = (int)(MAX_VOCAB - 1 - (list[tid] & (MAX_VOCAB - 1)));
+  }
+}
+
 template <class T>
-__global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Args a, int slice) {
+__global__ void __launch_bounds__(NT, 2) cluster_kernel(const __grid_constant__ Args a, int slice) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
   Shared &s = *reinterpret_cast<Shared *>(smem);
   T *xs = reinterpret_cast<T *>(smem + (sizeof(Shared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / C;
   const int V = (int)a.vocab, i0 = rank * slice, n = max(0, min(slice, V - i0));
@@ -200,6 +280,7 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
     const float m = reduce(fmaxf(m0, m1), [](float x, float y) { return fmaxf(x, y); }, reinterpret_cast<float *>(s.red));
     if (tid < C) cluster.map_shared_rank(s.maxima, tid)[rank] = m;
   }
+  if (tid == 0) s.n_fast = 0;
   cluster.sync();
   float gmax = -INFINITY;
   int owner = 0;  // lowest rank that has the maximum
@@ -238,7 +319,12 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
   float pmin = a.min_p ? a.min_p[r] : 0.f;
   pmin = pmin > 1.f ? 1.f : pmin;
   // the lowest logit that has a weight: below it (and NaN) nothing matters
-  float cut = of_key(lowest_key(kmax, [&](float x) { return Row::w(f.e(x)) > 0; }));
+  float cut = of_key(lowest_key(kmax, gmax - 22.180709f * temp, [&](float x) { return Row::w(f.e(x)) > 0; }));
+  // lowest logit of the bins up to b
+  auto bin_end = [&](int b) {
+    return lowest_key(kmax, gmax - (float)(b + 1) * (SPAN / NB) * temp, [&](float x) { return bin_of(x) <= b; });
+  };
+  const uint32_t key_pmin = pmin > 0.f ? lowest_key(kmax, gmax + logf(pmin) * temp, [&](float x) { return f.e(x) >= pmin; }) : 0;
   u64 thr = 0;  // rank word of the last kept element
 
   if (by_count || by_mass) {
@@ -252,11 +338,37 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
       __syncthreads();
       u64 before;
       const int b = crossing<NB>(s, (u64)k, [&](int i) { return (u64)s.hc[i]; }, &before);
-      if (b < NB) cut_k = fmaxf(cut, of_key(lowest_key(kmax, [&](float x) { return bin_of(x) <= b; })));
+      if (b < NB) cut_k = fmaxf(cut, of_key(bin_end(b)));
+      if (k <= FAST_K) {
+        // 2  candidates to rank 0; how many there are, to everyone
+        int mine = 0;
+        for (int v = v0 + lane; v < v1; v += 32) {
+          const uint4 q = xv[v];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float x = get(q, j);
+            if (x >= cut_k) {
+              ++mine;
+              const int at = atomicAdd(cluster.map_shared_rank(&s.n_fast, 0), 1);
+              if (at < CAP) cluster.map_shared_rank(s.list[0], 0)[at] = rank_word(key_of(x), i0 + v * VEC + j);
+            }
+          }
+        }
+        mine = reduce(mine, [](int x, int y) { return x + y; }, reinterpret_cast<int *>(s.red));
+        if (tid < C) cluster.map_shared_rank(s.counts, tid)[rank] = mine;
+        cluster.sync();
+        int all = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) all += s.counts[c];
+        if (all <= CAP) {
+          if (rank == 0) draw_sorted(s, a, r, f, all, k, p, key_pmin);
+          return;
+        }
+      }
       for (int i = tid; i < NB; i += NT) s.hc[i] = 0;
       __syncthreads();
     }
-    // 2  histogram
+    // 3  histogram
     for (int v = v0 + lane; v < v1; v += 32) {
       const uint4 q = xv[v];
 #pragma unroll
@@ -286,7 +398,7 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
     }
     cluster.sync();
 
-    // 3  the element at which the running count (or weight), from the largest
+    // 4  the element at which the running count (or weight), from the largest
     // element down, reaches `target`: its rank word; *mass: weight up to it
     auto find = [&](bool count, u64 target, int buf, u64 *mass) -> u64 {
       u64 before, other;
@@ -302,8 +414,7 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
         other = reduce(o, add, s.red);
       }
       u64 acc_w = count ? other : before, acc = before;  // weight, and the target's measure, before the range
-      const uint32_t k_lo = lowest_key(kmax, [&](float x) { return bin_of(x) <= b; });
-      const uint32_t k_hi = b ? lowest_key(kmax, [&](float x) { return bin_of(x) < b; }) - 1 : kmax;
+      const uint32_t k_lo = bin_end(b), k_hi = b ? bin_end(b - 1) - 1 : kmax;
       u64 lo = rank_word(k_lo, (int)MAX_VOCAB - 1), hi = rank_word(k_hi, 0);  // range of rank words
       const float x_lo = fmaxf(of_key(k_lo), cut), x_hi = of_key(k_hi);
       uint32_t cnt = s.gc[b];
@@ -452,11 +563,11 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
     }
   }
 
-  // 4  kept weight, in index order
+  // 5  kept weight, in index order
   const uint32_t thr_key = (uint32_t)(thr >> IDX_BITS);
   const int thr_idx = (int)(MAX_VOCAB - 1 - (thr & (MAX_VOCAB - 1)));  // of the elements equal to it, up to this index
   if (thr) cut = fmaxf(cut, of_key(thr_key));
-  if (pmin > 0.f) cut = fmaxf(cut, of_key(lowest_key(kmax, [&](float x) { return f.e(x) >= pmin; })));
+  if (pmin > 0.f) cut = fmaxf(cut, of_key(key_pmin));
   const float tie = thr ? of_key(thr_key) : -INFINITY;
   auto kept = [&](float x, int i) -> u64 {  // weight of element i, 0 if it is not kept
     if (!(x >= cut) || (x == tie && i > thr_idx)) return 0;
@@ -521,7 +632,7 @@ __global__ void __launch_bounds__(NT) cluster_kernel(const __grid_constant__ Arg
 }
 
 template <class T>
-int launch_cluster(const Args &a, int C, int slice, cudaStream_t st, int device) {
+int launch_cluster(const Args &a, int slice, cudaStream_t st, int device) {
   const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)slice * sizeof(T);
   static ContextOnce attr;
   if (int s = attr.run(device, []() -> int {
@@ -544,16 +655,11 @@ int launch_cluster(const Args &a, int C, int slice, cudaStream_t st, int device)
   return launch_status("sample_tokens");
 }
 
-// CTAs per row, and elements per CTA; 0 where a row does not fit a cluster
-int cluster_for(const Args &a, int *slice) {
-  const int64_t es = dtype_size((int)a.dtype);
-  for (int C = MAX_C; C >= 1; C /= 2) {
-    const int64_t n = ((a.vocab + C - 1) / C + 7) / 8 * 8;
-    *slice = (int)n;
-    if (n <= MAX_SLICE && (sizeof(Shared) + 15) / 16 * 16 + n * es <= 227 * 1024) return C;
-    if (C == MAX_C) return 0;
-  }
-  return 0;
+// elements per CTA; 0 where a row does not fit a cluster
+int slice_of(const Args &a) {
+  const int64_t n = ((a.vocab + C - 1) / C + 7) / 8 * 8;
+  const bool fits = n <= MAX_SLICE && (sizeof(Shared) + 15) / 16 * 16 + n * dtype_size((int)a.dtype) <= 227 * 1024;
+  return fits ? (int)n : 0;
 }
 
 // ---- rows of any length ------------------------------------------------------
@@ -728,7 +834,7 @@ __global__ void __launch_bounds__(THREADS) long_row_kernel(const __grid_constant
 
 int check_args(const Args &a) {
   auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("sample_tokens: ") + m); };
-  if (a.rows < 0 || a.rows > INT32_MAX / MAX_C || a.vocab < 1) return bad("rows or vocab out of range");
+  if (a.rows < 0 || a.rows > INT32_MAX / C || a.vocab < 1) return bad("rows or vocab out of range");
   if (a.dtype != NKB_F32 && a.dtype != NKB_BF16 && a.dtype != NKB_F16)
     return fail(NKB_ERR_UNSUPPORTED, "sample_tokens: logits must be float32, bfloat16 or float16");
   if (a.vocab > MAX_VOCAB) return fail(NKB_ERR_UNSUPPORTED, "sample_tokens: more than 2^21 entries");
@@ -740,11 +846,10 @@ int check_args(const Args &a) {
 int run(const Args &a, cudaStream_t st, int device) {
   if (int s = check_args(a)) return s;
   if (a.rows == 0) return NKB_OK;
-  int slice = 0;
-  if (const int C = cluster_for(a, &slice)) {
-    if (a.dtype == NKB_F32) return launch_cluster<float>(a, C, slice, st, device);
-    if (a.dtype == NKB_BF16) return launch_cluster<__nv_bfloat16>(a, C, slice, st, device);
-    return launch_cluster<__half>(a, C, slice, st, device);
+  if (const int slice = slice_of(a)) {
+    if (a.dtype == NKB_F32) return launch_cluster<float>(a, slice, st, device);
+    if (a.dtype == NKB_BF16) return launch_cluster<__nv_bfloat16>(a, slice, st, device);
+    return launch_cluster<__half>(a, slice, st, device);
   }
   long_row_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(a);
   return launch_status("sample_tokens");
