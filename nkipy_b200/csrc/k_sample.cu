@@ -10,18 +10,23 @@
 //
 // A cluster of 8 CTAs holds a row in its shared memory: the logits are read from
 // memory once.  What bounds the kernel is then the instructions per element and
-// the cluster's meetings, so that elements which cannot matter are dropped by
-// one comparison with a cut: the lowest logit with a nonzero weight, and for
-// top-k a bound from the threads' own maxima.
-//   1  logits to shared memory, each thread's maxima; the row's maximum
-//   2  top-k of up to FAST_K: what passes the bound (some 8 k elements) goes to
-//      one CTA, which sorts it and does the rest alone; otherwise
-//   3  top-k / top-p: histogram of counts and weights over bins linear in
-//      (max - x) / temperature; summed over the cluster, every CTA gets it
-//   4  the elements of the bin that the threshold falls in go to every CTA,
-//      which finds the threshold among them (narrowing by rank word)
-//   5  kept weight per warp, contiguous in the row; the warp in which the
-//      running sum passes u times the total walks its part
+// the cluster's meetings (about a microsecond each), so each way of filtering has
+// the fewest it can:
+//   greedy  the CTAs' maxima: one meeting
+//   top-k   of up to FAST_K: a CTA's k-th largest thread maximum bounds the row's
+//           k-th largest element; what passes (some 8 k elements) goes to one CTA,
+//           which sorts it, applies the other filters and draws alone: two
+//   top-p, other top-k   a histogram of counts and exact weights over 512 bins
+//           linear in (max - x) / temperature, summed over the cluster (again
+//           within the threshold's bin if that holds too many); the elements of
+//           the threshold's bin go to every CTA, which narrows them down and ranks
+//           the last few one against another: five (one more for both)
+//   none    the kept weight of each warp, whose part of the row is contiguous; the
+//           warp in which the running sum passes u times the total walks its part:
+//           two
+// Where that does not do (thousands of equal logits at a threshold) the threshold
+// is found bit by bit over the cluster.
+
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -59,37 +64,41 @@ struct Row {
   // floor(2^32 e) for e in [0, 1]: the significand, moved
   static __device__ __forceinline__ u64 w(float e) {
     const uint32_t b = __float_as_uint(e);
-    const int down = 126 - (int)(b >> 23);
-    if (down < 0) return 1ull << 32;  // e = 1
-    return down > 31 ? 0 : (((b & 0x7fffffu) | 0x800000u) << 8) >> down;
+    const uint32_t low = __funnelshift_rc((b << 8) | 0x80000000u, 0, 126 - (b >> 23));
+    return ((u64)((b + 0x00800000u) >> 30) << 32) | low;  // e = 1 alone has bit 32, and no lower bits
   }
+  // weight of a finite logit (max and inv are finite too), without branches
+  __device__ __forceinline__ u64 weight(float x) const { return w(expf(t(x))); }
 };
 
 // ---- rows in a cluster's shared memory -------------------------------------
-constexpr int NT = 512, NW = NT / 32;
-constexpr int NB = 1024;    // bins
-constexpr int CAP = 1024;   // elements of a bin that a CTA takes
-constexpr int FEW = 96;     // elements that are ranked one against another
-constexpr int C = 8;        // CTAs of a cluster
-constexpr int FAST_K = 100; // top-k that one CTA sorts: C * FAST_K candidates are expected, CAP fit
-constexpr int MAX_SLICE = 65528;  // weights' 16-bit halves sum to less than 2^32
+constexpr int NT = 256, NW = NT / 32, C = 8;
+constexpr int CAP = 2048;         // elements that a CTA lists
+constexpr int FEW = 256;          // elements that are ranked one against another
+constexpr int FAST_K = 100;       // top-k that one CTA sorts: some C * FAST_K candidates are expected, CAP fit
+constexpr int MAX_SLICE = 65528;  // elements per CTA
+constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
 constexpr float SPAN = 22.25f;    // e^-SPAN < 2^-32
 
+constexpr int OWN = 3 * BINS / 2; // elements that a CTA gives to the list
+
 struct Shared {
-  u64 list[2][CAP], lw[2][CAP];  // rank words and weights of the threshold bin: top-k's, top-p's
-  u64 gm[NB];                    // weights per bin, whole row
-  u64 sums[C], red[NW], red2[NW], few[FEW], few_w[FEW];
-  uint32_t hc[NB], hl[NB], hh[NB];  // this CTA's bins: counts, low and high halves of the weights
-  uint32_t gc[NB];                  // counts per bin, whole row
-  uint32_t nc[NB], nl[NB], nh[NB];  // narrowing
+  u64 list[CAP], few[FEW], weights[FEW];
+  u64 row_w[BINS];                                        // weights per bin, whole row
+  u64 warp_sums[C][NW], sums[2][C], part_red[NW][16], red[NW], out[2];
+  uint32_t row_c[BINS];                                   // counts
+  union {
+    struct {
+      uint32_t hc[BINS], hl[BINS], hh[BINS];              // this CTA's counts and halves of the weights
+    };
+    u64 own[OWN];                                         // its elements of one bin, afterwards
+  };
   float maxima[C];
-  int counts[C], n_fast;
-  u64 out_a, out_b, out_c;
-  int n_list, bin;
+  int counts[2][C], n_list, n_own, n_few, bin;
 };
 
 template <class V, class Op>
-__device__ V reduce(V v, Op op, V *shared) {  // over the block, to every thread
+__device__ __forceinline__ V reduce(V v, Op op, V *shared) {  // over the block, to every thread
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int w = 16; w; w >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, w));
@@ -101,46 +110,15 @@ __device__ V reduce(V v, Op op, V *shared) {  // over the block, to every thread
   for (int w = NW / 2; w; w >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, w));
   return v;
 }
+__device__ __forceinline__ u64 add64(u64 x, u64 y) { return x + y; }
 
-// Lowest key in (-inf, inf] that `yes` holds for, where it holds for `top` and
-// for every key above one it holds for: by one warp, first the 32 keys around a
-// guess, then 32 pivots at a time.
-template <class Yes>
-__device__ uint32_t lowest_key(uint32_t top, float guess, Yes yes) {
-  uint32_t lo = KEY_NEG_INF, hi = top;  // not at lo, at hi
-  const int lane = threadIdx.x & 31;
-  {
-    const uint32_t g = key_of(guess);
-    const uint32_t base = g > KEY_NEG_INF + 16 && g < top ? g - 16 : KEY_NEG_INF;
-    const uint32_t at = min(base + 1 + lane, hi);
-    const uint32_t m = __ballot_sync(0xffffffffu, yes(of_key(at)));
-    const int f = __ffs(m) - 1;
-    if (f > 0) return min(base + 1 + f, hi);
-    if (f == 0) hi = min(base + 1, hi);
-    else lo = base + 32;
-  }
-  while (hi - lo > 1) {
-    const uint32_t step = (hi - lo - 1) / 32 + 1;
-    const uint32_t off = step * (lane + 1), at = off < hi - lo ? lo + off : hi;
-    const uint32_t m = __ballot_sync(0xffffffffu, yes(of_key(at)));
-    const int f = __ffs(m) - 1;  // the last pivot is hi or above it
-    const uint32_t up = step * (f + 1);
-    hi = up < hi - lo ? lo + up : hi;
-    lo += step * f;
-  }
-  return hi;
-}
+// The steps below run once or twice a row: code that is shared is fetched once.
+__device__ __noinline__ u64 block_total(Shared &s, u64 v) { return reduce(v, add64, s.red); }
 
-// First bin, from bin 0, in which the running sum of get(bin) reaches `target`
-// (the last one if none does): its index and the sum before it, to every thread.
-template <int N, class Get>
-__device__ int crossing(Shared &s, u64 target, Get get, u64 *before) {
-  constexpr int PER = N / NT;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  u64 v[PER], sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) sum += v[i] = get(tid * PER + i);
-  u64 x = sum;
+// Exclusive sum over the block's threads; *total gets the sum.
+__device__ __noinline__ u64 scan(Shared &s, u64 v, u64 *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 x = v;
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
     const u64 y = __shfl_up_sync(0xffffffffu, x, w);
@@ -148,54 +126,121 @@ __device__ int crossing(Shared &s, u64 target, Get get, u64 *before) {
   }
   __syncthreads();
   if (lane == 31) s.red[warp] = x;
-  if (tid == 0) s.bin = N;
   __syncthreads();
-  u64 at = x - sum;
-  for (int w = 0; w < warp; ++w) at += s.red[w];
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += s.red[w];
+    all += s.red[w];
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// First bin in which the running sum of get(bin) reaches `target` (-1: none),
+// to every thread; the sum before it in s.out[0].
+template <int N, class Get>
+__device__ __forceinline__ int crossing(Shared &s, u64 target, Get get) {
+  constexpr int PER = N / NT;
+  const int tid = threadIdx.x;
+  u64 v[PER], own = 0, all;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) own += v[i] = get(tid * PER + i);
+  if (tid == 0) s.bin = -1;
+  u64 before = scan(s, own, &all);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (at < target && target <= at + v[i]) {
+    if (before < target && target <= before + v[i]) {
       s.bin = tid * PER + i;
-      s.out_a = at;
+      s.out[0] = before;
     }
-    at += v[i];
+    before += v[i];
   }
   __syncthreads();
-  *before = s.out_a;
   return s.bin;
 }
 
-// The rest of a row whose n candidates (rank words, at most CAP) hold its k
-// largest elements, by one CTA.
-__device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, int n, int k, float p, uint32_t key_pmin) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  u64 *list = s.list[0];
+// Lowest key in (-inf, inf] that `yes` holds for, where it holds for `top` and
+// for every key above one it holds for: by one warp, first the 32 keys around a
+// guess, then 32 pivots at a time.
+template <class Yes>
+__device__ __forceinline__ uint32_t lowest_key(uint32_t top, float guess, Yes yes) {
+  uint32_t lo = KEY_NEG_INF, hi = top;  // not at lo, at hi
+  const int lane = threadIdx.x & 31;
+  const uint32_t g = key_of(guess);
+  const uint32_t base = g > KEY_NEG_INF + 16 && g < top ? g - 16 : KEY_NEG_INF;
+  uint32_t step = 1, from = base;
+  while (true) {
+    const uint32_t off = step * (lane + 1), at = off < hi - from ? from + off : hi;
+    const uint32_t m = __ballot_sync(0xffffffffu, yes(of_key(at)));
+    const int f = __ffs(m) - 1;  // first pivot it holds for
+    if (f < 0) {
+      lo = from + 32 * step;  // (only around the guess: else the last pivot is hi)
+    } else {
+      const uint32_t up = step * (f + 1);
+      const uint32_t was = from;
+      if (up < hi - from) hi = from + up;
+      if (f > 0) lo = was + step * f;
+    }
+    if (hi - lo <= 1) return hi;
+    from = lo;
+    step = (hi - lo - 1) / 32 + 1;
+  }
+}
+
+// Fine bin of a logit, and the lowest logit of the bins up to q (NaN, which no
+// logit is at or above, for q < 0).
+__device__ __forceinline__ int bin_of(const Row &f, float x) { return min(QN - 1, (int)__fmul_rn(f.t(x), -(float)QN / SPAN)); }
+__device__ __noinline__ float edge_of(float max, float inv, float temp, int q) {
+  if (q < 0) return __uint_as_float(0x7fc00000u);
+  const Row f{max, inv};
+  return of_key(lowest_key(key_of(max), max - (float)(q + 1) * (SPAN / QN) * temp, [&](float x) { return bin_of(f, x) <= q; }));
+}
+
+// Sorts list[0, n), n <= CAP, largest first (a bitonic network, padded with zeros
+// to a power of two).
+__device__ void sort_down(u64 *list, int n) {
   int N = 64;
   while (N < n) N *= 2;
-  for (int i = n + tid; i < N; i += NT) list[i] = 0;
+  for (int i = n + threadIdx.x; i < N; i += NT) list[i] = 0;
   __syncthreads();
-  // bitonic, largest first; a warp keeps the 64 elements of its short strides to itself
   for (int size = 2; size <= N; size *= 2)
     for (int stride = size / 2; stride; stride /= 2) {
-      if (tid < N / 2) {
-        const int i = 2 * tid - (tid & (stride - 1)), j = i + stride;
+#pragma unroll
+      for (int m = 0; m < CAP / 2 / NT; ++m) {
+        const int q = threadIdx.x + m * NT;
+        if (q >= N / 2) break;
+        const int i = 2 * q - (q & (stride - 1)), j = i + stride;
         const u64 x = list[i], y = list[j];
         if ((x < y) == ((i & size) == 0)) {
           list[i] = y;
           list[j] = x;
         }
       }
-      // the next stride's elements are this warp's own while it is at most 32
+      // while the stride is at most 32, the next one's elements are this warp's own
       if (stride > 1 && stride <= 32) __syncwarp();
       else __syncthreads();
     }
+}
+
+// The random place among `total`.
+__device__ __forceinline__ u64 place(float u, u64 total) {
+  const u64 at = (u64)((double)(u > 0.f ? u : 0.f) * (double)total);
+  return at < total ? at : total - 1;
+}
+
+// The rest of a row whose n candidates (rank words in s.list) hold its k largest
+// elements, by one CTA.
+__device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, int n, int k, float p, uint32_t key_pmin) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  sort_down(s.list, n);
   const int m = min(k, n);
   static_assert(FAST_K <= 128, "four warps hold the k largest");
   u64 w = 0, sum = 0;
   uint32_t key = 0;
   if (tid < 128) {
     if (tid < m) {
-      key = (uint32_t)(list[tid] >> IDX_BITS);
+      key = (uint32_t)(s.list[tid] >> IDX_BITS);
       w = Row::w(f.e(of_key(key)));
     }
     sum = w;
@@ -213,77 +258,162 @@ __device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, i
     const double want = (double)p * (double)W;
     const u64 T = p < 1.f ? (want >= 1.0 ? (u64)want : 1) : ~0ull;
     const bool keep = tid < m && sum - w < T && key >= key_pmin;
-    s.lw[0][tid] = keep ? w : 0;
+    s.weights[tid] = keep ? w : 0;
   }
   __syncthreads();
   if (tid < 128) {
-    const u64 own = s.lw[0][tid];
+    const u64 own = s.weights[tid];
     u64 total = 0, upto = 0;  // of all, and of those up to this one in index order
     for (int i = 0; i < m; ++i) {
-      const u64 x = s.lw[0][i];
+      const u64 x = s.weights[i];
       total += x;
-      if (tid < m && (list[i] & (MAX_VOCAB - 1)) >= (list[tid] & (MAX_VOCAB - 1))) upto += x;
+      if (tid < m && (s.list[i] & (MAX_VOCAB - 1)) >= (s.list[tid] & (MAX_VOCAB - 1))) upto += x;
     }
-    const float u = a.u[r];
-    u64 at = (u64)((double)(u > 0.f ? u : 0.f) * (double)total);
-    at = at < total ? at : total - 1;
-    if (own && upto > at && upto - own <= at) a.tokens[r] = (int)(MAX_VOCAB - 1 - (list[tid] & (MAX_VOCAB - 1)));
+    const u64 at = place(a.u[r], total);
+    if (own && upto > at && upto - own <= at) a.tokens[r] = (int)(MAX_VOCAB - 1 - (s.list[tid] & (MAX_VOCAB - 1)));
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(NT, 2) cluster_kernel(const __grid_constant__ Args a, int slice) {
-  constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ __align__(16) uint8_t smem[];
-  Shared &s = *reinterpret_cast<Shared *>(smem);
-  T *xs = reinterpret_cast<T *>(smem + (sizeof(Shared) + 15) / 16 * 16);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t r = blockIdx.x / C;
-  const int V = (int)a.vocab, i0 = rank * slice, n = max(0, min(slice, V - i0));
-  const T *row = static_cast<const T *>(a.logits) + r * a.row_stride + i0;
-  // vectors of this warp: contiguous, [v0, v1)
-  const int nv = (n + VEC - 1) / VEC, per = (nv + NW - 1) / NW, v0 = min(nv, warp * per), v1 = min(nv, v0 + per);
-  auto get = [](const uint4 &q, int j) -> float {
+struct Slice {  // a CTA's part of a row, in shared memory
+  static constexpr int VEC = 16 / sizeof(T);
+  const uint4 *xv;
+  int i0, v0, v1;  // first index; this warp's vectors
+  __device__ static __forceinline__ float get(const uint4 &q, int j) {
     const uint32_t w = (&q.x)[j / (VEC / 4)];
     float x;
     if constexpr (sizeof(T) == 4) x = __uint_as_float(w);
     else if constexpr (std::is_same<T, __half>::value) x = __half2float(__ushort_as_half((unsigned short)(j & 1 ? w >> 16 : w)));
     else x = __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
     return x + 0.f;
-  };
-  const uint4 *xv = reinterpret_cast<const uint4 *>(xs);
-
-  // 1  logits to shared memory; the tail of the last vector is -inf
-  float m0 = -INFINITY, m1 = -INFINITY;  // this thread's maxima: even and odd steps
-  if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(row);
-    const int full = n / VEC;
-#pragma unroll 4
-    for (int v = tid; v < full; v += NT) reinterpret_cast<uint4 *>(xs)[v] = __ldcs(src + v);
-    for (int i = full * VEC + tid; i < nv * VEC; i += NT) xs[i] = i < n ? row[i] : (T)(-INFINITY);
-  } else {
-#pragma unroll 4
-    for (int i = tid; i < nv * VEC; i += NT) xs[i] = i < n ? row[i] : (T)(-INFINITY);
   }
-  __syncthreads();
-  for (int v = v0 + lane, odd = 0; v < v1; v += 32, odd ^= 1) {
-    const uint4 q = xv[v];
+  __device__ static __forceinline__ float top(const uint4 &q) {
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) m = fmaxf(m, get(q, j));  // NaN is passed over
-    if (odd) m1 = fmaxf(m1, m);
-    else m0 = fmaxf(m0, m);
+    return m;
   }
+  // f(x, index of the first) for this warp's vectors (FEW: those that have an element from `cut` up)
+  template <bool FEW, class F>
+  __device__ __forceinline__ void vectors(float cut, F f) const {
+    for (int v = v0 + (threadIdx.x & 31); v < v1; v += 32) {
+      const uint4 q = xv[v];
+      if (FEW && !(top(q) >= cut)) continue;
+      float x[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = get(q, j);
+      f(x, i0 + v * VEC);
+    }
+  }
+  // the same for the vectors that have an element in [from, to)
+  template <class F>
+  __device__ __forceinline__ void between(float from, float to, F f) const {
+    vectors<true>(from, [&](const float (&x)[VEC], int first) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) any |= x[j] >= from && !(x[j] >= to);
+      if (any) f(x, first);
+    });
+  }
+  // f(x, index) for this warp's elements from `cut` up (never NaN), where they are few
+  template <class F>
+  __device__ __forceinline__ void each(float cut, F f) const {
+    vectors<true>(cut, [&](const float (&x)[VEC], int first) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (x[j] >= cut) f(x[j], first + j);
+    });
+  }
+};
+
+// The largest rank word that `target` elements (count) or a weight of `target`
+// reach, among the elements with rank words from `least`; *mass: the weight from
+// it up.  Bit by bit, every CTA of the cluster together.
+template <class T>
+__device__ __noinline__ u64 find_slowly(Shared &s, const Slice<T> &x, const Row &f, float cut, bool count, u64 target,
+                                        u64 least, u64 *mass) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  int turn = 0;
+  cluster.sync();  // the sums, which are used for other things before, are read
+  auto measure = [&](u64 from, bool by_count) {
+    u64 sum = 0;
+    x.each(cut, [&](float y, int i) {
+      const u64 word = rank_word(key_of(y), i);
+      if (word >= from && word >= least) sum += by_count ? 1 : f.weight(y);
+    });
+    sum = reduce(sum, add64, s.red);
+    // a CTA can be one turn ahead of another, not two
+    if (threadIdx.x < C) cluster.map_shared_rank(s.sums[turn & 1], threadIdx.x)[rank] = sum;
+    cluster.sync();
+    u64 all = 0;
+    for (int c = 0; c < C; ++c) all += s.sums[turn & 1][c];
+    ++turn;
+    return all;
+  };
+  u64 word = 0;
+  if (measure(0, count) > target || !count) {
+    for (int bit = 52; bit >= 0; --bit)
+      if (measure(word | (1ull << bit), count) >= target) word |= 1ull << bit;
+  }
+  *mass = measure(word, false);
+  cluster.sync();  // the sums are read
+  return word;
+}
+
+template <class T>
+__global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ Args a, int slice) {
+  using X = Slice<T>;
+  constexpr int VEC = X::VEC;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Shared &s = *reinterpret_cast<Shared *>(smem);
+  T *xs = reinterpret_cast<T *>(smem + (sizeof(Shared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // another CTA's shared memory may be touched once all have begun: waited for below
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int64_t r = blockIdx.x / C;
+  const int V = (int)a.vocab, i0 = rank * slice, n = max(0, min(slice, V - i0));
+  const T *row = static_cast<const T *>(a.logits) + r * a.row_stride + i0;
+  // vectors of this warp: contiguous, [v0, v1)
+  const int nv = (n + VEC - 1) / VEC, per = (nv + NW - 1) / NW;
+  const X x{reinterpret_cast<const uint4 *>(xs), i0, min(nv, warp * per), min(nv, (warp + 1) * per)};
+
+  // logits to shared memory, two maxima a thread; the tail of the last vector is -inf
+  float m0 = -INFINITY, m1 = -INFINITY;
+  const int full = (reinterpret_cast<uintptr_t>(row) & 15) == 0 ? n / VEC : 0;  // vectors that can be read as such
+  constexpr int U = 5;
+  for (int v = tid; v < full; v += U * NT) {
+    uint4 q[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < full) q[i] = __ldcs(reinterpret_cast<const uint4 *>(row) + v + i * NT);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < full) {
+        reinterpret_cast<uint4 *>(xs)[v + i * NT] = q[i];
+        float &m = i & 1 ? m1 : m0;
+        m = fmaxf(m, X::top(q[i]));
+      }
+  }
+  if (full < nv) {
+#pragma unroll 4
+    for (int i = full * VEC + tid; i < nv * VEC; i += NT) xs[i] = i < n ? row[i] : (T)(-INFINITY);
+    __syncthreads();
+    for (int v = full + tid; v < nv; v += NT) m0 = fmaxf(m0, X::top(x.xv[v]));
+  }
+  for (int i = tid; i < BINS; i += NT) s.hc[i] = s.hl[i] = s.hh[i] = 0;
+  if (tid == 0) s.n_list = s.n_own = 0;
   {
     const float m = reduce(fmaxf(m0, m1), [](float x, float y) { return fmaxf(x, y); }, reinterpret_cast<float *>(s.red));
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < C) cluster.map_shared_rank(s.maxima, tid)[rank] = m;
   }
-  if (tid == 0) s.n_fast = 0;
   cluster.sync();
   float gmax = -INFINITY;
   int owner = 0;  // lowest rank that has the maximum
+#pragma unroll
   for (int c = C - 1; c >= 0; --c)
     if (s.maxima[c] >= gmax) {
       gmax = s.maxima[c];
@@ -294,339 +424,346 @@ __global__ void __launch_bounds__(NT, 2) cluster_kernel(const __grid_constant__ 
     return;
   }
   const float temp = a.temperature ? a.temperature[r] : 1.f;
-  auto add = [](u64 x, u64 y) { return x + y; };
-  auto low = [](u64 x, u64 y) { return x < y ? x : y; };
-  auto high = [](u64 x, u64 y) { return x > y ? x : y; };
   if (!(temp > 0.f)) {
     if (rank != owner) return;
     u64 first = V;
-    for (int v = v0 + lane; v < v1; v += 32) {
-      const uint4 q = xv[v];
-      for (int j = VEC - 1; j >= 0; --j)
-        if (get(q, j) == gmax) first = min(first, (u64)(i0 + v * VEC + j));
-    }
-    first = reduce(first, low, s.red);
+    x.each(gmax, [&](float, int i) { first = min(first, (u64)i); });
+    first = reduce(first, [](u64 x, u64 y) { return x < y ? x : y; }, s.red);
     if (tid == 0) a.tokens[r] = (int)first;
     return;
   }
 
-  const Row f{gmax, 1.f / temp};
+  if (gmax == INFINITY) {  // only the infinite logits have a weight, all the same: ones among -infinities
+    for (int i = tid; i < nv * VEC; i += NT) xs[i] = (float)xs[i] == INFINITY ? (T)1.f : (T)(-INFINITY);
+    gmax = 1.f;
+    m0 = fmaxf(m0, m1) == INFINITY ? 1.f : -INFINITY;
+    m1 = -INFINITY;
+    __syncthreads();
+  }
+  const Row f{gmax, fminf(1.f / temp, 3.4028235e38f)};
   const uint32_t kmax = key_of(gmax);
-  auto bin_of = [&](float x) { return min(NB - 1, (int)__fmul_rn(f.t(x), -(float)NB / SPAN)); };
+  auto bin = [&](float x) { return bin_of(f, x); };
+  auto edge = [&](int q) { return edge_of(gmax, f.inv, temp, q); };
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.f;
   const bool by_count = k > 0 && k < V, by_mass = p < 1.f;
   float pmin = a.min_p ? a.min_p[r] : 0.f;
   pmin = pmin > 1.f ? 1.f : pmin;
   // the lowest logit that has a weight: below it (and NaN) nothing matters
-  float cut = of_key(lowest_key(kmax, gmax - 22.180709f * temp, [&](float x) { return Row::w(f.e(x)) > 0; }));
-  // lowest logit of the bins up to b
-  auto bin_end = [&](int b) {
-    return lowest_key(kmax, gmax - (float)(b + 1) * (SPAN / NB) * temp, [&](float x) { return bin_of(x) <= b; });
-  };
+  const float cut = of_key(lowest_key(kmax, gmax - 22.180709f * temp, [&](float x) { return Row::w(f.e(x)) > 0; }));
   const uint32_t key_pmin = pmin > 0.f ? lowest_key(kmax, gmax + logf(pmin) * temp, [&](float x) { return f.e(x) >= pmin; }) : 0;
-  u64 thr = 0;  // rank word of the last kept element
+  u64 thr = 0;  // rank word of the last element that is kept
 
-  if (by_count || by_mass) {
-    for (int i = tid; i < NB; i += NT) s.hc[i] = s.hl[i] = s.hh[i] = 0;
+  if (by_count && k <= FAST_K) {
+    if (m0 >= cut) atomicAdd(&s.hc[bin(m0) / BINS], 1u);
+    if (m1 >= cut) atomicAdd(&s.hc[bin(m1) / BINS], 1u);
     __syncthreads();
-    float cut_k = cut;
-    if (by_count && k <= 2 * NT) {
-      // k of this CTA's thread maxima lie in the bins up to b: so do the row's k largest
-      if (m0 >= cut) atomicAdd(&s.hc[bin_of(m0)], 1u);
-      if (m1 >= cut) atomicAdd(&s.hc[bin_of(m1)], 1u);
-      __syncthreads();
-      u64 before;
-      const int b = crossing<NB>(s, (u64)k, [&](int i) { return (u64)s.hc[i]; }, &before);
-      if (b < NB) cut_k = fmaxf(cut, of_key(bin_end(b)));
-      if (k <= FAST_K) {
-        // 2  candidates to rank 0; how many there are, to everyone
-        int mine = 0;
-        for (int v = v0 + lane; v < v1; v += 32) {
-          const uint4 q = xv[v];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float x = get(q, j);
-            if (x >= cut_k) {
-              ++mine;
-              const int at = atomicAdd(cluster.map_shared_rank(&s.n_fast, 0), 1);
-              if (at < CAP) cluster.map_shared_rank(s.list[0], 0)[at] = rank_word(key_of(x), i0 + v * VEC + j);
-            }
-          }
-        }
-        mine = reduce(mine, [](int x, int y) { return x + y; }, reinterpret_cast<int *>(s.red));
-        if (tid < C) cluster.map_shared_rank(s.counts, tid)[rank] = mine;
-        cluster.sync();
-        int all = 0;
-#pragma unroll
-        for (int c = 0; c < C; ++c) all += s.counts[c];
-        if (all <= CAP) {
-          if (rank == 0) draw_sorted(s, a, r, f, all, k, p, key_pmin);
-          return;
-        }
-      }
-      for (int i = tid; i < NB; i += NT) s.hc[i] = 0;
-      __syncthreads();
-    }
-    // 3  histogram
-    for (int v = v0 + lane; v < v1; v += 32) {
-      const uint4 q = xv[v];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float x = get(q, j);
-        if (x >= cut_k) {
-          const u64 full = Row::w(f.e(x));
-          const int b = bin_of(x);
-          atomicAdd(&s.hc[b], 1u);
-          atomicAdd(&s.hl[b], (uint32_t)full & 0xffffu);
-          atomicAdd(&s.hh[b], (uint32_t)(full >> 16));
-        }
-      }
-    }
+    // k of this CTA's thread maxima lie in the bins up to b: so do the row's k largest
+    const int b = crossing<BINS>(s, (u64)k, [&](int i) { return (u64)s.hc[i]; });
+    const float cut_k = b >= 0 ? fmaxf(cut, edge(BINS * b + BINS - 1)) : cut;
+    int mine = 0;
+    x.each(cut_k, [&](float y, int i) {
+      ++mine;
+      const int at = atomicAdd(cluster.map_shared_rank(&s.n_list, 0), 1);
+      if (at < CAP) cluster.map_shared_rank(s.list, 0)[at] = rank_word(key_of(y), i);
+    });
+    mine = reduce(mine, [](int x, int y) { return x + y; }, reinterpret_cast<int *>(s.red));
+    if (tid < C) cluster.map_shared_rank(&s.counts[0][0], tid)[rank] = mine;
     cluster.sync();
-    for (int i = rank * (NB / C) + tid; i < (rank + 1) * (NB / C); i += NT) {
-      uint32_t c = 0;
-      u64 m = 0;
-      for (int o = 0; o < C; ++o) {
-        c += cluster.map_shared_rank(s.hc, o)[i];
-        m += cluster.map_shared_rank(s.hl, o)[i] + ((u64)cluster.map_shared_rank(s.hh, o)[i] << 16);
-      }
-      for (int o = 0; o < C; ++o) {
-        cluster.map_shared_rank(s.gc, o)[i] = c;
-        cluster.map_shared_rank(s.gm, o)[i] = m;
-      }
+    int sum = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum += s.counts[0][c];
+    if (sum <= CAP) {
+      if (rank == 0) draw_sorted(s, a, r, f, sum, k, p, key_pmin);
+      return;
     }
-    cluster.sync();
+    if (tid == 0) s.n_list = 0;
+    for (int i = tid; i < BINS; i += NT) s.hc[i] = 0;
+    __syncthreads();
+  }
 
-    // 4  the element at which the running count (or weight), from the largest
-    // element down, reaches `target`: its rank word; *mass: weight up to it
-    auto find = [&](bool count, u64 target, int buf, u64 *mass) -> u64 {
-      u64 before, other;
-      const int b = count ? crossing<NB>(s, target, [&](int i) { return (u64)s.gc[i]; }, &before)
-                          : crossing<NB>(s, target, [&](int i) { return s.gm[i]; }, &before);
-      if (b >= NB) {  // fewer elements have a weight: all are kept
-        *mass = reduce((u64)(s.gm[2 * tid] + s.gm[2 * tid + 1]), add, s.red);
-        return 0;
-      }
-      {  // the other measure before the bin
-        u64 o = 0;
-        for (int i = tid; i < b; i += NT) o += count ? s.gm[i] : (u64)s.gc[i];
-        other = reduce(o, add, s.red);
-      }
-      u64 acc_w = count ? other : before, acc = before;  // weight, and the target's measure, before the range
-      const uint32_t k_lo = bin_end(b), k_hi = b ? bin_end(b - 1) - 1 : kmax;
-      u64 lo = rank_word(k_lo, (int)MAX_VOCAB - 1), hi = rank_word(k_hi, 0);  // range of rank words
-      const float x_lo = fmaxf(of_key(k_lo), cut), x_hi = of_key(k_hi);
-      uint32_t cnt = s.gc[b];
-      uint32_t mine_before = 0;  // elements of the range in lower ranks
-      if (cnt <= CAP) {
-        for (int o = 0; o < rank; ++o) mine_before += cluster.map_shared_rank(s.hc, o)[b];
-      }
-      while (cnt > CAP) {
-        // narrow the range over the whole cluster, NB parts at a time
-        const int shift = max(0, 64 - __clzll(hi - lo) - 10);
-        cluster.sync();  // earlier reads of the narrowing bins are done
-        for (int i = tid; i < NB; i += NT) s.nc[i] = s.nl[i] = s.nh[i] = 0;
-        __syncthreads();
-        for (int v = v0 + lane; v < v1; v += 32) {
-          const uint4 q = xv[v];
-          for (int j = 0; j < VEC; ++j) {
-            const float x = get(q, j);
-            if (x < x_lo || !(x <= x_hi)) continue;
-            const u64 word = rank_word(key_of(x), i0 + v * VEC + j);
-            if (word < lo || word > hi) continue;
-            const int i = (int)((hi - word) >> shift);
-            const u64 w = Row::w(f.e(x));
-            atomicAdd(&s.nc[i], 1u);
-            atomicAdd(&s.nl[i], (uint32_t)w & 0xffffu);
-            atomicAdd(&s.nh[i], (uint32_t)(w >> 16));
-          }
-        }
-        cluster.sync();
-        auto all_c = [&](int i) {
-          u64 c = 0;
-          for (int o = 0; o < C; ++o) c += cluster.map_shared_rank(s.nc, o)[i];
-          return c;
-        };
-        auto all_w = [&](int i) {
-          u64 w = 0;
-          for (int o = 0; o < C; ++o)
-            w += cluster.map_shared_rank(s.nl, o)[i] + ((u64)cluster.map_shared_rank(s.nh, o)[i] << 16);
-          return w;
-        };
-        u64 in;
-        const int part = count ? crossing<NB>(s, target - acc, all_c, &in) : crossing<NB>(s, target - acc, all_w, &in);
-        u64 o = 0;
-        for (int i = tid; i < part; i += NT) o += all_w(i);
-        acc_w += reduce(o, add, s.red);
-        acc += in;
-        hi -= (u64)part << shift;
-        const u64 width = ((u64)1 << shift) - 1;
-        lo = hi - lo > width ? hi - width : lo;
-        cnt = (uint32_t)all_c(part);
-        mine_before = 0;
-        for (int o = 0; o < rank; ++o) mine_before += cluster.map_shared_rank(s.nc, o)[part];
-      }
-      // the range's elements, to every CTA of the cluster
-      if (tid == 0) s.n_list = 0;
-      __syncthreads();
-      for (int v = v0 + lane; v < v1; v += 32) {
-        const uint4 q = xv[v];
+  // top-k, then top-p
+  if (by_count || by_mass) {
+    // fine bins `base` .. of 2^shift each: counts and weights of the row's elements in 512 of them, to every CTA
+    auto histogram = [&](float from, float end, int base, int shift) {
+      x.between(from, end, [&](const float (&y)[VEC], int) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float x = get(q, j);
-          if (!(x >= x_lo) || x > x_hi) continue;
-          const u64 word = rank_word(key_of(x), i0 + v * VEC + j);
-          if (word < lo || word > hi) continue;
-          const int at = (int)mine_before + atomicAdd(&s.n_list, 1);
-          const u64 w = Row::w(f.e(x));
-          for (int o = 0; o < C; ++o) {
-            cluster.map_shared_rank(s.list[buf], o)[at] = word;
-            cluster.map_shared_rank(s.lw[buf], o)[at] = w;
-          }
+        for (int i = 0; i < VEC; ++i) {
+          if (!(y[i] >= from) || y[i] >= end) continue;
+          const u64 w = f.weight(y[i]);
+          const int b = (bin(y[i]) - base) >> shift;
+          if (by_count) atomicAdd(&s.hc[b], 1u);
+          atomicAdd(&s.hl[b], (uint32_t)w & 0xffffu);
+          atomicAdd(&s.hh[b], (uint32_t)(w >> 16));
+        }
+      });
+      cluster.sync();
+      if (tid < BINS / C) {
+        const int b = rank * (BINS / C) + tid;
+        uint32_t c = 0;
+        u64 w = 0;
+#pragma unroll
+        for (int o = 0; o < C; ++o) {
+          c += cluster.map_shared_rank(s.hc, o)[b];
+          w += cluster.map_shared_rank(s.hl, o)[b] + ((u64)cluster.map_shared_rank(s.hh, o)[b] << 16);
+        }
+#pragma unroll
+        for (int o = 0; o < C; ++o) {
+          cluster.map_shared_rank(s.row_c, o)[b] = c;
+          cluster.map_shared_rank(s.row_w, o)[b] = w;
         }
       }
       cluster.sync();
-      const u64 *list = s.list[buf], *lw = s.lw[buf];
-      const int total = (int)cnt;
-      while (cnt > FEW) {  // narrow the range within the list
-        u64 mn = ~0ull, mx = 0;
-        for (int i = tid; i < total; i += NT)
-          if (list[i] >= lo && list[i] <= hi) {
-            mn = min(mn, list[i]);
-            mx = max(mx, list[i]);
-          }
-        lo = reduce(mn, low, s.red);
-        hi = reduce(mx, high, s.red2);
-        const int shift = max(0, 64 - __clzll(hi - lo) - 10);
-        for (int i = tid; i < NB; i += NT) s.nc[i] = s.nl[i] = s.nh[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < total; i += NT)
-          if (list[i] >= lo && list[i] <= hi) {
-            const int at = (int)((hi - list[i]) >> shift);
-            atomicAdd(&s.nc[at], 1u);
-            atomicAdd(&s.nl[at], (uint32_t)lw[i] & 0xffffu);
-            atomicAdd(&s.nh[at], (uint32_t)(lw[i] >> 16));
-          }
-        __syncthreads();
-        auto part_w = [&](int i) { return s.nl[i] + ((u64)s.nh[i] << 16); };
-        u64 in;
-        const int part = count ? crossing<NB>(s, target - acc, [&](int i) { return (u64)s.nc[i]; }, &in)
-                               : crossing<NB>(s, target - acc, part_w, &in);
-        u64 o = 0;
-        for (int i = tid; i < part; i += NT) o += part_w(i);
-        acc_w += reduce(o, add, s.red);
-        acc += in;
-        hi -= (u64)part << shift;
-        const u64 width = ((u64)1 << shift) - 1;
-        lo = hi - lo > width ? hi - width : lo;
-        cnt = s.nc[part];
-        __syncthreads();
-      }
-      if (tid == 0) s.n_list = 0;
-      __syncthreads();
-      for (int i = tid; i < total; i += NT)
-        if (list[i] >= lo && list[i] <= hi) {
-          const int at = atomicAdd(&s.n_list, 1);
-          s.few[at] = list[i];
-          s.few_w[at] = lw[i];
-        }
-      __syncthreads();
-      const int few = s.n_list;
-      if (tid < few) {
-        const u64 me = s.few[tid], w = s.few_w[tid];
-        u64 c = 0, m = 0;
-        for (int j = 0; j < few; ++j)
-          if (s.few[j] > me) {
-            ++c;
-            m += s.few_w[j];
-          }
-        const u64 ex = acc + (count ? c : m), own = count ? 1 : w;
-        if (ex < target && target <= ex + own) {
-          s.out_b = me;
-          s.out_c = acc_w + m + w;
-        }
-      }
-      __syncthreads();
-      *mass = s.out_c;
-      return s.out_b;
     };
-
-    u64 W;
-    if (by_count) thr = find(true, (u64)k, 0, &W);
-    else W = reduce((u64)(s.gm[2 * tid] + s.gm[2 * tid + 1]), add, s.red);
-    if (by_mass) {
+    auto weight_before = [&](int n) {  // of the first n bins
+      u64 v = 0;
+      for (int i = tid; i < n; i += NT) v += s.row_w[i];
+      return block_total(s, v);
+    };
+    const float none = __uint_as_float(0x7fc00000u);  // NaN: no logit is at or above it
+    histogram(cut, none, 0, 9);
+    u64 W = weight_before(BINS);  // weight that top-p divides
+    int fine = -1;  // the bin that has been looked at closer
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+      const bool mass = round;
+      if (!(mass ? by_mass : by_count)) continue;
       const double want = (double)p * (double)W;
-      u64 dummy;
-      const u64 t = find(false, want >= 1.0 ? (u64)want : 1, 1, &dummy);
-      thr = max(thr, t);
+      const u64 target = mass ? (want >= 1.0 ? (u64)want : 1) : (u64)k;
+      if (fine >= 0) {  // top-k looked closer into a bin: the whole range again
+        for (int i = tid; i < BINS; i += NT) s.hc[i] = s.hl[i] = s.hh[i] = 0;
+        __syncthreads();
+        histogram(cut, none, 0, 9);
+        fine = -1;
+      }
+      float from = cut, end = none;
+      u64 before = 0, above_w = 0;  // of what lies above the range: the round's measure, and the weight
+      int base = 0, shift = 9;
+      int n = 0;
+      while (true) {
+        const int b = crossing<BINS>(s, target - before, [&](int i) { return mass ? s.row_w[i] : (u64)s.row_c[i]; });
+        if (b < 0) break;  // fewer elements have a weight (a rounding at most, for a weight)
+        before += s.out[0];
+        above_w += weight_before(b);
+        const int q = base + (b << shift);
+        from = fmaxf(from, edge(q + (1 << shift) - 1));
+        const float up = edge(q - 1);
+        end = b ? up : end;
+        // the bin's elements, to every CTA (each has them in an order of its own)
+        x.between(from, end, [&](const float (&y)[VEC], int first) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            if (!(y[i] >= from) || y[i] >= end) continue;
+            const int at = atomicAdd(&s.n_own, 1);
+            if (at < OWN) s.own[at] = rank_word(key_of(y[i]), first + i);
+          }
+        });
+        __syncthreads();
+        const int mine = s.n_own;
+        if (tid < C) cluster.map_shared_rank(&s.counts[shift ? 0 : 1][0], tid)[rank] = mine;
+        cluster.sync();
+        int first = 0;
+        bool fits = true;
+        n = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int m = s.counts[shift ? 0 : 1][c];
+          if (c == rank) first = n;
+          fits &= m <= OWN;
+          n += m;
+        }
+        fits &= n <= CAP;
+        if (fits) {
+          for (int i = tid; i < C * mine; i += NT) {
+            const int to = i / mine, j = i - to * mine;
+            cluster.map_shared_rank(s.list, to)[first + j] = s.own[j];
+          }
+          cluster.sync();
+          break;
+        }
+        n = 0;
+        if (shift == 0) break;
+        if (tid == 0) s.n_own = 0;
+        for (int i = tid; i < BINS; i += NT) s.hc[i] = s.hl[i] = s.hh[i] = 0;
+        __syncthreads();
+        base = fine = q;
+        shift = 0;
+        histogram(from, end, base, 0);
+      }
+      const bool ok = n > 0;
+      u64 found = 0, found_w = 0;
+      if (ok) {
+        // narrow the list's range of rank words until few are left
+        u64 lo = 0, hi = ~0ull >> 1;
+        int in = n;
+        while (in > FEW) {
+          u64 mn = ~0ull, mx = 0;
+          for (int i = tid; i < n; i += NT) {
+            const u64 word = s.list[i];
+            if (word < lo || word > hi) continue;
+            mn = min(mn, word);
+            mx = max(mx, word);
+          }
+          lo = reduce(mn, [](u64 x, u64 y) { return x < y ? x : y; }, s.red);
+          hi = reduce(mx, [](u64 x, u64 y) { return x > y ? x : y; }, s.red);
+          const int down = max(0, 64 - __clzll(hi - lo) - 3);
+          u64 m[8], c[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m[j] = c[j] = 0;
+          for (int i = tid; i < n; i += NT) {
+            const u64 word = s.list[i];
+            if (word < lo || word > hi) continue;
+            const u64 w = f.weight(of_key((uint32_t)(word >> IDX_BITS)));
+            const int g = (int)((hi - word) >> down);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              m[j] += g == j ? w : 0;
+              c[j] += g == j;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int w = 16; w; w >>= 1) {
+              m[j] += __shfl_xor_sync(0xffffffffu, m[j], w);
+              c[j] += __shfl_xor_sync(0xffffffffu, c[j], w);
+            }
+            if (lane == 0) {
+              s.part_red[warp][j] = m[j];
+              s.part_red[warp][8 + j] = c[j];
+            }
+          }
+          __syncthreads();
+          int g = 0;
+          for (; g < 8; ++g) {
+            u64 gm = 0, gc = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+              gm += s.part_red[w][g];
+              gc += s.part_red[w][8 + g];
+            }
+            if (before + (mass ? gm : gc) >= target || g == 7) {
+              in = (int)gc;
+              break;
+            }
+            before += mass ? gm : gc;
+            above_w += gm;
+          }
+          __syncthreads();
+          hi -= (u64)g << down;
+          const u64 size = ((u64)1 << down) - 1;
+          lo = hi - lo > size ? hi - size : lo;
+        }
+        if (tid == 0) {
+          s.n_few = 0;
+          s.out[0] = 0;
+        }
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+          const u64 word = s.list[i];
+          if (word < lo || word > hi) continue;
+          const int at = atomicAdd(&s.n_few, 1);
+          s.few[at] = word;
+          s.weights[at] = f.weight(of_key((uint32_t)(word >> IDX_BITS)));
+        }
+        __syncthreads();
+        // the element at which the running count or weight, largest first, reaches the target
+        if (tid < in) {
+          const u64 me = s.few[tid], w = s.weights[tid];
+          u64 c = 0, m = 0;
+#pragma unroll 8
+          for (int j = 0; j < in; ++j) {
+            const bool above = s.few[j] > me;
+            c += above;
+            m += above ? s.weights[j] : 0;
+          }
+          const u64 ex = before + (mass ? m : c), own = mass ? w : 1;
+          if (ex < target && target <= ex + own) {
+            s.out[0] = me;
+            s.out[1] = above_w + m + w;
+          }
+        }
+        __syncthreads();
+        found = s.out[0];
+        found_w = s.out[1];
+      }
+      if (!found) found = find_slowly(s, x, f, cut, !mass, target, thr, &found_w);
+      thr = max(thr, found);
+      W = found_w;
+      if (round == 0 && by_mass) {  // the list is used again
+        cluster.sync();
+        if (tid == 0) s.n_own = 0;
+        __syncthreads();
+      }
     }
   }
 
-  // 5  kept weight, in index order
-  const uint32_t thr_key = (uint32_t)(thr >> IDX_BITS);
-  const int thr_idx = (int)(MAX_VOCAB - 1 - (thr & (MAX_VOCAB - 1)));  // of the elements equal to it, up to this index
-  if (thr) cut = fmaxf(cut, of_key(thr_key));
-  if (pmin > 0.f) cut = fmaxf(cut, of_key(key_pmin));
-  const float tie = thr ? of_key(thr_key) : -INFINITY;
-  auto kept = [&](float x, int i) -> u64 {  // weight of element i, 0 if it is not kept
-    if (!(x >= cut) || (x == tie && i > thr_idx)) return 0;
-    return Row::w(f.e(x));
+  // the kept weight of each warp, to everyone
+  const float from = fmaxf(fmaxf(cut, thr ? of_key((uint32_t)(thr >> IDX_BITS)) : -INFINITY), key_pmin ? of_key(key_pmin) : -INFINITY);
+  const float tie = thr ? of_key((uint32_t)(thr >> IDX_BITS)) : -INFINITY;
+  const int tie_idx = (int)(MAX_VOCAB - 1 - (thr & (MAX_VOCAB - 1)));
+  auto kept = [&](float y, int i) -> u64 {
+    const u64 w = f.weight(y);
+    return y >= from && !(y == tie && i > tie_idx) ? w : 0;
   };
-  u64 sum = 0;
-  for (int v = v0 + lane; v < v1; v += 32) {
-    const uint4 q = xv[v];
+  u64 sum_kept = 0;
+  auto add_kept = [&](const float (&y)[VEC], int first) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum += kept(get(q, j), i0 + v * VEC + j);
-  }
+    for (int i = 0; i < VEC; ++i) sum_kept += kept(y[i], first + i);
+  };
+  if (thr || key_pmin) x.template vectors<true>(from, add_kept);
+  else x.template vectors<false>(from, add_kept);
 #pragma unroll
-  for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-  __syncthreads();
-  if (lane == 0) s.red[warp] = sum;
-  __syncthreads();
-  u64 mine = 0, before = 0;
-  for (int w = 0; w < NW; ++w) {
-    if (w == warp) before = mine;
-    mine += s.red[w];
-  }
-  if (tid < C) cluster.map_shared_rank(s.sums, tid)[rank] = mine;
+  for (int w = 16; w; w >>= 1) sum_kept += __shfl_xor_sync(0xffffffffu, sum_kept, w);
+  if (lane < C) cluster.map_shared_rank(&s.warp_sums[0][0], lane)[rank * NW + warp] = sum_kept;
   cluster.sync();
-  u64 total = 0;
-  for (int c = 0; c < C; ++c) {
-    if (c == rank) before += total;
-    total += s.sums[c];
-  }
-  const float u = a.u[r];
-  u64 at = (u64)((double)(u > 0.f ? u : 0.f) * (double)total);
-  at = at < total ? at : total - 1;
-  if (before <= at && at < before + sum) {
-    for (int v = v0; v < v1; v += 32) {
-      const uint4 q = v + lane < v1 ? xv[v + lane] : make_uint4(0, 0, 0, 0);
-      u64 own = 0;
-      if (v + lane < v1) {
+
+  // the warp in which the running sum passes the place
+  static_assert(C * NW == 64, "two sums a lane");
+  u64 total, before, mine = (&s.warp_sums[0][0])[rank * NW + warp];
+  {
+    const u64 s0 = (&s.warp_sums[0][0])[2 * lane], s1 = (&s.warp_sums[0][0])[2 * lane + 1];
+    u64 up = s0 + s1;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) own += kept(get(q, j), i0 + (v + lane) * VEC + j);
+    for (int w = 1; w < 32; w <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, up, w);
+      if (lane >= w) up += y;
+    }
+    total = __shfl_sync(0xffffffffu, up, 31);
+    const int me = rank * NW + warp;
+    before = __shfl_sync(0xffffffffu, up - (me & 1 ? s1 : s0 + s1), me / 2);
+  }
+  const u64 at = place(a.u[r], total);
+  if (before <= at && at < before + mine) {
+    for (int v = x.v0; v < x.v1; v += 32) {
+      const bool in = v + lane < x.v1;
+      const uint4 q = in ? x.xv[v + lane] : make_uint4(0, 0, 0, 0);
+      const int first = i0 + (v + lane) * VEC;
+      u64 own = 0;
+      if (in) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) own += kept(X::get(q, j), first + j);
       }
-      u64 x = own;
+      u64 sum = own;
 #pragma unroll
       for (int w = 1; w < 32; w <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, x, w);
-        if (lane >= w) x += y;
+        const u64 y = __shfl_up_sync(0xffffffffu, sum, w);
+        if (lane >= w) sum += y;
       }
-      const uint32_t over = __ballot_sync(0xffffffffu, before + x > at);
+      const uint32_t over = __ballot_sync(0xffffffffu, before + sum > at);
       if (over) {
         if (lane == __ffs(over) - 1) {
-          u64 c = before + x - own;
+          u64 c = before + sum - own;
           int j = 0;
           for (; j < VEC - 1; ++j) {
-            c += kept(get(q, j), i0 + (v + lane) * VEC + j);
+            c += kept(X::get(q, j), first + j);
             if (c > at) break;
           }
-          a.tokens[r] = i0 + (v + lane) * VEC + j;
+          a.tokens[r] = first + j;
         }
         break;
       }
-      before += __shfl_sync(0xffffffffu, x, 31);
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
   }
 }
