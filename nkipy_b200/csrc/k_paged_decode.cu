@@ -50,12 +50,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
   using S = Shape<DP>;
   constexpr int WN = S::WN, NT = WN / 8, CH = DP / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t *sQ = smem, *body = smem + ROWS * DP * 2;
+  uint8_t *sQ = smem;
   const Args &a = p.a;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x;
   const int heads = (int)a.kv_heads * p.groups;  // units per sequence
   const int G = (int)(a.q_heads / a.kv_heads), D = (int)a.head_dim;
-  uint8_t *ring = body + warp * S::RING;
+  uint8_t *ring = smem + S::STAGES * S::QBUF + warp * S::RING;
+  float2 *s_ml = reinterpret_cast<float2 *>(smem + S::STAGES * S::QBUF + WARPS * S::RING);  // (max, sum) of the warps' rows
 
   const Found at = find<S::BK>(a, [&](int64_t blocks, int, int64_t first, int64_t n) {
     const int ctas = workers(blocks * heads, p.ctas);
@@ -69,184 +70,233 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
     pdl_wait();
     return;
   }
-  const int64_t f0 = share(total, c, ctas), f1 = share(total, c + 1, ctas);
-  int64_t f = f0, before = at.before * heads;  // `before`: blocks before sequence b
-  int b = at.seq;
-  while (f < f1) {
-    const Visible vis = visible_of(a, b);
-    const int nb = max(1, (vis.n + S::BK - 1) / S::BK);
-    const int unit = (int)((f - before) / nb), k0 = (int)((f - before) % nb);
-    const int k1 = (int)min((int64_t)nb, k0 + (f1 - f));
-    const int hk = unit / p.groups, h0 = hk * G + (unit % p.groups) * ROWS, rows = min(ROWS, (hk + 1) * G - h0);
-    const T *kc = static_cast<const T *>(a.k_cache) + hk * a.k_cache_head;
-    const T *vc = static_cast<const T *>(a.v_cache) + hk * a.v_cache_head;
-    const int32_t *table = a.page_table + b * a.table_stride;
+  const int64_t f0 = share(total, c, ctas);
+  const int n_blocks = (int)(share(total, c + 1, ctas) - f0);
 
-    __syncthreads();  // the join buffer and Q of the segment before are read
-    for (int i = threadIdx.x; i < ROWS * CH; i += THREADS) {
-      const int r = i / CH, ch = i % CH;
-      const bool ok = r < rows && ch * 8 < D;
-      cp_async16(smem_addr(sQ) + mma::swz(r, ch, DP * 2),
-                 static_cast<const T *>(a.q) + b * a.q_token + (ok ? (h0 + r) * a.q_head + ch * 8 : 0), ok);
+  // a place in the share: block k of nb of a (sequence, 16-row group of heads)
+  struct At {
+    int b, unit, k, nb;
+    Visible vis;
+  };
+  auto sequence = [&](At &x, int b) {
+    x.b = b;
+    x.vis = visible_of(a, b);
+    x.nb = max(1, (x.vis.n + S::BK - 1) / S::BK);
+  };
+  auto step = [&](At &x) {
+    if (++x.k < x.nb) return;
+    x.k = 0;
+    if (++x.unit < heads) return;
+    x.unit = 0;
+    if (x.b + 1 < (int)a.seqs) sequence(x, x.b + 1);
+  };
+  At ahead;  // of the next block to locate
+  sequence(ahead, at.seq);
+  {
+    const int in = (int)(f0 - at.before * heads);
+    ahead.unit = in / ahead.nb;
+    ahead.k = in - ahead.unit * ahead.nb;
+  }
+  At now = ahead;  // of the block at work
+
+  // where this lane's key of a located block and its value begin (null: no such
+  // key or page), and the block's unit
+  const char *k_row, *v_row;
+  int unit_b, unit, located = 0;
+  bool starts;  // the block is the first of its segment: Q goes with it
+  auto locate = [&]() {
+    k_row = v_row = nullptr;
+    starts = ahead.k == 0 || located == 0;
+    unit_b = ahead.b;
+    unit = ahead.unit;
+    if (located++ >= n_blocks) return;
+    const int v = ahead.k * S::BK + warp * WN + lane;
+    if (lane < WN && v < ahead.vis.n) {
+      const int key = ahead.vis.key(v), i = key / (int)a.page_size, slot = key - i * (int)a.page_size;
+      const int page = a.page_table[ahead.b * a.table_stride + i];
+      if (paged::page_ok(page, a.pages)) {
+        const int hk = p.groups == 1 ? unit : unit / p.groups;
+        k_row = reinterpret_cast<const char *>(static_cast<const T *>(a.k_cache) + page * a.k_page + slot * a.k_slot +
+                                               hk * a.k_cache_head);
+        v_row = reinterpret_cast<const char *>(static_cast<const T *>(a.v_cache) + page * a.v_page + slot * a.v_slot +
+                                               hk * a.v_cache_head);
+      }
     }
+    step(ahead);
+  };
+  int q_next = 0, q_at = 0;  // Q buffers: the next to fill, the one in use
+  // the located block into `stage`; rows without a page are zeros
+  auto load = [&](int stage) {
+    const uint32_t kd = smem_addr(ring + stage * 2 * S::TILE), vd = kd + S::TILE;
+#pragma unroll
+    for (int j = 0; j < WN * CH / 32; ++j) {
+      const int idx = j * 32 + lane, r = idx / CH, ch = idx % CH;
+      const uint64_t k = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(k_row), r);
+      const uint64_t v = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(v_row), r);
+      const bool ok = k && ch * 8 < D;
+      cp_async16(kd + mma::swz(r, ch, DP * 2), ok ? reinterpret_cast<const char *>(k) + ch * 16 : a.k_cache, ok);
+      cp_async16(vd + mma::swz(r, ch, DP * 2), ok ? reinterpret_cast<const char *>(v) + ch * 16 : a.v_cache, ok);
+    }
+    if (starts) {  // each warp copies a quarter of the rows of Q
+      const int hk = unit / p.groups, g0 = (unit - hk * p.groups) * ROWS, rows = min(ROWS, G - g0);
+      const T *q = static_cast<const T *>(a.q) + unit_b * a.q_token + (hk * G + g0) * a.q_head;
+      const uint32_t qd = smem_addr(sQ + q_next * S::QBUF);
+#pragma unroll
+      for (int j = 0; j < (ROWS / WARPS * CH + 31) / 32; ++j) {
+        const int idx = j * 32 + lane, r = warp * (ROWS / WARPS) + idx / CH, ch = idx % CH;
+        const bool ok = r < rows && ch * 8 < D;
+        cp_async16(qd + mma::swz(r, ch, DP * 2), q + (ok ? r * a.q_head + ch * 8 : 0), ok);
+      }
+      q_next = q_next + 1 == S::STAGES ? 0 : q_next + 1;
+    }
+  };
+  locate();
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; ++s) {
+    if (s < n_blocks) load(s);
+    locate();
     cp_commit();
+  }
 
-    // page id (-1: none) and slot of this lane's key of block kb
-    auto locate = [&](int kb, int &page, int &slot) {
-      const int v = kb * S::BK + warp * WN + lane;
-      page = -1;
-      slot = 0;
-      if (lane < WN && kb < k1 && v < vis.n) {
-        const int key = vis.key(v), i = key / (int)a.page_size;
-        slot = key - i * (int)a.page_size;
-        page = table[i];
-        if (!paged::page_ok(page, a.pages)) page = -1;
-      }
-    };
-    auto load = [&](int stage, int page, int slot) {  // rows without a page are zeros
-      const uint32_t kd = smem_addr(ring + stage * 2 * S::TILE), vd = kd + S::TILE;
-#pragma unroll
-      for (int j = 0; j < WN * CH / 32; ++j) {
-        const int idx = j * 32 + lane, r = idx / CH, ch = idx % CH;
-        const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
-        const bool ok = pg >= 0 && ch * 8 < D;
-        const int64_t ko = ok ? pg * a.k_page + sl * a.k_slot + ch * 8 : 0;
-        const int64_t vo = ok ? pg * a.v_page + sl * a.v_slot + ch * 8 : 0;
-        cp_async16(kd + mma::swz(r, ch, DP * 2), kc + ko, ok);
-        cp_async16(vd + mma::swz(r, ch, DP * 2), vc + vo, ok);
-      }
-    };
-    int page, slot;
-    locate(k0, page, slot);
-#pragma unroll
-    for (int s = 0; s < S::STAGES - 1; ++s) {
-      const int pg = page, sl = slot;
-      locate(k0 + s + 1, page, slot);
-      if (k0 + s < k1) load(s, pg, sl);
+  uint32_t qf[DP / 16][4];
+  float o[CH][4], m[2], l[2];  // rows lane / 4 and lane / 4 + 8, log2 units
+  int stage = 0, k0 = 0;  // k0: the segment's first block in its unit
+  bool first = true;      // the next block starts one
+#pragma unroll 1
+  for (int i = 0; i < n_blocks; ++i) {
+    __syncwarp();  // every lane has read the stage that is filled next
+    {
+      int fill = stage + S::STAGES - 1;
+      fill = fill >= S::STAGES ? fill - S::STAGES : fill;
+      if (i + S::STAGES - 1 < n_blocks) load(fill);
+      locate();
       cp_commit();
     }
     cp_wait<S::STAGES - 1>();
-    __syncthreads();
-    uint32_t qf[DP / 16][4];
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
-      ldsm_x4(smem_addr(sQ) + mma::swz(lane % 16, kk * 2 + lane / 16, DP * 2), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
-
-    float o[CH][4];
-#pragma unroll
-    for (int j = 0; j < CH; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows lane / 4 and lane / 4 + 8, log2 units
-    int stage = 0;
-#pragma unroll 1
-    for (int kb = k0; kb < k1; ++kb) {
-      __syncwarp();  // every lane has read the stage that is filled next
-      {
-        const int pg = page, sl = slot, next = kb + S::STAGES - 1;
-        locate(next + 1, page, slot);
-        int fill = stage + S::STAGES - 1;
-        fill = fill >= S::STAGES ? fill - S::STAGES : fill;
-        if (next < k1) load(fill, pg, sl);
-        cp_commit();
-      }
-      cp_wait<S::STAGES - 1>();
-      __syncwarp();  // this block's rows, copied by every lane, are visible
-      const uint32_t kt = smem_addr(ring + stage * 2 * S::TILE), vt = kt + S::TILE;
-      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-      float s[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    __syncwarp();  // this block's rows, copied by every lane, are visible
+    uint8_t *tile = ring + stage * 2 * S::TILE;
+    const uint32_t kt = smem_addr(tile), vt = kt + S::TILE;
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+    if (first) {
+      __syncthreads();  // every warp's rows of Q
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk)
+        ldsm_x4(smem_addr(sQ + q_at * S::QBUF) + mma::swz(lane % 16, kk * 2 + lane / 16, DP * 2), qf[kk][0], qf[kk][1],
+                qf[kk][2], qf[kk][3]);
+      q_at = q_at + 1 == S::STAGES ? 0 : q_at + 1;
 #pragma unroll
-        for (int j = 0; j < NT; j += 2) {
-          uint32_t b0, b1, b2, b3;
-          const int r = j * 8 + (lane % 8) + (lane / 16) * 8;
-          ldsm_x4(kt + mma::swz(r, kk * 2 + (lane / 8) % 2, DP * 2), b0, b1, b2, b3);
-          mma_tile<T>(s[j], qf[kk], b0, b1);
-          mma_tile<T>(s[j + 1], qf[kk], b2, b3);
-        }
-      const int v0 = kb * S::BK + warp * WN;
-      float mx[2] = {m[0], m[1]};
+      for (int j = 0; j < CH; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+      k0 = now.k;
+      first = false;
+    }
+    float s[NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = v0 + j * 8 + (lane % 4) * 2 + (e & 1);
-          s[j][e] = v < vis.n ? s[j][e] * p.scale_log2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-        }
-      float alpha[2], sum[2] = {0.f, 0.f}, base[2];
+    for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        base[i] = mx[i] == -INFINITY ? 0.f : mx[i];  // a warp whose keys are all masked so far
-        alpha[i] = ex2(m[i] - base[i]);
-        m[i] = mx[i];
+      for (int j = 0; j < NT; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        const int r = j * 8 + (lane % 8) + (lane / 16) * 8;
+        ldsm_x4(kt + mma::swz(r, kk * 2 + (lane / 8) % 2, DP * 2), b0, b1, b2, b3);
+        mma_tile<T>(s[j], qf[kk], b0, b1);
+        mma_tile<T>(s[j + 1], qf[kk], b2, b3);
       }
+    const int v0 = now.k * S::BK + warp * WN;
+    float mx[2] = {m[0], m[1]};
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[j][e] = ex2(s[j][e] - base[e >> 1]);
-          sum[e >> 1] += s[j][e];
-        }
-      l[0] = l[0] * alpha[0] + sum[0];
-      l[1] = l[1] * alpha[1] + sum[1];
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        o[j][0] *= alpha[0];
-        o[j][1] *= alpha[0];
-        o[j][2] *= alpha[1];
-        o[j][3] *= alpha[1];
+      for (int e = 0; e < 4; ++e) {
+        const int v = v0 + j * 8 + (lane % 4) * 2 + (e & 1);
+        s[j][e] = v < now.vis.n ? s[j][e] * p.scale_log2 : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
       }
+    float alpha[2], sum[2] = {0.f, 0.f}, base[2];
 #pragma unroll
-      for (int kk = 0; kk < NT / 2; ++kk) {
-        // probabilities rounded to the cache's type, as the product's operand
-        const uint32_t pf[4] = {pack<T>(s[2 * kk][0], s[2 * kk][1]), pack<T>(s[2 * kk][2], s[2 * kk][3]),
-                                pack<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      base[i] = mx[i] == -INFINITY ? 0.f : mx[i];  // a warp whose keys are all masked so far
+      alpha[i] = ex2(m[i] - base[i]);
+      m[i] = mx[i];
+    }
 #pragma unroll
-        for (int j = 0; j < CH; j += 2) {
-          uint32_t b0, b1, b2, b3;
-          const int r = kk * 16 + (lane % 8) + ((lane / 8) % 2) * 8;
-          ldsm_x4_t(vt + mma::swz(r, j + lane / 16, DP * 2), b0, b1, b2, b3);
-          mma_tile<T>(o[j], pf, b0, b1);
-          mma_tile<T>(o[j + 1], pf, b2, b3);
-        }
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = ex2(s[j][e] - base[e >> 1]);
+        sum[e >> 1] += s[j][e];
+      }
+    l[0] = l[0] * alpha[0] + sum[0];
+    l[1] = l[1] * alpha[1] + sum[1];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      o[j][0] *= alpha[0];
+      o[j][1] *= alpha[0];
+      o[j][2] *= alpha[1];
+      o[j][3] *= alpha[1];
+    }
+#pragma unroll
+    for (int kk = 0; kk < NT / 2; ++kk) {
+      // probabilities rounded to the cache's type, as the product's operand
+      const uint32_t pf[4] = {pack<T>(s[2 * kk][0], s[2 * kk][1]), pack<T>(s[2 * kk][2], s[2 * kk][3]),
+                              pack<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+      for (int j = 0; j < CH; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        const int r = kk * 16 + (lane % 8) + ((lane / 8) % 2) * 8;
+        ldsm_x4_t(vt + mma::swz(r, j + lane / 16, DP * 2), b0, b1, b2, b3);
+        mma_tile<T>(o[j], pf, b0, b1);
+        mma_tile<T>(o[j + 1], pf, b2, b3);
       }
     }
-    // join the four warps
-    cp_wait<0>();
-    __syncthreads();
-    float *s_o = reinterpret_cast<float *>(body), *s_m = s_o + WARPS * ROWS * S::OPAD, *s_l = s_m + WARPS * ROWS;
+    if (now.k + 1 < now.nb && i + 1 < n_blocks) {
+      ++now.k;
+      continue;
+    }
+
+    // the segment's end: join the four warps, in the stage that each has just read
+    // (the others are being filled)
+    const int hk = now.unit / p.groups, g0 = (now.unit - hk * p.groups) * ROWS, rows = min(ROWS, G - g0);
+    auto at_o = [](int r, int d) { return r * DP + (d ^ ((r & 3) * 8)); };
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      const int r = warp * ROWS + lane / 4 + i * 8;
-      if (lane % 4 == 0) {
-        s_m[r] = m[i];
-        s_l[r] = l[i];
-      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = lane / 4 + i * 8;
+      if (r >= rows) continue;
+      if (lane % 4 == 0) s_ml[warp * ROWS + r] = make_float2(m[i], l[i]);
 #pragma unroll
       for (int j = 0; j < CH; ++j)
-        *reinterpret_cast<float2 *>(s_o + r * S::OPAD + j * 8 + (lane % 4) * 2) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(tile) + at_o(r, j * 8 + (lane % 4) * 2)) =
+            make_float2(o[j][2 * i], o[j][2 * i + 1]);
     }
     __syncthreads();
-    const bool all = k0 == 0 && k1 == nb, whole = all && !p.keep;
-    const int64_t at_slot = all ? 2 * p.ctas + (int64_t)b * heads + unit : 2 * c + (f != f0);
+    const bool all = k0 == 0 && now.k + 1 == now.nb, whole = all && !p.keep;
+    const int64_t at_slot = all ? 2 * p.ctas + (int64_t)now.b * heads + now.unit : 2 * c + (i + 1 > now.k + 1 - k0);
     float *slot_ws = p.ws + at_slot * S::SLOT;
     for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+      float2 ml[WARPS];
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * ROWS + r]);
+      for (int w = 0; w < WARPS; ++w) {
+        ml[w] = s_ml[w * ROWS + r];
+        M = fmaxf(M, ml[w].x);
+      }
       float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float mw = s_m[w * ROWS + r], g = mw == -INFINITY ? 0.f : ex2(mw - M);
-        const float4 y = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + r) * S::OPAD + d);
-        L += s_l[w * ROWS + r] * g;
+        const float g = ml[w].x == -INFINITY ? 0.f : ex2(ml[w].x - M);
+        const uint8_t *part = tile + (w - warp) * S::RING;
+        const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(part) + at_o(r, d));
+        L += ml[w].y * g;
         x[0] += y.x * g;
         x[1] += y.y * g;
         x[2] += y.z * g;
@@ -255,18 +305,16 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
       if (whole) {
         const float inv = L > 0.f ? 1.f / L : 0.f;
         if (d < D)
-          *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + b * a.out_token + (h0 + r) * a.out_head + d) =
+          *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + now.b * a.out_token + (hk * G + g0 + r) * a.out_head + d) =
               make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
       } else {
         *reinterpret_cast<float4 *>(slot_ws + r * DP + d) = make_float4(x[0], x[1], x[2], x[3]);
         if (d == 0) *reinterpret_cast<float2 *>(slot_ws + ROWS * DP + 2 * r) = make_float2(M, L);
       }
     }
-    f += k1 - k0;
-    if (f - before == (int64_t)nb * heads) {
-      before = f;
-      ++b;
-    }
+    __syncthreads();  // the stages may be filled again
+    step(now);
+    first = true;
   }
   pdl_wait();  // launched early, this grid must not end before the one it follows
 }

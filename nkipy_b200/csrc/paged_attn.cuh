@@ -147,10 +147,9 @@ struct Shape {
   static constexpr int TILE = WN * DP * 2;             // bytes of K (or V) per stage
   static constexpr int STAGES = 3;
   static constexpr int RING = STAGES * 2 * TILE;       // per warp
-  static constexpr int OPAD = DP + 4;                  // row stride of the join buffer (floats)
-  static constexpr int JOIN = WARPS * ROWS * (OPAD + 2) * 4;
-  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
-  static constexpr int SMEM = ROWS * DP * 2 + BODY;
+  static constexpr int QBUF = ROWS * DP * 2;           // Q of one segment: there are as many as stages
+  static constexpr int SMEM = STAGES * QBUF + WARPS * RING + WARPS * ROWS * 8;
+  static_assert(ROWS * DP * 4 <= 2 * TILE, "a warp's outputs fit a stage");
   static constexpr int SLOT = ROWS * (DP + 2);         // floats of one partial: outputs, then max and sum
 };
 
@@ -187,37 +186,43 @@ __device__ __forceinline__ Found find(const Args &a, Want want) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, B = (int)a.seqs;
   Found r;
   r.total = 0;
-  for (int base = 0; base < B; base += THREADS) {  // the sum
-    const int b = base + threadIdx.x;
-    int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
-#pragma unroll
-    for (int w = 16; w; w >>= 1) n += __shfl_xor_sync(0xffffffffu, n, w);
-    __syncthreads();
-    if (lane == 0) s_warp[warp] = n;
-    __syncthreads();
-    r.total += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
-  }
-  int64_t done = 0;
-  for (int base = 0; base < B; base += THREADS) {  // the sequence
-    const int b = base + threadIdx.x;
-    const int64_t n = b < B ? blocks_of<BK>(a, b) : 0;
+  int64_t n = 0, first = 0;  // blocks of this thread's sequence, and before it
+  auto chunk = [&](int base) {
+    const int b = base + (int)threadIdx.x;
+    n = b < B ? blocks_of<BK>(a, b) : 0;
     int64_t p = n;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) {
       const int64_t x = __shfl_up_sync(0xffffffffu, p, w);
       if (lane >= w) p += x;
     }
-    __syncthreads();
+    if (base) __syncthreads();  // the sums of the chunk before are read
     if (lane == 31) s_warp[warp] = p;
     __syncthreads();
-    int64_t first = done + p - n;
+    first = r.total + p - n;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) first += s_warp[w];
-      done += s_warp[w];
+      r.total += s_warp[w];
     }
+    return b;
+  };
+  int b = 0;
+  for (int base = 0; base < B; base += THREADS) b = chunk(base);
+  if (B <= THREADS) {
     if (b < B && want(r.total, b, first, n)) {
       s_seq = b;
       s_before = first;
+    }
+  } else {  // the sum was for the total: once more
+    const int64_t total = r.total;
+    r.total = 0;
+    __syncthreads();
+    for (int base = 0; base < B; base += THREADS) {
+      b = chunk(base);
+      if (b < B && want(total, b, first, n)) {
+        s_seq = b;
+        s_before = first;
+      }
     }
   }
   __syncthreads();
