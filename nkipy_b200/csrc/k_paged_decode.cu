@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_const
   for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
     if (d >= D) continue;
-    Joined x;
+    Joined<8> x;
     x.add(parts.n, [&](int j) {
       const float *slot = p.ws + (int64_t)parts.slot(j) * S::SLOT;
       return Partial{slot + r * DP + d, slot + ROWS * DP + 2 * r};

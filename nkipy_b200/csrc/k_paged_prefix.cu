@@ -23,11 +23,11 @@ __global__ void __launch_bounds__(THREADS)
   const Args &a = p.a;
   const int t = blockIdx.x, hk = blockIdx.y, G = p.G, D = (int)a.head_dim, per = 2 * p.P;
   single::Found at = {0, 0, 0};
-  if (!p.own) at = single::find<S::BK>(a, [&](int64_t, int b, int64_t, int64_t) { return b == t; });
-  pdl_wait();
+  if (p.own) pdl_wait();  // the pairs are a list of the kernels before
+  else at = single::find<S::BK>(a, [&](int64_t, int b, int64_t, int64_t) { return b == t; });
   const several::Walk walk(p, 0);
   auto unit_parts = [&](int u, int &tok, int &seq) {  // of pair u
-    const several::Pair x = p.pairs[u];
+    const several::Pair x = several::pair_of(p, u);
     const int64_t n = several::blocks_of(p, x).n;
     tok = t - x.tok0;
     seq = x.seq;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(THREADS)
   Parts own;
   seq = 0;
   if (p.own) {  // the pair of this token among the sequences' own
-    int lo = (int)((a.tokens + per - 1) / per), hi = (int)p.head[0] - 1;
+    int lo = (int)((a.tokens + per - 1) / per), hi = walk.pairs - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if (p.pairs[mid].tok0 <= t) lo = mid;
@@ -47,19 +47,24 @@ __global__ void __launch_bounds__(THREADS)
     own = unit_parts(lo, otok, seq);
   }
   const int heads = (int)a.kv_heads * s.groups;
+  auto own_parts = [&](int g) {
+    const int unit = hk * s.groups + g / single::ROWS, nb = single::blocks_of<S::BK>(a, t);
+    return parts_of(at.total * heads, at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
+  };
+  if (!p.own) {
+    own = own_parts(min((int)threadIdx.x / (DP / 4), G - 1));
+    pdl_wait();
+  }
   for (int i = threadIdx.x; i < G * (DP / 4); i += THREADS) {
     const int g = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (!p.own) {
-      const int unit = hk * s.groups + g / single::ROWS, nb = single::blocks_of<S::BK>(a, t);
-      own = parts_of(at.total * heads, at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
-    }
+    if (!p.own && i >= THREADS) own = own_parts(g);
     auto tile_part = [&](const Parts &x, int j, int tok) {
       const float *slot = p.ws + (int64_t)x.slot(j) * SLOT;
       const int row = tok / p.P * several::BM + tok % p.P * G + g;
       return Partial{slot + row * DP + d, slot + ML + 2 * row};
     };
     if (d >= D) continue;
-    Joined x;
+    Joined<8> x;
     if (seq != -2) {  // (a token of no sequence sees nothing)
       x.add(pre.n, [&](int j) { return tile_part(pre, j, ptok); });
       if (p.own) x.add(own.n, [&](int j) { return tile_part(own, j, otok); });

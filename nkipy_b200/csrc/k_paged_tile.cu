@@ -97,7 +97,7 @@ __device__ __forceinline__ void tokens_of(const Args &a, int i, int &first, int 
 __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Params p) {
   const Args &a = p.a;
   const int per = 2 * p.P, B = (int)a.seqs, T = (int)a.tokens;
-  const int lists = p.own ? B + 2 : 0, front = p.prefix ? (T + per - 1) / per : 0;
+  const int lists = B + 2, front = p.prefix ? (T + per - 1) / per : 0;
   pdl_trigger();
   int64_t npairs = front;
   for (int base = 0; base < lists; base += SCHED) {
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(JOIN) tile_join_kernel(const __grid_constant__
       const int row = item % PARTS * 32 + i / (DP / 4), d = i % (DP / 4) * 4, t = row / BM, r = row % BM;
       const int g = r % p.G, tok = t * p.P + r / p.G;
       if (r >= p.P * p.G || tok >= s.x.ntok || d >= (int)a.head_dim) continue;
-      Joined x;
+      Joined<4> x;
       x.add(parts.n, [&](int j) {
         const float *slot = p.ws + (int64_t)parts.slot(j) * C::SLOT;
         return Partial{slot + row * DP + d, slot + 2 * BM * DP + 2 * row};
@@ -767,12 +767,14 @@ int launch(const Params &p, cudaStream_t st, int device) {
   if (int s = make_bf16_map(&mq, a.q, 4, dims, strides, box)) return s;
   if (int s = cache_map(&mk, a.k_cache, a, a.k_page, a.k_slot, a.k_cache_head)) return s;
   if (int s = cache_map(&mv, a.v_cache, a, a.v_page, a.v_slot, a.v_cache_head)) return s;
-  pairs_kernel<<<1, SCHED, 0, st>>>(p);
-  if (int s = launch_status("paged pairs")) return s;
-  NKB_CUDA_TRY(launch_pdl(true, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
+  if (p.own) {
+    pairs_kernel<<<1, SCHED, 0, st>>>(p);
+    if (int s = launch_status("paged pairs")) return s;
+  }
+  NKB_CUDA_TRY(launch_pdl(p.own, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
   if (int s = launch_status("paged_tile")) return s;
   if (p.keep || p.max_ctas < 2) return NKB_OK;
-  NKB_CUDA_TRY(launch_pdl(true, tile_join_kernel<T, DP>, dim3(4 * p.max_ctas), dim3(JOIN), 0, st, p));
+  NKB_CUDA_TRY(launch_pdl(true, tile_join_kernel<T, DP>, dim3((p.max_ctas - 1) * (2 * BM / 32)), dim3(JOIN), 0, st, p));
   return launch_status("paged_tile join");
 }
 

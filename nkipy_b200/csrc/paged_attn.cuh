@@ -80,18 +80,21 @@ __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t *>(&h);
 }
 
-// Four outputs of a row, joined from partials that are read eight at a time.
+// Four outputs of a row, joined from partials that are read U at a time.
+template <int U>
 struct Joined {
   float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
   template <class At>
   __device__ __forceinline__ void add(int n, At at) {
-    constexpr int U = 8;
     for (int j0 = 0; j0 < n; j0 += U) {
       float2 ml[U];
       float4 y[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const Partial q = at(min(j0 + j, n - 1));
+        ml[j] = make_float2(-INFINITY, 0.f);
+        y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j0 + j >= n) continue;
+        const Partial q = at(j0 + j);
         ml[j] = __ldcg(reinterpret_cast<const float2 *>(q.ml));
         y[j] = __ldcg(reinterpret_cast<const float4 *>(q.o));
       }
@@ -105,7 +108,7 @@ struct Joined {
       for (int i = 0; i < 4; ++i) x[i] *= f;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const float g = j0 + j < n ? ex2(ml[j].x - top) : 0.f;
+        const float g = ex2(ml[j].x - top);
         if (g == 0.f) continue;  // a part that saw nothing has nothing written for it to scale
         l += ml[j].y * g;
         x[0] += y[j].x * g;
@@ -294,6 +297,21 @@ __device__ __forceinline__ int tile_blocks(const Params &p, const Pair &x, const
   return end == 0 ? 0 : k.ns + max(0, (end + BN - 1) / BN - k.w0);
 }
 
+// The list of pairs.  With a prefix alone (own = 0) it follows from the sizes:
+// 2 P tokens each, all of the prefix's blocks; else k_paged_tile.cu writes it.
+__device__ __forceinline__ int pairs_of(const Params &p) {
+  const int per = 2 * p.P;
+  return p.own ? (int)p.head[0] : (int)((p.a.tokens + per - 1) / per);
+}
+__device__ __forceinline__ Pair pair_of(const Params &p, int u) {
+  const int per = 2 * p.P;
+  return p.own ? p.pairs[u] : Pair{-1, u * per, min(per, (int)p.a.tokens - u * per), 0};
+}
+// blocks (per key head) before pair u
+__device__ __forceinline__ int64_t blocks_before(const Params &p, int u) {
+  return p.own ? p.head[1 + u] : u * max((int64_t)1, (p.a.prefix_len + BN - 1) / BN);
+}
+
 // ---- segments: what a CTA's share holds of each unit -----------------------------
 struct Segment {
   Pair x;
@@ -310,11 +328,11 @@ constexpr int WHOLE = 4;  // units per CTA from which they stay whole
 struct Walk {
   const Params &p;
   int64_t total, f, f0, f1;
-  int ctas, c, units;
+  int ctas, c, pairs, units;
   bool whole;
   __device__ __forceinline__ Walk(const Params &q, int cta) : p(q), c(cta) {
-    const int pairs = (int)p.head[0];
-    total = p.head[1 + pairs] * p.a.kv_heads;
+    pairs = pairs_of(p);
+    total = blocks_before(p, pairs) * p.a.kv_heads;
     units = pairs * (int)p.a.kv_heads;
     whole = units >= WHOLE * p.max_ctas;
     ctas = workers(total, p.max_ctas);
@@ -325,34 +343,35 @@ struct Walk {
   __device__ __forceinline__ Parts parts(int u, int hk, int64_t n) const {
     const int unit = u * (int)p.a.kv_heads + hk;
     if (whole) return Parts{1, 0, 2 * p.max_ctas + unit};
-    return parts_of(total, p.head[1 + u] * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
+    return parts_of(total, blocks_before(p, u) * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
   }
   // unit that holds block `at`: a whole warp looks, 32 pivots at a time
   __device__ __forceinline__ void locate(int64_t at, Segment &s, int lane) const {
     const int64_t row = at / p.a.kv_heads;  // pairs are kv_heads * n blocks long
-    int lo = 0, n = (int)p.head[0];
+    int lo = 0, n = pairs;
     while (n > 1) {
       const int step = (n + 31) / 32, i = lane * step;
-      const uint32_t m = __ballot_sync(0xffffffffu, i < n && p.head[1 + lo + min(i, n - 1)] <= row);
+      const uint32_t m = __ballot_sync(0xffffffffu, i < n && blocks_before(p, lo + min(i, n - 1)) <= row);
       const int last = 31 - __clz(m | 1u);
       lo += last * step;
       n = min(step, n - last * step);
     }
     set(lo, s);
-    const int in = (int)(at - p.head[1 + lo] * p.a.kv_heads);
+    const int in = (int)(at - blocks_before(p, lo) * p.a.kv_heads);
     s.hk = in / s.k.n;
     s.k0 = in - s.hk * s.k.n;
   }
   __device__ __forceinline__ void set(int u, Segment &s) const {
     s.u = u;
-    s.x = p.pairs[u];
+    s.x = pair_of(p, u);
     s.k = blocks_of(p, s.x);
   }
   // the next segment of the share (a whole warp)
   __device__ __forceinline__ bool next(Segment &s, int lane) {
     if (whole) {
       int i = c;
-      if (f != f0 && lane == 0) i = atomicAdd(p.next, 1);
+      if (!p.own) i += (int)(f - f0) * p.max_ctas;  // all of a length
+      else if (f != f0 && lane == 0) i = atomicAdd(p.next, 1);
       i = __shfl_sync(0xffffffffu, i, 0);
       ++f;
       if (i >= units) return false;
