@@ -80,6 +80,18 @@ struct Row {
   __device__ __forceinline__ uint32_t weight(float x) const { return w(pow2(t(x))); }
 };
 
+// floor(p * total) for p in [0, 1), exactly: total times the significand, moved.
+__device__ __forceinline__ u64 part_of(float p, u64 total) {
+  const uint32_t b = __float_as_uint(p), e = b >> 23;
+  const u64 m = (b & 0x7fffffu) | 0x800000u, lo = total * m, hi = __umul64hi(total, m);
+  const uint32_t down = 150 - e;  // from 24; total * m < 2^77
+  return !(p > 0.f) || down >= 77 ? 0 : down >= 64 ? hi >> (down - 64) : (hi << (64 - down)) | (lo >> down);
+}
+// The weight that top-p asks for: one at least.
+__device__ __forceinline__ u64 share_of(float p, u64 total) { return max((u64)1, part_of(p, total)); }
+// The random place among `total`.
+__device__ __forceinline__ u64 place(float u, u64 total) { return u >= 1.f ? total - 1 : part_of(u, total); }
+
 // ---- rows in a cluster's shared memory -------------------------------------
 constexpr int NT = 256, NW = NT / 32, C = 8;
 constexpr int CAP = 2048;         // elements that a CTA lists
@@ -231,10 +243,26 @@ __device__ void sort_down(u64 *list, int n) {
     }
 }
 
-// The random place among `total`.
-__device__ __forceinline__ u64 place(float u, u64 total) {
-  const u64 at = (u64)((double)(u > 0.f ? u : 0.f) * (double)total);
-  return at < total ? at : total - 1;
+// Sorts the values of the block's first n threads, largest first (the others have 0).
+__device__ __noinline__ void sort_down_few(u64 *shared, u64 &v, int n) {
+  static_assert(FEW == NT, "one a thread");
+  const int i = threadIdx.x;
+#pragma unroll 1
+  for (int size = 2; size < 2 * n; size *= 2)
+#pragma unroll 1
+    for (int stride = size / 2; stride; stride /= 2) {
+      u64 other;
+      if (stride < 32) {
+        other = __shfl_xor_sync(0xffffffffu, v, stride);
+      } else {
+        __syncthreads();
+        shared[i] = v;
+        __syncthreads();
+        other = shared[i ^ stride];
+      }
+      const bool first = (i & stride) == 0, down = (i & size) == 0;
+      v = (first == down) == (other > v) ? other : v;
+    }
 }
 
 // The rest of a row whose n candidates (rank words in s.list) hold its k largest
@@ -263,8 +291,7 @@ __device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, i
   if (tid < 128) {
     for (int i = 0; i < warp; ++i) sum += s.red[i];
     const u64 W = s.red[0] + s.red[1] + s.red[2] + s.red[3];
-    const double want = (double)p * (double)W;
-    const u64 T = p < 1.f ? (want >= 1.0 ? (u64)want : 1) : ~0ull;
+    const u64 T = p < 1.f ? share_of(p, W) : ~0ull;
     const bool keep = tid < m && sum - w < T && key >= key_pmin;
     s.weights[tid] = keep ? w : 0;
   }
@@ -536,8 +563,7 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
     for (int round = 0; round < 2; ++round) {
       const bool mass = round;
       if (!(mass ? by_mass : by_count)) continue;
-      const double want = (double)p * (double)W;
-      const u64 target = mass ? (want >= 1.0 ? (u64)want : 1) : (u64)k;
+      const u64 target = mass ? share_of(p, W) : (u64)k;
       if (fine >= 0) {  // top-k looked closer into a bin: the whole range again
         for (int i = tid; i < BINS; i += NT) s.hc[i] = s.hl[i] = s.hh[i] = 0;
         __syncthreads();
@@ -672,24 +698,17 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
           if (word < lo || word > hi) continue;
           const int at = atomicAdd(&s.n_few, 1);
           s.few[at] = word;
-          s.weights[at] = f.weight(of_key((uint32_t)(word >> IDX_BITS)));
         }
         __syncthreads();
-        // the element at which the running count or weight, largest first, reaches the target
-        if (tid < in) {
-          const u64 me = s.few[tid], w = s.weights[tid];
-          u64 c = 0, m = 0;
-#pragma unroll 8
-          for (int j = 0; j < in; ++j) {
-            const bool above = s.few[j] > me;
-            c += above;
-            m += above ? s.weights[j] : 0;
-          }
-          const u64 ex = before + (mass ? m : c), own = mass ? w : 1;
-          if (ex < target && target <= ex + own) {
-            s.out[0] = me;
-            s.out[1] = above_w + m + w;
-          }
+        // largest first, the element at which the running count or weight reaches the target
+        u64 me = tid < in ? s.few[tid] : 0;
+        sort_down_few(s.few, me, in);
+        const u64 w = me ? f.weight(of_key((uint32_t)(me >> IDX_BITS))) : 0;
+        u64 all;
+        const u64 m = scan(s, w, &all), ex = before + (mass ? m : (u64)tid), own = mass ? w : 1;
+        if (me && ex < target && target <= ex + own) {
+          s.out[0] = me;
+          s.out[1] = above_w + m + w;
         }
         __syncthreads();
         found = s.out[0];
@@ -900,8 +919,7 @@ __global__ void __launch_bounds__(THREADS) long_row_kernel(const __grid_constant
       return s + (ties < quota ? ties : quota) * wt;
     };
     const u64 W = mass(0);
-    const double want = (double)p * (double)W;
-    const u64 T = want >= 1.0 ? (u64)want : 1;
+    const u64 T = share_of(p, W);
     uint32_t t = 0;
     for (int bit = 31; bit >= 0; --bit)
       if (mass(t | (1u << bit)) >= T) t |= 1u << bit;
@@ -949,9 +967,7 @@ __global__ void __launch_bounds__(THREADS) long_row_kernel(const __grid_constant
   }
   auto upto = [&](u64 sum, u64 n) { return sum + (n < quota ? n : quota) * wt; };
   const u64 total = upto(S, N);
-  const double x = (double)(a.u[r] > 0.f ? a.u[r] : 0.f) * (double)total;
-  u64 at = (u64)x;
-  at = at < total ? at : total - 1;
+  const u64 at = place(a.u[r], total);
   if (upto(before, ties_before) <= at && at < upto(before + s, ties_before + ties)) {
     for (int base = i0; base < i1; base += 32) {
       const int i = base + lane;

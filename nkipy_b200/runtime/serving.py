@@ -28,6 +28,7 @@ try:
     import torch
 
     _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _FLOAT32, _INT32, _CONTIGUOUS = torch.float32, torch.int32, torch.contiguous_format
 except ImportError:  # pragma: no cover
     torch = None
 
@@ -50,51 +51,64 @@ def _on_device(*tensors):
     return device
 
 
-def _float(t, name, ndim):
-    """The type code of a float tensor with ``ndim`` axes, the last one contiguous."""
-    code = _CODES.get(t.dtype)
+def _rows(t, name, ndim):
+    """Type code, shape and strides of a float tensor with ``ndim`` axes, the last one contiguous."""
+    code, shape, strides = _CODES.get(t.dtype), t.shape, t.stride()
     if code is None:
         raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != ndim:
-        _fail(f"{name}: expected {ndim} axes, got shape {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    if len(strides) != ndim:
+        _fail(f"{name}: expected {ndim} axes, got shape {tuple(shape)}")
+    if strides[-1] != 1 and shape[-1] > 1:
         _fail(f"{name}: the last axis must be contiguous")
-    return code
+    return code, shape, strides
 
 
-def _int32(t, name, *shape):
+def _int32(t, name, length=None):
     """Checks a contiguous int32 vector of the given length (None: any length)."""
-    if t.dtype is not torch.int32:
+    if t.dtype is not _INT32:
         raise TypeError(f"{name}: expected int32, got {t.dtype}")
-    if t.dim() != 1 or (shape and t.shape[0] != shape[0]) or not t.is_contiguous():
-        _fail(f"{name}: expected a contiguous vector{f' of {shape[0]}' if shape else ''}, got shape {tuple(t.shape)}")
+    if t.dim() != 1 or (length is not None and t.numel() != length) or not t.is_contiguous():
+        of = "" if length is None else f" of {length}"
+        _fail(f"{name}: expected a contiguous vector{of}, got shape {tuple(t.shape)}")
 
 
 def _batch(page_table, kv_len, q_start, tokens):
     """Checks a call's page table and lengths; sequences, table width and row stride."""
-    if page_table.dtype is not torch.int32:
+    if page_table.dtype is not _INT32:
         raise TypeError(f"page_table: expected int32, got {page_table.dtype}")
     if page_table.dim() != 2:
         _fail(f"page_table: expected 2 axes, got shape {tuple(page_table.shape)}")
     seqs, width = page_table.shape
-    stride = page_table.stride()
-    if stride[1] != 1 and width > 1:
+    stride, last = page_table.stride()
+    if last != 1 and width > 1:
         _fail("page_table: the last axis must be contiguous")
     _int32(kv_len, "kv_len", seqs)
     if q_start is not None:
         _int32(q_start, "q_start", seqs + 1)
     elif tokens != seqs:
         _fail(f"without q_start there is one token per sequence: {tokens} tokens, {seqs} sequences")
-    return seqs, width, stride[0]
+    return seqs, width, stride
 
 
 def _caches(k_cache, v_cache):
-    code = _float(k_cache, "k_cache", 4)
-    if v_cache.dtype is not k_cache.dtype or v_cache.shape != k_cache.shape:
-        _fail(f"k_cache and v_cache differ: {tuple(k_cache.shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
-    if v_cache.stride(-1) != 1 and v_cache.shape[-1] > 1:
+    """Type code and shape of the caches, and both strides up to the last axis."""
+    code, shape, ks = _rows(k_cache, "k_cache", 4)
+    vs = v_cache.stride()
+    if v_cache.dtype is not k_cache.dtype or v_cache.shape != shape:
+        _fail(f"k_cache and v_cache differ: {tuple(shape)} {k_cache.dtype}, {tuple(v_cache.shape)} {v_cache.dtype}")
+    if vs[3] != 1 and shape[3] > 1:
         _fail("v_cache: the last axis must be contiguous")
-    return code
+    return code, shape, ks[:3] + vs[:3]
+
+
+def _like(t, code, shape, out, name):
+    """``out``, checked against ``t``, or a new tensor; and its first two strides."""
+    if out is None:
+        return torch.empty_like(t, memory_format=_CONTIGUOUS), (shape[1] * shape[2], shape[2])
+    other, other_shape, strides = _rows(out, name, 3)
+    if other != code or other_shape != shape:
+        _fail(f"{name} {tuple(other_shape)} {out.dtype} differs from q {tuple(shape)} {t.dtype}")
+    return out, strides[:2]
 
 
 def _ptr(t):
@@ -118,7 +132,7 @@ def attention_workspace(sizes, tokens_by_start) -> int:
 
 def _launch(fn, packed, device):
     """Issues a call on the current stream of ``device``."""
-    if torch.cuda.current_device() != device:
+    if torch._C._cuda_getDevice() != device:
         with torch.cuda.device(device):
             return _launch(fn, packed, device)
     status = fn(packed, torch._C._cuda_getCurrentRawStream(device))
@@ -136,13 +150,12 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=Non
     None without ``q``.  A row whose page is not in the cache, or whose position is
     outside the table, is not stored."""
     device = _on_device(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, sin, q_out)
-    code = _float(k, "k", 3)
-    tokens, hkv, d = k.shape
-    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
-    if v.shape != k.shape or v.dtype is not k.dtype or (vs[2] != 1 and d > 1):
-        _fail(f"k and v differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype} (strides {ks}, {vs})")
-    cache_code = _caches(k_cache, v_cache)
-    pages, page_size, heads, dim = k_cache.shape
+    code, shape, ks = _rows(k, "k", 3)
+    tokens, hkv, d = shape
+    vs = v.stride()
+    if v.shape != shape or v.dtype is not k.dtype or (vs[2] != 1 and d > 1):
+        _fail(f"k and v differ: {tuple(shape)} {k.dtype}, {tuple(v.shape)} {v.dtype} (strides {ks}, {vs})")
+    cache_code, (pages, page_size, heads, dim), cache_strides = _caches(k_cache, v_cache)
     if heads != hkv or dim != d:
         _fail(f"caches hold {heads} heads of {dim}, k has {hkv} of {d}")
     seqs, width, table_stride = _batch(page_table, kv_len, q_start, tokens)
@@ -150,52 +163,43 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=Non
     if (cos is None) != (sin is None):
         _fail("cos and sin go together")
     if cos is not None:
-        rope_code = _float(cos, "cos", 2)
-        if sin.shape != cos.shape or sin.dtype != cos.dtype or sin.stride() != cos.stride():
+        rope_code, (rows, rot), rope_strides = _rows(cos, "cos", 2)
+        if sin.shape != cos.shape or sin.dtype is not cos.dtype or sin.stride() != rope_strides:
             _fail("cos and sin differ in shape, type or strides")
-        rows, rot = cos.shape
-        rot, stride = 2 * rot, cos.stride(0)
+        rot, stride = 2 * rot, rope_strides[0]
         if rot > d:
             _fail(f"cos and sin rotate {rot} dimensions, head_dim is {d}")
-    hq = q_token = q_head = qo_token = qo_head = 0
+    hq, q_strides, out_strides = 0, (0, 0), (0, 0)
     if q is not None:
-        if _float(q, "q", 3) != code or q.shape[0] != tokens or q.shape[2] != d:
-            _fail(f"q {tuple(q.shape)} {q.dtype} does not go with k {tuple(k.shape)} {k.dtype}")
-        hq = q.shape[1]
-        q_token, q_head, _ = q.stride()
-        if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif _float(q_out, "q_out", 3) != code or q_out.shape != q.shape:
-            _fail(f"q_out {tuple(q_out.shape)} {q_out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
-        qo_token, qo_head, _ = q_out.stride()
+        q_code, q_shape, q_strides = _rows(q, "q", 3)
+        hq = q_shape[1]
+        if q_code != code or q_shape[0] != tokens or q_shape[2] != d:
+            _fail(f"q {tuple(q_shape)} {q.dtype} does not go with k {tuple(shape)} {k.dtype}")
+        q_out, out_strides = _like(q, code, q_shape, q_out, "q_out")
     elif q_out is not None:
         _fail("q_out without q")
     packed = _APPEND.pack(
         k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
         kv_len.data_ptr(), _ptr(q_start), _ptr(cos), _ptr(sin), code, cache_code, rope_code, tokens, seqs, hq, hkv, d, rot,
-        rows, stride, pos_offset, ks[0], ks[1], vs[0], vs[1], q_token, q_head, qo_token, qo_head, pages, page_size, kc[0],
-        kc[1], kc[2], vc[0], vc[1], vc[2], width, table_stride)
+        rows, stride, pos_offset, ks[0], ks[1], vs[0], vs[1], q_strides[0], q_strides[1], *out_strides, pages, page_size,
+        *cache_strides, width, table_stride)
     _launch(_nkb.lib().nkb_paged_append, packed, device)
     return q_out
 
 
 def _attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, out, prefix_pages, prefix_len):
     device = _on_device(q, k_cache, v_cache, page_table, kv_len, q_start, out, prefix_pages)
-    code = _float(q, "q", 3)
-    tokens, hq, d = q.shape
-    if _caches(k_cache, v_cache) != code:
+    code, shape, qs = _rows(q, "q", 3)
+    tokens, hq, d = shape
+    cache_code, (pages, page_size, hkv, dim), cache_strides = _caches(k_cache, v_cache)
+    if cache_code != code:
         raise TypeError(f"q is {q.dtype}, the caches are {k_cache.dtype}")
-    pages, page_size, hkv, dim = k_cache.shape
     if dim != d or hkv == 0 or hq % hkv:
-        _fail(f"q {tuple(q.shape)} does not go with caches of {hkv} heads of {dim}")
+        _fail(f"q {tuple(shape)} does not go with caches of {hkv} heads of {dim}")
     seqs, width, table_stride = _batch(page_table, kv_len, q_start, tokens)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif _float(out, "out", 3) != code or out.shape != q.shape:
-        _fail(f"out {tuple(out.shape)} {out.dtype} differs from q {tuple(q.shape)} {q.dtype}")
-    qs, os_, kc, vc = q.stride(), out.stride(), k_cache.stride(), v_cache.stride()
-    sizes = (code, tokens, seqs, hq, hkv, d, qs[0], qs[1], os_[0], os_[1], pages, page_size, kc[0], kc[1], kc[2], vc[0],
-             vc[1], vc[2], width, table_stride, window, sinks, prefix_len)
+    out, out_strides = _like(q, code, shape, out, "out")
+    sizes = (code, tokens, seqs, hq, hkv, d, qs[0], qs[1], *out_strides, pages, page_size, *cache_strides, width,
+             table_stride, window, sinks, prefix_len)
     need = _workspace(q_start is not None, *sizes)
     room = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(_nkb.lib().nkb_paged_attention, _ATTENTION.pack(
@@ -233,18 +237,17 @@ def sample_tokens(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     the order temperature, top-k, top-p, min-p; a temperature of 0 takes the largest
     logit.  A row without a finite logit or +inf gives -1."""
     device = _on_device(logits, u, temperature, top_k, top_p, min_p, out)
-    code = _float(logits, "logits", 2)
-    rows, vocab = logits.shape
+    code, (rows, vocab), strides = _rows(logits, "logits", 2)
     for t, name in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
-        if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != rows or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _FLOAT32 or t.dim() != 1 or t.numel() != rows or not t.is_contiguous()):
             _fail(f"{name}: expected a contiguous float32 tensor of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
     if top_k is not None:
         _int32(top_k, "top_k", rows)
     if out is None:
-        out = logits.new_empty(rows, dtype=torch.int32)
+        out = logits.new_empty(rows, dtype=_INT32)
     else:
         _int32(out, "out", rows)
     packed = _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-                          out.data_ptr(), code, rows, vocab, logits.stride(0))
+                          out.data_ptr(), code, rows, vocab, strides[0])
     _launch(_nkb.lib().nkb_sample_tokens, packed, device)
     return out
