@@ -96,7 +96,7 @@ __device__ __forceinline__ u64 place(float u, u64 total) { return u >= 1.f ? tot
 constexpr int NT = 256, NW = NT / 32, C = 8;
 constexpr int CAP = 2048;         // elements that a CTA lists
 constexpr int FEW = 256;          // elements that are ranked one against another
-constexpr int FAST_K = 100;       // top-k that one CTA sorts: some C * FAST_K candidates are expected, CAP fit
+constexpr int FAST_K = 128;       // top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit
 constexpr int MAX_SLICE = 65528;  // elements per CTA
 constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
 constexpr float SPAN = 31.1f;     // 2^-SPAN < 2^-31
@@ -115,7 +115,7 @@ struct Shared {
     u64 own[OWN];                                         // its elements of one bin, afterwards
   };
   float maxima[C];
-  int counts[2][C], n_list, n_own, n_few, bin;
+  int counts[2][C], found[C], bounds[2], n_list, n_own, n_few, bin;
 };
 
 template <class V, class Op>
@@ -269,7 +269,15 @@ __device__ __noinline__ void sort_down_few(u64 *shared, u64 &v, int n) {
 // elements, by one CTA.
 __device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, int n, int k, float p, uint32_t key_pmin) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  sort_down(s.list, n);
+  if (n <= FEW) {
+    u64 v = tid < n ? s.list[tid] : 0;
+    sort_down_few(s.few, v, n);
+    __syncthreads();
+    s.list[tid] = v;
+    __syncthreads();
+  } else {
+    sort_down(s.list, n);
+  }
   const int m = min(k, n);
   static_assert(FAST_K <= 128, "four warps hold the k largest");
   u64 w = 0, sum = 0;
@@ -493,9 +501,37 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
     if (m0 >= cut) atomicAdd(&s.hc[bin(m0) / BINS], 1u);
     if (m1 >= cut) atomicAdd(&s.hc[bin(m1) / BINS], 1u);
     __syncthreads();
-    // k of this CTA's thread maxima lie in the bins up to b: so do the row's k largest
-    const int b = crossing<BINS>(s, (u64)k, [&](int i) { return (u64)s.hc[i]; });
-    const float cut_k = b >= 0 ? fmaxf(cut, edge(BINS * b + BINS - 1)) : cut;
+    // The row's k largest elements lie in the bins up to the one that holds this
+    // CTA's k-th largest thread maximum, or up to the last of those that hold the
+    // CTAs' k / C-th: both from all CTAs, the best of them bounds the row.
+    {
+      const u64 part = (k + C - 1) / C;
+      u64 all, v[BINS / NT], own = 0;
+#pragma unroll
+      for (int i = 0; i < BINS / NT; ++i) own += v[i] = s.hc[tid * (BINS / NT) + i];
+      if (tid == 0) s.bounds[0] = s.bounds[1] = BINS;
+      u64 before = scan(s, own, &all);
+#pragma unroll
+      for (int i = 0; i < BINS / NT; ++i) {
+        if (before < (u64)k && (u64)k <= before + v[i]) s.bounds[0] = tid * (BINS / NT) + i;
+        if (before < part && part <= before + v[i]) s.bounds[1] = tid * (BINS / NT) + i;
+        before += v[i];
+      }
+      __syncthreads();
+      if (tid < C) {
+        cluster.map_shared_rank(&s.counts[0][0], tid)[rank] = s.bounds[0];
+        cluster.map_shared_rank(&s.counts[1][0], tid)[rank] = s.bounds[1];
+      }
+    }
+    cluster.sync();
+    int b = BINS, parts = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      b = min(b, s.counts[0][c]);
+      parts = max(parts, s.counts[1][c]);
+    }
+    b = min(b, parts);
+    const float cut_k = b < BINS ? fmaxf(cut, edge(BINS * b + BINS - 1)) : cut;
     int mine = 0;
     x.each(cut_k, [&](float y, int i) {
       ++mine;
@@ -503,11 +539,11 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
       if (at < CAP) cluster.map_shared_rank(s.list, 0)[at] = rank_word(key_of(y), i);
     });
     mine = reduce(mine, [](int x, int y) { return x + y; }, reinterpret_cast<int *>(s.red));
-    if (tid < C) cluster.map_shared_rank(&s.counts[0][0], tid)[rank] = mine;
+    if (tid < C) cluster.map_shared_rank(s.found, tid)[rank] = mine;
     cluster.sync();
     int sum = 0;
 #pragma unroll
-    for (int c = 0; c < C; ++c) sum += s.counts[0][c];
+    for (int c = 0; c < C; ++c) sum += s.found[c];
     if (sum <= CAP) {
       if (rank == 0) draw_sorted(s, a, r, f, sum, k, p, key_pmin);
       return;
