@@ -1,24 +1,30 @@
-"""Build ``libnkb.so`` (the C-ABI runtime + kernel library) in-tree.
+"""Build ``libnkb.so`` (the C-ABI runtime + kernel library) and ``nkb_torch.so`` in-tree.
 
 Every ``csrc/*.cu`` file is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) with ``nvcc`` and linked into
-``nkipy_b200/_lib/libnkb.so``.  Objects are rebuilt when their source or a
+``nkipy_b200/_lib/libnkb.so``.  ``csrc/torch_serving.cpp``, the serving calls on
+torch tensors, becomes the Python module ``_lib/nkb_torch.so`` against the
+installed torch's headers.  Objects are rebuilt when their source or a
 header is newer.  Run ``python -m nkipy_b200.build``.
 """
 
 import concurrent.futures
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(HERE, "_lib", "obj")
 LIB = os.path.join(OUT_DIR, "libnkb.so")
+TORCH_LIB = os.path.join(OUT_DIR, "nkb_torch.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CUDA_INCLUDE = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
 FLAGS = [
     "-gencode",
     "arch=compute_100a,code=sm_100a",
@@ -64,6 +70,24 @@ def _compile(src, verbose):
     return obj
 
 
+def _build_torch(verbose):
+    src = os.path.join(CSRC, "torch_serving.cpp")
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not _stale(TORCH_LIB, [src, os.path.join(INCLUDE, "nkb.h")]):
+        return
+    torch = spec.submodule_search_locations[0]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", src, "-o", TORCH_LIB]
+    cmd += [f"-I{d}" for d in (INCLUDE, os.path.join(torch, "include"), os.path.join(torch, "include/torch/csrc/api/include"),
+                               sysconfig.get_paths()["include"], CUDA_INCLUDE)]
+    cmd += [f"-L{OUT_DIR}", "-lnkb", f"-L{os.path.join(torch, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose=False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = _sources()
@@ -76,6 +100,7 @@ def build(verbose=False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_torch(verbose)
     return LIB
 
 
