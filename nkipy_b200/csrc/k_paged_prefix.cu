@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(THREADS)
   else at = single::find<S::BK>(a, [&](int64_t, int b, int64_t, int64_t) { return b == t; });
   const several::Walk walk(p, 0);
   auto unit_parts = [&](int u, int &tok, int &seq) {  // of pair u
-    const several::Pair x = several::pair_of(p, u);
+    const several::Pair x = walk.list.pair(u);
     const int64_t n = several::blocks_of(p, x).n;
     tok = t - x.tok0;
     seq = x.seq;

@@ -10,7 +10,7 @@
 // keys.  The blocks of all (pair, key head) units form one run that the
 // resident CTAs split evenly, whatever the lengths; a unit that crosses a
 // share's end is joined from partials by a second kernel.  Lengths are read on
-// the device: a small kernel lists the pairs first.
+// the device, where the pairs are listed: by a small kernel, a short list by each CTA.
 //
 // A block is taken in two halves of 64 keys, each with its own score buffer, so
 // that the scores of the next half are there when a softmax ends: the softmax
@@ -50,12 +50,22 @@ constexpr float RESCALE = 8.f;  // log2 headroom before the running maximum is r
 
 __device__ int g_tile_error = 0;
 
+// A short list is made by each CTA of the tile kernel for itself, in its shared
+// memory: that takes a microsecond or two, the kernel above and its launch four.
+constexpr int LIST = 256;  // pairs, and sequences
+struct OwnList {
+  int64_t head[LIST + 2];
+  Pair pairs[LIST];
+  int seq_pairs[LIST + 2];
+};
+
 template <int DP>
 struct Cfg {
   static constexpr int HALVES = DP / 64, TILE = HALVES * HALF, STAGES = DP == 128 ? 2 : 4;
   static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + STAGES * TILE, OFF_BAR = OFF_V + STAGES * TILE;
   static constexpr int OFF_ITEMS = OFF_BAR + 448;
-  static constexpr int SMEM = 1024 + OFF_ITEMS + RING * 64;
+  static constexpr int OFF_LIST = OFF_ITEMS + RING * 64;
+  static constexpr int SMEM = 1024 + OFF_LIST + (int)sizeof(OwnList);
   static constexpr int SLOT = slot_floats(DP);
 };
 
@@ -94,27 +104,49 @@ __device__ __forceinline__ void tokens_of(const Args &a, int i, int &first, int 
   n = max(0, min(hi, T) - first);
 }
 
-__global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Params p) {
+// Who lists: a block of SCHED threads, or one warp.
+struct Block {
+  static constexpr int N = SCHED;
+  static __device__ __forceinline__ int id() { return threadIdx.x; }
+  static __device__ __forceinline__ int64_t scan(int64_t v, int64_t *total) { return block_scan(v, total); }
+  static __device__ __forceinline__ void sync() { __syncthreads(); }
+};
+struct Warp {
+  static constexpr int N = 32;
+  static __device__ __forceinline__ int id() { return threadIdx.x & 31; }
+  static __device__ __forceinline__ int64_t scan(int64_t v, int64_t *total) {
+    int64_t x = v;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, w);
+      if (id() >= w) x += y;
+    }
+    *total = __shfl_sync(0xffffffffu, x, 31);
+    return x - v;
+  }
+  static __device__ __forceinline__ void sync() { __syncwarp(); }
+};
+template <class Group>
+__device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair *pairs, int *seq_pairs) {
   const Args &a = p.a;
   const int per = 2 * p.P, B = (int)a.seqs, T = (int)a.tokens;
   const int lists = B + 2, front = p.prefix ? (T + per - 1) / per : 0;
-  pdl_trigger();
   int64_t npairs = front;
-  for (int base = 0; base < lists; base += SCHED) {
-    const int i = base + threadIdx.x;
+  for (int base = 0; base < lists; base += Group::N) {
+    const int i = base + Group::id();
     int first, n = 0;
     if (i < lists) tokens_of(a, i, first, n);
     int64_t all;
-    const int64_t at = npairs + block_scan((n + per - 1) / per, &all);
-    if (i < lists) p.seq_pairs[i] = (int)min(at, (int64_t)p.max_pairs);
+    const int64_t at = npairs + Group::scan((n + per - 1) / per, &all);
+    if (i < lists) seq_pairs[i] = (int)min(at, (int64_t)p.max_pairs);
     npairs += all;
   }
   // the list holds max_pairs: q_start entries that overlap, which no caller means, would need more
   const int U = (int)min(npairs, (int64_t)p.max_pairs);
-  __syncthreads();
+  Group::sync();
   int64_t blocks = 0;
-  for (int base = 0; base < U; base += SCHED) {
-    const int u = base + threadIdx.x;
+  for (int base = 0; base < U; base += Group::N) {
+    const int u = base + Group::id();
     int64_t nb = 0;
     Pair x = {-2, 0, 0, 0};
     if (u < front) {
@@ -123,12 +155,12 @@ __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Pa
       int lo = 0, hi = lists - 1;  // the last list that begins at or before u
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (p.seq_pairs[mid] <= u) lo = mid;
+        if (seq_pairs[mid] <= u) lo = mid;
         else hi = mid - 1;
       }
       int first, n;
       tokens_of(a, lo, first, n);
-      const int off = (u - p.seq_pairs[lo]) * per;
+      const int off = (u - seq_pairs[lo]) * per;
       x.tok0 = first + off;
       x.ntok = max(0, min(per, n - off));
       if (lo >= 1 && lo <= B) {
@@ -138,18 +170,24 @@ __global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Pa
     }
     if (u < U) {
       nb = blocks_of(p, x).n;
-      p.pairs[u] = x;
+      pairs[u] = x;
     }
     int64_t all;
-    const int64_t at = blocks + block_scan(nb, &all);
-    if (u < U) p.head[1 + u] = at;
+    const int64_t at = blocks + Group::scan(nb, &all);
+    if (u < U) head[1 + u] = at;
     blocks += all;
   }
-  if (threadIdx.x == 0) {
-    *p.next = p.max_ctas;  // the CTAs' first units are their own numbers
-    p.head[0] = U;
-    p.head[1 + U] = blocks;
+  if (Group::id() == 0) {
+    head[0] = U;
+    head[1 + U] = blocks;
   }
+  Group::sync();
+}
+
+__global__ void __launch_bounds__(SCHED) pairs_kernel(const __grid_constant__ Params p) {
+  pdl_trigger();
+  list_pairs<Block>(p, p.head, p.pairs, p.seq_pairs);
+  if (threadIdx.x == 0) *p.next = p.max_ctas;  // the CTAs' first units are their own numbers
 }
 
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
@@ -356,7 +394,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------- segments of this CTA's share, TMA producer ----------------
       const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
       uint32_t segs = 0, blk = 0;
-      Walk walk(p, blockIdx.x);
+      OwnList *own = reinterpret_cast<OwnList *>(smem + C::OFF_LIST);
+      if (p.inside) {
+        list_pairs<Warp>(p, own->head, own->pairs, own->seq_pairs);
+        if (blockIdx.x == 0) {  // for the join
+          for (int i = lane; i < own->head[0] + 2; i += 32) p.head[i] = own->head[i];
+          for (int i = lane; i < own->head[0]; i += 32) p.pairs[i] = own->pairs[i];
+        }
+      }
+      Walk walk(p, blockIdx.x, p.inside ? own->head : p.head, p.inside ? own->pairs : p.pairs);
       Segment s;
       while (ok) {
         const bool more = walk.next(s, lane);
@@ -767,13 +813,16 @@ int launch(const Params &p, cudaStream_t st, int device) {
   if (int s = make_bf16_map(&mq, a.q, 4, dims, strides, box)) return s;
   if (int s = cache_map(&mk, a.k_cache, a, a.k_page, a.k_slot, a.k_cache_head)) return s;
   if (int s = cache_map(&mv, a.v_cache, a, a.v_page, a.v_slot, a.v_cache_head)) return s;
-  if (p.own) {
+  const bool listed = p.own && !p.inside;
+  if (listed) {
     pairs_kernel<<<1, SCHED, 0, st>>>(p);
     if (int s = launch_status("paged pairs")) return s;
   }
-  NKB_CUDA_TRY(launch_pdl(p.own, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
+  NKB_CUDA_TRY(launch_pdl(listed, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
   if (int s = launch_status("paged_tile")) return s;
-  if (p.keep || p.max_ctas < 2) return NKB_OK;
+  // nothing to join where the tokens alone make enough units for them to stay whole
+  const int64_t per = 2 * p.P, units = (a.tokens + per - 1) / per * a.kv_heads;
+  if (p.keep || p.max_ctas < 2 || units >= (int64_t)WHOLE * p.max_ctas) return NKB_OK;
   NKB_CUDA_TRY(launch_pdl(true, tile_join_kernel<T, DP>, dim3((p.max_ctas - 1) * (2 * BM / 32)), dim3(JOIN), 0, st, p));
   return launch_status("paged_tile join");
 }
@@ -809,6 +858,8 @@ int tile_params(const Args &a, int device, void *workspace, bool own, bool prefi
   p->wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
   const Layout x = layout(a, p->max_ctas, own, prefix, keep);
   p->max_pairs = x.max_pairs;
+  // (units that may stay whole are handed out by a counter that the list's kernel sets)
+  p->inside = own && x.max_pairs <= LIST && a.seqs <= LIST && x.max_pairs * a.kv_heads < (int64_t)WHOLE * p->max_ctas;
   char *w = static_cast<char *>(workspace);
   p->head = reinterpret_cast<int64_t *>(w);
   p->next = reinterpret_cast<int *>(w + x.next);

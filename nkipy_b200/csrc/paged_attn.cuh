@@ -257,6 +257,7 @@ struct Params {
   int G, P, page_shift, max_pairs, max_ctas;
   int own, prefix;  // list the sequences' own keys / the prefix
   int keep;         // write every unit as a partial
+  int inside;       // each CTA of the tile kernel lists the pairs for itself
   int wide;         // rows of out start at 32-byte boundaries
   float scale_log2;
   int64_t *head;   // number of pairs, then the pairs' first blocks (max_pairs + 1)
@@ -299,18 +300,23 @@ __device__ __forceinline__ int tile_blocks(const Params &p, const Pair &x, const
 
 // The list of pairs.  With a prefix alone (own = 0) it follows from the sizes:
 // 2 P tokens each, all of the prefix's blocks; else k_paged_tile.cu writes it.
-__device__ __forceinline__ int pairs_of(const Params &p) {
-  const int per = 2 * p.P;
-  return p.own ? (int)p.head[0] : (int)((p.a.tokens + per - 1) / per);
-}
-__device__ __forceinline__ Pair pair_of(const Params &p, int u) {
-  const int per = 2 * p.P;
-  return p.own ? p.pairs[u] : Pair{-1, u * per, min(per, (int)p.a.tokens - u * per), 0};
-}
-// blocks (per key head) before pair u
-__device__ __forceinline__ int64_t blocks_before(const Params &p, int u) {
-  return p.own ? p.head[1 + u] : u * max((int64_t)1, (p.a.prefix_len + BN - 1) / BN);
-}
+struct List {
+  const Params &p;
+  const int64_t *head;
+  const Pair *pairs;
+  __device__ __forceinline__ int size() const {
+    const int per = 2 * p.P;
+    return p.own ? (int)head[0] : (int)((p.a.tokens + per - 1) / per);
+  }
+  __device__ __forceinline__ Pair pair(int u) const {
+    const int per = 2 * p.P;
+    return p.own ? pairs[u] : Pair{-1, u * per, min(per, (int)p.a.tokens - u * per), 0};
+  }
+  // blocks (per key head) before pair u
+  __device__ __forceinline__ int64_t before(int u) const {
+    return p.own ? head[1 + u] : u * max((int64_t)1, (p.a.prefix_len + BN - 1) / BN);
+  }
+};
 
 // ---- segments: what a CTA's share holds of each unit -----------------------------
 struct Segment {
@@ -327,12 +333,15 @@ struct Segment {
 constexpr int WHOLE = 4;  // units per CTA from which they stay whole
 struct Walk {
   const Params &p;
+  const List list;
   int64_t total, f, f0, f1;
   int ctas, c, pairs, units;
   bool whole;
-  __device__ __forceinline__ Walk(const Params &q, int cta) : p(q), c(cta) {
-    pairs = pairs_of(p);
-    total = blocks_before(p, pairs) * p.a.kv_heads;
+  __device__ __forceinline__ Walk(const Params &q, int cta) : Walk(q, cta, q.head, q.pairs) {}
+  __device__ __forceinline__ Walk(const Params &q, int cta, const int64_t *head, const Pair *items)
+      : p(q), list{q, head, items}, c(cta) {
+    pairs = list.size();
+    total = list.before(pairs) * p.a.kv_heads;
     units = pairs * (int)p.a.kv_heads;
     whole = units >= WHOLE * p.max_ctas;
     ctas = workers(total, p.max_ctas);
@@ -343,7 +352,7 @@ struct Walk {
   __device__ __forceinline__ Parts parts(int u, int hk, int64_t n) const {
     const int unit = u * (int)p.a.kv_heads + hk;
     if (whole) return Parts{1, 0, 2 * p.max_ctas + unit};
-    return parts_of(total, blocks_before(p, u) * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
+    return parts_of(total, list.before(u) * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
   }
   // unit that holds block `at`: a whole warp looks, 32 pivots at a time
   __device__ __forceinline__ void locate(int64_t at, Segment &s, int lane) const {
@@ -351,19 +360,19 @@ struct Walk {
     int lo = 0, n = pairs;
     while (n > 1) {
       const int step = (n + 31) / 32, i = lane * step;
-      const uint32_t m = __ballot_sync(0xffffffffu, i < n && blocks_before(p, lo + min(i, n - 1)) <= row);
+      const uint32_t m = __ballot_sync(0xffffffffu, i < n && list.before(lo + min(i, n - 1)) <= row);
       const int last = 31 - __clz(m | 1u);
       lo += last * step;
       n = min(step, n - last * step);
     }
     set(lo, s);
-    const int in = (int)(at - blocks_before(p, lo) * p.a.kv_heads);
+    const int in = (int)(at - list.before(lo) * p.a.kv_heads);
     s.hk = in / s.k.n;
     s.k0 = in - s.hk * s.k.n;
   }
   __device__ __forceinline__ void set(int u, Segment &s) const {
     s.u = u;
-    s.x = pair_of(p, u);
+    s.x = list.pair(u);
     s.k = blocks_of(p, s.x);
   }
   // the next segment of the share (a whole warp)
