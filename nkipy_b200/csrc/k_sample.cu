@@ -93,11 +93,11 @@ __device__ __forceinline__ u64 share_of(float p, u64 total) { return max((u64)1,
 __device__ __forceinline__ u64 place(float u, u64 total) { return u >= 1.f ? total - 1 : part_of(u, total); }
 
 // ---- rows in a cluster's shared memory -------------------------------------
-constexpr int NT = 256, NW = NT / 32, C = 8;
+constexpr int NT = 256, NW = NT / 32, MAX_C = 8;
 constexpr int CAP = 2048;         // elements that a CTA lists
 constexpr int FEW = 256;          // elements that are ranked one against another
 constexpr int FAST_K = 128;       // top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit
-constexpr int MAX_SLICE = 65528;  // elements per CTA
+constexpr int MAX_SLICE = 65528;  // elements per CTA: their low halves' sum stays in 32 bits
 constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
 constexpr float SPAN = 31.1f;     // 2^-SPAN < 2^-31
 
@@ -106,7 +106,7 @@ constexpr int OWN = 3 * BINS / 2; // elements that a CTA gives to the list
 struct Shared {
   u64 list[CAP], few[FEW], weights[FEW];
   u64 row_w[BINS];                                        // weights per bin, whole row
-  u64 warp_sums[C][NW], sums[2][C], part_red[NW][16], red[NW], out[2];
+  u64 warp_sums[MAX_C][NW], sums[2][MAX_C], part_red[NW][16], red[NW], out[2];
   uint32_t row_c[BINS];                                   // counts
   union {
     struct {
@@ -114,8 +114,8 @@ struct Shared {
     };
     u64 own[OWN];                                         // its elements of one bin, afterwards
   };
-  float maxima[C];
-  int counts[2][C], found[C], bounds[2], n_list, n_own, n_few, bin;
+  float maxima[MAX_C];
+  int counts[2][MAX_C], found[MAX_C], bounds[2], n_list, n_own, n_few, bin;
 };
 
 template <class V, class Op>
@@ -372,7 +372,7 @@ struct Slice {  // a CTA's part of a row, in shared memory
 // The largest rank word that `target` elements (count) or a weight of `target`
 // reach, among the elements with rank words from `least`; *mass: the weight from
 // it up.  Bit by bit, every CTA of the cluster together.
-template <class T>
+template <class T, int C>
 __device__ __noinline__ u64 find_slowly(Shared &s, const Slice<T> &x, const Row &f, float cut, bool count, u64 target,
                                         u64 least, u64 *mass) {
   cg::cluster_group cluster = cg::this_cluster();
@@ -404,7 +404,7 @@ __device__ __noinline__ u64 find_slowly(Shared &s, const Slice<T> &x, const Row 
   return word;
 }
 
-template <class T>
+template <class T, int C>
 __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ Args a, int slice) {
   using X = Slice<T>;
   constexpr int VEC = X::VEC;
@@ -569,8 +569,7 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
         }
       });
       cluster.sync();
-      if (tid < BINS / C) {
-        const int b = rank * (BINS / C) + tid;
+      for (int b = rank * (BINS / C) + tid; b < (rank + 1) * (BINS / C); b += NT) {
         uint32_t c = 0;
         u64 w = 0;
 #pragma unroll
@@ -750,7 +749,7 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
         found = s.out[0];
         found_w = s.out[1];
       }
-      if (!found) found = find_slowly(s, x, f, cut, !mass, target, thr, &found_w);
+      if (!found) found = find_slowly<T, C>(s, x, f, cut, !mass, target, thr, &found_w);
       thr = max(thr, found);
       W = found_w;
       if (round == 0 && by_mass) {  // the list is used again
@@ -789,10 +788,11 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
   cluster.sync();
 
   // the warp in which the running sum passes the place
-  static_assert(C * NW == 64, "two sums a lane");
+  static_assert(C * NW <= 64, "two sums a lane");
   u64 total, before, mine = (&s.warp_sums[0][0])[rank * NW + warp];
   {
-    const u64 s0 = (&s.warp_sums[0][0])[2 * lane], s1 = (&s.warp_sums[0][0])[2 * lane + 1];
+    const bool in = 2 * lane < C * NW;
+    const u64 s0 = in ? (&s.warp_sums[0][0])[2 * lane] : 0, s1 = in ? (&s.warp_sums[0][0])[2 * lane + 1] : 0;
     u64 up = s0 + s1;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) {
@@ -838,12 +838,12 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
   }
 }
 
-template <class T>
+template <class T, int C>
 int launch_cluster(const Args &a, int slice, cudaStream_t st, int device) {
   const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)slice * sizeof(T);
   static ContextOnce attr;
   if (int s = attr.run(device, []() -> int {
-        NKB_CUDA_TRY(cudaFuncSetAttribute(cluster_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        NKB_CUDA_TRY(cudaFuncSetAttribute(cluster_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         return NKB_OK;
       }))
     return s;
@@ -858,15 +858,33 @@ int launch_cluster(const Args &a, int slice, cudaStream_t st, int device) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  NKB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_kernel<T>, a, slice));
+  NKB_CUDA_TRY(cudaLaunchKernelEx(&cfg, cluster_kernel<T, C>, a, slice));
   return launch_status("sample_tokens");
 }
 
-// elements per CTA; 0 where a row does not fit a cluster
-int slice_of(const Args &a) {
-  const int64_t n = ((a.vocab + C - 1) / C + 7) / 8 * 8;
-  const bool fits = n <= MAX_SLICE && (sizeof(Shared) + 15) / 16 * 16 + n * dtype_size((int)a.dtype) <= 227 * 1024;
-  return fits ? (int)n : 0;
+// elements of a CTA of c, and its shared memory
+int slice_of(const Args &a, int c) { return (int)(((a.vocab + c - 1) / c + 7) / 8 * 8); }
+size_t smem_of(const Args &a, int c) { return (sizeof(Shared) + 15) / 16 * 16 + (size_t)slice_of(a, c) * dtype_size((int)a.dtype); }
+
+// CTAs per row; 0: the row does not fit a cluster.  Eight for few rows; where that
+// makes more than two CTAs per SM, half as many while two still fit an SM: CTAs
+// that wait for a place cost more than longer slices.  Measured with top-p 0.95,
+// bf16, us with 8 / 4 / 2 / 1 CTAs per row: 8 rows of 32000 fp32 20 / 22 / 28 / 43,
+// 32 x 32000 23 / 21 / 27 / 38, 128 x 32000 76 / 46 / 33 / 39, 512 x 32000 272 /
+// 128 / 93 / 86, 128 x 151936 152 / 118 / 151 / -.
+int cluster_of(const Args &a, int device) {
+  if (slice_of(a, MAX_C) > MAX_SLICE || smem_of(a, MAX_C) > 227 * 1024) return 0;
+  int c = MAX_C;
+  while (c > 1 && a.rows * c > 2 * num_sms(device) && smem_of(a, c / 2) <= 113 * 1024) c /= 2;
+  return c;
+}
+
+template <class T>
+int launch_rows(const Args &a, int c, cudaStream_t st, int device) {
+  if (c == 1) return launch_cluster<T, 1>(a, slice_of(a, c), st, device);
+  if (c == 2) return launch_cluster<T, 2>(a, slice_of(a, c), st, device);
+  if (c == 4) return launch_cluster<T, 4>(a, slice_of(a, c), st, device);
+  return launch_cluster<T, 8>(a, slice_of(a, c), st, device);
 }
 
 // ---- rows of any length ------------------------------------------------------
@@ -1038,7 +1056,7 @@ __global__ void __launch_bounds__(THREADS) long_row_kernel(const __grid_constant
 
 int check_args(const Args &a) {
   auto bad = [](const char *m) { return fail(NKB_ERR_INVALID, std::string("sample_tokens: ") + m); };
-  if (a.rows < 0 || a.rows > INT32_MAX / C || a.vocab < 1) return bad("rows or vocab out of range");
+  if (a.rows < 0 || a.rows > INT32_MAX / MAX_C || a.vocab < 1) return bad("rows or vocab out of range");
   if (a.dtype != NKB_F32 && a.dtype != NKB_BF16 && a.dtype != NKB_F16)
     return fail(NKB_ERR_UNSUPPORTED, "sample_tokens: logits must be float32, bfloat16 or float16");
   if (a.vocab > MAX_VOCAB) return fail(NKB_ERR_UNSUPPORTED, "sample_tokens: more than 2^21 entries");
@@ -1050,10 +1068,10 @@ int check_args(const Args &a) {
 int run(const Args &a, cudaStream_t st, int device) {
   if (int s = check_args(a)) return s;
   if (a.rows == 0) return NKB_OK;
-  if (const int slice = slice_of(a)) {
-    if (a.dtype == NKB_F32) return launch_cluster<float>(a, slice, st, device);
-    if (a.dtype == NKB_BF16) return launch_cluster<__nv_bfloat16>(a, slice, st, device);
-    return launch_cluster<__half>(a, slice, st, device);
+  if (const int c = cluster_of(a, device)) {
+    if (a.dtype == NKB_F32) return launch_rows<float>(a, c, st, device);
+    if (a.dtype == NKB_BF16) return launch_rows<__nv_bfloat16>(a, c, st, device);
+    return launch_rows<__half>(a, c, st, device);
   }
   long_row_kernel<<<(unsigned)a.rows, THREADS, 0, st>>>(a);
   return launch_status("sample_tokens");

@@ -560,6 +560,21 @@ def test_sample(vocab, dtype, spread):
     check_sample(logits, u, temperature=temperature)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows, vocab", [(40, 9001), (100, 5000), (300, 700), (320, 20001)])
+def test_sample_many_rows(rows, vocab, dtype):
+    """Weights are whole numbers: a row's token is the same however many rows go with it."""
+    rng = np.random.default_rng(700 + vocab)
+    logits = (randn(rng, (rows, vocab), F32) * 2).to(dtype)
+    some = lambda values, t: torch.tensor([values[i] for i in rng.integers(len(values), size=rows)], dtype=t, device="cuda")  # noqa: E731
+    given = [torch.tensor(rng.uniform(size=rows), dtype=torch.float32, device="cuda"), some([1.0, 0.3, 2.0, 0.0], torch.float32),
+             some([0, 1, 20, 128, 300], torch.int32), some([1.0, 0.95, 0.5], torch.float32), some([0.0, 0.02], torch.float32)]
+    got = nk.sample_tokens(logits, *given).tolist()
+    assert got == [x for r in range(0, rows, 8) for x in nk.sample_tokens(logits[r:r + 8], *(g[r:r + 8] for g in given)).tolist()]
+    host = [g[:8].tolist() for g in given]
+    assert check_sample(logits[:8], *host).tolist() == got[:8]
+
+
 def test_sample_ties():
     """Equal logits rank by index: whole rows of one value, and a threshold inside a run of equals."""
     x = torch.zeros((4, 5000), device="cuda")
