@@ -352,7 +352,7 @@ NKB_API int nkb_paged_attention_workspace(const nkb_paged_attention_args *args, 
 
 /* One token per row of logits (rows, vocab), row stride in elements, drawn with
  * the row's u in [0, 1).  Weights are e = exp((x - max) / temperature) in fp32,
- * held as whole multiples of 2^-31, so every sum is exact and the result does
+ * held as whole multiples of 2^-32, so every sum is exact and the result does
  * not depend on an order of additions.  Kept: the top_k largest (0 or >= vocab:
  * all), of them the shortest run in descending order whose weights reach
  * top_p of their sum (>= 1: all), of those the ones with e >= min_p; equal

@@ -1,7 +1,7 @@
 // Draws one token per row of logits: temperature, top-k, top-p and min-p, then
 // the inverse of the kept weights' running sum at u.
 //
-// Weights are w = floor(2^31 exp((x - max) / temperature)): whole numbers, so
+// Weights are w = floor(2^32 exp((x - max) / temperature)): whole numbers, so
 // every sum below is exact and independent of its order, whatever the number
 // of threads.  A logit's key is the order-preserving image of its fp32 value
 // (-0 as +0, NaN as -inf); elements are ordered by their rank word, the key
@@ -57,27 +57,23 @@ __device__ __forceinline__ u64 rank_word(uint32_t key, int idx) {
   return ((u64)key << IDX_BITS) | (uint32_t)(MAX_VOCAB - 1 - idx);
 }
 
-// The softmax's terms.  The exponent is one fp32 product with log2(e) / temperature
-// (log2(e) in fp32 is off by 1.3e-8), and the power of two the special-function unit's (relative error
-// about 2^-22): a term is as near as the fp32 logits' difference lets it be.
+// The softmax's terms: each step is rounded to fp32 as the definition says, so that
+// the drawn token is the definition's.  (One product by log2(e) / temperature and the
+// power-of-two unit took 76 us instead of 84 for 128 mixed rows of 151936 entries, and
+// in some batches one row drew a neighbour of its token.)
 struct Row {
-  float max, scale;  // largest logit, log2(e) / temperature
-  __device__ __forceinline__ Row(float max, float temperature)
-      : max(max), scale(fminf(1.44269504f / temperature, 3.4028234e38f)) {}
-  __device__ __forceinline__ float t(float x) const { return __fmul_rn(__fsub_rn(x, max), scale); }
-  static __device__ __forceinline__ float pow2(float t) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-    return y;
-  }
-  __device__ __forceinline__ float e(float x) const { return x == max ? 1.f : x == -INFINITY ? 0.f : pow2(t(x)); }
-  // floor(2^31 e) for e in [0, 1]: the significand, moved (0 for NaN)
-  static __device__ __forceinline__ uint32_t w(float e) {
+  float max, inv;  // largest logit, 1 / temperature
+  __device__ __forceinline__ Row(float max, float temperature) : max(max), inv(fminf(1.f / temperature, 3.4028235e38f)) {}
+  __device__ __forceinline__ float t(float x) const { return __fmul_rn(__fsub_rn(x, max), inv); }
+  __device__ __forceinline__ float e(float x) const { return x == max ? 1.f : x == -INFINITY ? 0.f : expf(t(x)); }
+  // floor(2^32 e) for e in [0, 1]: the significand, moved (0 for NaN)
+  static __device__ __forceinline__ u64 w(float e) {
     const uint32_t b = __float_as_uint(e);
-    return __funnelshift_rc((b << 8) | 0x80000000u, 0, 127 - (b >> 23));
+    const uint32_t low = __funnelshift_rc((b << 8) | 0x80000000u, 0, 126 - (b >> 23));
+    return ((u64)(b == 0x3f800000u) << 32) | low;  // e = 1 alone has bit 32, and no lower bits
   }
   // weight of a logit, where max is finite: without branches (0 for -inf and NaN)
-  __device__ __forceinline__ uint32_t weight(float x) const { return w(pow2(t(x))); }
+  __device__ __forceinline__ u64 weight(float x) const { return w(expf(t(x))); }
 };
 
 // floor(p * total) for p in [0, 1), exactly: total times the significand, moved.
@@ -99,7 +95,7 @@ constexpr int FEW = 256;          // elements that are ranked one against anothe
 constexpr int FAST_K = 128;       // top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit
 constexpr int MAX_SLICE = 65528;  // elements per CTA: their low halves' sum stays in 32 bits
 constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
-constexpr float SPAN = 31.1f;     // 2^-SPAN < 2^-31
+constexpr float SPAN = 22.25f;    // e^-SPAN < 2^-32
 
 constexpr int OWN = 3 * BINS / 2; // elements that a CTA gives to the list
 
@@ -214,7 +210,7 @@ __device__ __forceinline__ uint32_t lowest_key(uint32_t top, float guess, Yes ye
 __device__ __forceinline__ int bin_of(const Row &f, float x) { return min(QN - 1, (int)__fmul_rn(f.t(x), -(float)QN / SPAN)); }
 __device__ __noinline__ float edge_of(const Row &f, int q) {
   if (q < 0) return __uint_as_float(0x7fc00000u);
-  return of_key(lowest_key(key_of(f.max), f.max - (float)(q + 1) * (SPAN / QN) / f.scale, [&](float x) { return bin_of(f, x) <= q; }));
+  return of_key(lowest_key(key_of(f.max), f.max - (float)(q + 1) * (SPAN / QN) / f.inv, [&](float x) { return bin_of(f, x) <= q; }));
 }
 
 // Sorts list[0, n), n <= CAP, largest first (a bitonic network, padded with zeros
@@ -493,8 +489,8 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
   float pmin = a.min_p ? a.min_p[r] : 0.f;
   pmin = pmin > 1.f ? 1.f : pmin;
   // the lowest logit that has a weight: below it (and NaN) nothing matters
-  const float cut = of_key(lowest_key(kmax, gmax - 31.f / f.scale, [&](float x) { return Row::w(f.e(x)) > 0; }));
-  const uint32_t key_pmin = pmin > 0.f ? lowest_key(kmax, gmax + log2f(pmin) / f.scale, [&](float x) { return f.e(x) >= pmin; }) : 0;
+  const float cut = of_key(lowest_key(kmax, gmax - 22.180709f / f.inv, [&](float x) { return Row::w(f.e(x)) > 0; }));
+  const uint32_t key_pmin = pmin > 0.f ? lowest_key(kmax, gmax + logf(pmin) / f.inv, [&](float x) { return f.e(x) >= pmin; }) : 0;
   u64 thr = 0;  // rank word of the last element that is kept
 
   if (by_count && k <= FAST_K) {
@@ -561,11 +557,11 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           if (!(y[i] >= from) || y[i] >= end) continue;
-          const uint32_t w = f.weight(y[i]);
+          const u64 w = f.weight(y[i]);
           const int b = (bin(y[i]) - base) >> shift;
           if (by_count) atomicAdd(&s.hc[b], 1u);
-          atomicAdd(&s.hl[b], w & 0xffffu);
-          atomicAdd(&s.hh[b], w >> 16);
+          atomicAdd(&s.hl[b], (uint32_t)w & 0xffffu);
+          atomicAdd(&s.hh[b], (uint32_t)(w >> 16));
         }
       });
       cluster.sync();
@@ -766,7 +762,7 @@ __global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ 
   const float tie = thr ? of_key((uint32_t)(thr >> IDX_BITS)) : -INFINITY;
   const int tie_idx = (int)(MAX_VOCAB - 1 - (thr & (MAX_VOCAB - 1)));
   auto kept = [&](float y, int i) -> u64 {
-    const uint32_t w = f.weight(y);
+    const u64 w = f.weight(y);
     return y >= from && !(y == tie && i > tie_idx) ? w : 0;
   };
   u64 sum_kept = 0;
