@@ -6,7 +6,11 @@
 // keys and values are read once per 2 P tokens instead of once per sequence.
 // Each sequence's own keys take the form for single tokens or for several, and
 // both leave partials (max, sum, unnormalised output) that the kernel here
-// joins per token and head.
+// joins per token and head.  Measured (32 / 8 heads of 128 bf16, GPU time): 64
+// sequences with some hundred keys each after a prefix of 8192, 47 us (the floor is
+// 14 us of reads; prefix 22, own keys 19 and join 12 us one by one, each in part
+// under the next: few blocks per CTA, so each is mostly its start and its partials);
+// 4 sequences after a prefix of 1000, 15.5 us.
 #include "paged_attn.cuh"
 
 namespace nkb {

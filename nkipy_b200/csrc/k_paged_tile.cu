@@ -30,6 +30,14 @@
 // not read (TMA fills zeros), and the unseen V rows of the others are set to
 // zero in shared memory before the product that would multiply them by zero.
 // TMEM: two score buffers of 64 columns and O of up to 128 for each tile.  Every wait is bounded.
+//
+// What bounds it is the softmax between the two products: the exponentials take as
+// many cycles as the products at head dimension 128 and twice as many at 64, so
+// 3/8 of them are polynomials on the FMA pipe.  Measured (GPU time): 4 prompts of
+// 2048 tokens, window 1024, 32 / 8 heads of 128 bf16, 134 us or 773 TFLOP/s of the
+// keys seen (tensor pipe busy 44 %, issue slots 44 %); 500 tokens over 16400 keys,
+// 32 / 4 heads of 64 fp16, 132 us with 14 of them in the join, 501 TFLOP/s (tensor
+// 30 %, exponential unit 38 %, issue 52 %).
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 
@@ -54,7 +62,7 @@ __device__ int g_tile_error = 0;
 // memory: that takes a microsecond or two, the kernel above and its launch four.
 constexpr int LIST = 256;  // pairs, and sequences
 struct OwnList {
-  int64_t head[LIST + 2];
+  int64_t head[LIST + 3];
   Pair pairs[LIST];
   int seq_pairs[LIST + 2];
 };
@@ -109,6 +117,14 @@ struct Block {
   static constexpr int N = SCHED;
   static __device__ __forceinline__ int id() { return threadIdx.x; }
   static __device__ __forceinline__ int64_t scan(int64_t v, int64_t *total) { return block_scan(v, total); }
+  static __device__ __forceinline__ int largest(int v) {
+    __shared__ int s;
+    if (threadIdx.x == 0) s = 0;
+    __syncthreads();
+    atomicMax(&s, v);
+    __syncthreads();
+    return s;
+  }
   static __device__ __forceinline__ void sync() { __syncthreads(); }
 };
 struct Warp {
@@ -124,6 +140,7 @@ struct Warp {
     *total = __shfl_sync(0xffffffffu, x, 31);
     return x - v;
   }
+  static __device__ __forceinline__ int largest(int v) { return __reduce_max_sync(0xffffffffu, v); }
   static __device__ __forceinline__ void sync() { __syncwarp(); }
 };
 template <class Group>
@@ -145,6 +162,7 @@ __device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair 
   const int U = (int)min(npairs, (int64_t)p.max_pairs);
   Group::sync();
   int64_t blocks = 0;
+  int longest = 0;
   for (int base = 0; base < U; base += Group::N) {
     const int u = base + Group::id();
     int64_t nb = 0;
@@ -170,6 +188,7 @@ __device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair 
     }
     if (u < U) {
       nb = blocks_of(p, x).n;
+      longest = max(longest, (int)nb);
       pairs[u] = x;
     }
     int64_t all;
@@ -177,9 +196,11 @@ __device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair 
     if (u < U) head[1 + u] = at;
     blocks += all;
   }
+  longest = Group::largest(longest);
   if (Group::id() == 0) {
     head[0] = U;
     head[1 + U] = blocks;
+    head[2 + U] = longest;
   }
   Group::sync();
 }
@@ -398,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (p.inside) {
         list_pairs<Warp>(p, own->head, own->pairs, own->seq_pairs);
         if (blockIdx.x == 0) {  // for the join
-          for (int i = lane; i < own->head[0] + 2; i += 32) p.head[i] = own->head[i];
+          for (int i = lane; i < own->head[0] + 3; i += 32) p.head[i] = own->head[i];
           for (int i = lane; i < own->head[0]; i += 32) p.pairs[i] = own->pairs[i];
         }
       }
@@ -776,7 +797,7 @@ Layout layout(const Args &a, int max_ctas, bool own, bool prefix, bool keep) {
   // every sequence, and the tokens before and after them, may end in a part of a pair
   x.max_pairs = (int)((prefix ? (T + per - 1) / per : 0) + (own ? T / per + a.seqs + 2 : 0));
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  x.next = ((size_t)x.max_pairs + 2) * 8;
+  x.next = ((size_t)x.max_pairs + 3) * 8;
   x.pairs = up(x.next + 8);
   x.seqs = x.pairs + up((size_t)x.max_pairs * sizeof(Pair));
   x.ws = x.seqs + up((size_t)(own ? a.seqs + 2 : 0) * 4);
@@ -858,8 +879,8 @@ int tile_params(const Args &a, int device, void *workspace, bool own, bool prefi
   p->wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
   const Layout x = layout(a, p->max_ctas, own, prefix, keep);
   p->max_pairs = x.max_pairs;
-  // (units that may stay whole are handed out by a counter that the list's kernel sets)
-  p->inside = own && x.max_pairs <= LIST && a.seqs <= LIST && x.max_pairs * a.kv_heads < (int64_t)WHOLE * p->max_ctas;
+  // (more units than CTAs may be handed out one by one, by a counter that the list's kernel sets)
+  p->inside = own && x.max_pairs <= LIST && a.seqs <= LIST && x.max_pairs * a.kv_heads <= p->max_ctas;
   char *w = static_cast<char *>(workspace);
   p->head = reinterpret_cast<int64_t *>(w);
   p->next = reinterpret_cast<int *>(w + x.next);

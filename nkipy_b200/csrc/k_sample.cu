@@ -8,22 +8,24 @@
 // above the complement of the index, so equal logits rank by index and the
 // kept set is "rank word >= threshold", with e >= min_p.
 //
-// A cluster of 8 CTAs holds a row in its shared memory: the logits are read from
-// memory once.  What bounds the kernel is then the instructions per element and
+// A cluster of up to 8 CTAs holds a row in its shared memory: the logits are read
+// from memory once.  What bounds the kernel is then the instructions per element and
 // the cluster's meetings (about a microsecond each), so each way of filtering has
-// the fewest it can:
-//   greedy  the CTAs' maxima: one meeting
-//   top-k   of up to FAST_K: a CTA's k-th largest thread maximum bounds the row's
-//           k-th largest element; what passes (some 8 k elements) goes to one CTA,
-//           which sorts it, applies the other filters and draws alone: two
+// the fewest it can (GPU times for 1 row of 32000 fp32, and 128 rows of 151936 bf16,
+// whose 39 MB a copy reads in 6 us):
+//   greedy  the CTAs' maxima: one meeting; 3 and 16 us
+//   top-k   of up to FAST_K: the CTAs' largest thread maxima bound the row's k-th
+//           largest element; what passes (two to three k elements) goes to one CTA,
+//           which sorts it, applies the other filters and draws alone: three; 10 and
+//           35 us for k = 50
 //   top-p, other top-k   a histogram of counts and exact weights over 512 bins
 //           linear in (max - x) / temperature, summed over the cluster (again
 //           within the threshold's bin if that holds too many); the elements of
-//           the threshold's bin go to every CTA, which narrows them down and ranks
-//           the last few one against another: five (one more for both)
+//           the threshold's bin go to every CTA, which narrows them down and sorts
+//           the last few: five (more for both); 21 and 151 us for p = 0.95
 //   none    the kept weight of each warp, whose part of the row is contiguous; the
 //           warp in which the running sum passes u times the total walks its part:
-//           two
+//           two; 6 and 50 us
 // Where that does not do (thousands of equal logits at a threshold) the threshold
 // is found bit by bit over the cluster.
 
@@ -91,7 +93,7 @@ __device__ __forceinline__ u64 place(float u, u64 total) { return u >= 1.f ? tot
 // ---- rows in a cluster's shared memory -------------------------------------
 constexpr int NT = 256, NW = NT / 32, MAX_C = 8;
 constexpr int CAP = 2048;         // elements that a CTA lists
-constexpr int FEW = 256;          // elements that are ranked one against another
+constexpr int FEW = 256;          // elements that are sorted one a thread
 constexpr int FAST_K = 128;       // top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit
 constexpr int MAX_SLICE = 65528;  // elements per CTA: their low halves' sum stays in 32 bits
 constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
@@ -100,7 +102,7 @@ constexpr float SPAN = 22.25f;    // e^-SPAN < 2^-32
 constexpr int OWN = 3 * BINS / 2; // elements that a CTA gives to the list
 
 struct Shared {
-  u64 list[CAP], few[FEW], weights[FEW];
+  u64 list[CAP], few[FEW], weights[FAST_K];
   u64 row_w[BINS];                                        // weights per bin, whole row
   u64 warp_sums[MAX_C][NW], sums[2][MAX_C], part_red[NW][16], red[NW], out[2];
   uint32_t row_c[BINS];                                   // counts
@@ -865,9 +867,10 @@ size_t smem_of(const Args &a, int c) { return (sizeof(Shared) + 15) / 16 * 16 + 
 // CTAs per row; 0: the row does not fit a cluster.  Eight for few rows; where that
 // makes more than two CTAs per SM, half as many while two still fit an SM: CTAs
 // that wait for a place cost more than longer slices.  Measured with top-p 0.95,
-// bf16, us with 8 / 4 / 2 / 1 CTAs per row: 8 rows of 32000 fp32 20 / 22 / 28 / 43,
-// 32 x 32000 23 / 21 / 27 / 38, 128 x 32000 76 / 46 / 33 / 39, 512 x 32000 272 /
-// 128 / 93 / 86, 128 x 151936 152 / 118 / 151 / -.
+// bf16, us with 8 / 4 / 2 / 1 CTAs per row: 8 rows of 32000 fp32 21 / 25 / 34 / 55,
+// 32 x 32000 26 / 23 / 33 / 48, 128 x 32000 81 / 51 / 40 / 50, 512 x 32000 288 /
+// 142 / 111 / 109, 128 x 151936 173 / 142 / 198 / -; with top-k 50 300 x 2000 55 /
+// 33 / 23 / 12.
 int cluster_of(const Args &a, int device) {
   if (slice_of(a, MAX_C) > MAX_SLICE || smem_of(a, MAX_C) > 227 * 1024) return 0;
   int c = MAX_C;

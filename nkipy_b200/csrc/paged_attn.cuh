@@ -260,7 +260,7 @@ struct Params {
   int inside;       // each CTA of the tile kernel lists the pairs for itself
   int wide;         // rows of out start at 32-byte boundaries
   float scale_log2;
-  int64_t *head;   // number of pairs, then the pairs' first blocks (max_pairs + 1)
+  int64_t *head;   // number of pairs, the pairs' first blocks (max_pairs + 1), the longest one's blocks
   int *next;       // the next unit that no CTA has, where whole units are handed out
   Pair *pairs;
   int *seq_pairs;  // first pair of each sequence (scheduler only)
@@ -316,6 +316,8 @@ struct List {
   __device__ __forceinline__ int64_t before(int u) const {
     return p.own ? head[1 + u] : u * max((int64_t)1, (p.a.prefix_len + BN - 1) / BN);
   }
+  // blocks of the longest of n pairs
+  __device__ __forceinline__ int64_t longest(int n) const { return p.own ? head[2 + n] : before(1); }
 };
 
 // ---- segments: what a CTA's share holds of each unit -----------------------------
@@ -326,11 +328,23 @@ struct Segment {
   bool all;           // the whole unit
   int slot;           // of its partial
 };
-// Where there are many units a CTA takes whole ones, the last pairs first (under
-// a causal mask the longest), the next when it has done one: no partial is
-// written, and the CTAs end within a unit of one another.  With few, their
-// blocks are shared evenly.
-constexpr int WHOLE = 4;  // units per CTA from which they stay whole
+// The units' blocks are shared evenly over the CTAs, which cuts units: partials are
+// written and joined, and a CTA may get many short units, each with its own start and
+// end.  Or a CTA takes whole units, the last pairs first (under a causal mask the
+// longest), the next when it has done one.  Cutting costs some 3 blocks' time, and 6
+// for each unit that a CTA gets (up to 4); staying whole costs what the last units
+// take beyond an equal share, half a unit where lengths vary.  The cheaper one, by
+// that estimate.  Measured, us, cut and whole (32 / 8 heads of 128 bf16): 512 tokens
+// 32 / 20, 1024 40 / 28, 2048 80 / 46, 2 x 2048 133 / 80, 8 x 128 after 4000 each 94 /
+// 75; 128 after 2000 36 / 43, 512 after 4000 61 / 76, 8 x 160 after 4000 121 / 136.
+constexpr int WHOLE = 6;  // units per CTA from which they always stay whole
+__device__ __forceinline__ bool stay_whole(int64_t total, int64_t longest, int units, int ctas) {
+  if (units >= WHOLE * ctas) return true;
+  const float n = (float)ctas, equal = (float)total / n, most = (float)longest;
+  const int rounds = (units + ctas - 1) / ctas;
+  const float whole = rounds == 1 ? most : fminf((float)rounds * most, equal + most / 2);
+  return whole <= equal + 3 + 6 * fminf((float)units / n, 4);
+}
 struct Walk {
   const Params &p;
   const List list;
@@ -343,7 +357,7 @@ struct Walk {
     pairs = list.size();
     total = list.before(pairs) * p.a.kv_heads;
     units = pairs * (int)p.a.kv_heads;
-    whole = units >= WHOLE * p.max_ctas;
+    whole = stay_whole(total, list.longest(pairs), units, p.max_ctas);
     ctas = workers(total, p.max_ctas);
     f0 = c < ctas ? share(total, c, ctas) : 0;
     f1 = c < ctas ? share(total, c + 1, ctas) : 0;
@@ -379,9 +393,12 @@ struct Walk {
   __device__ __forceinline__ bool next(Segment &s, int lane) {
     if (whole) {
       int i = c;
-      if (!p.own) i += (int)(f - f0) * p.max_ctas;  // all of a length
-      else if (f != f0 && lane == 0) i = atomicAdd(p.next, 1);
-      i = __shfl_sync(0xffffffffu, i, 0);
+      if (!p.own || p.inside) {  // all of a length, or one each
+        i += (int)(f - f0) * p.max_ctas;
+      } else if (f != f0) {  // the next that no CTA has
+        if (lane == 0) i = atomicAdd(p.next, 1);
+        i = __shfl_sync(0xffffffffu, i, 0);
+      }
       ++f;
       if (i >= units) return false;
       i = units - 1 - i;
