@@ -68,19 +68,18 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
   float2 *s_ml = reinterpret_cast<float2 *>(smem + S::STAGES * S::QBUF + WARPS * S::RING);  // (max, sum) of the warps' rows
 
   const Found at = find<S::BK>(a, [&](int64_t blocks, int, int64_t first, int64_t n) {
-    const int ctas = workers(blocks * heads, p.ctas);
-    const int64_t f = share(blocks * heads, min(c, ctas - 1), ctas);
+    const Split split(blocks * heads, p.ctas);
+    const int64_t f = split.first(min(c, split.ctas - 1));
     return first * heads <= f && f < (first + n) * heads;
   });
   pdl_trigger();
-  const int64_t total = at.total * heads;
-  const int ctas = workers(total, p.ctas);
-  if (c >= ctas) {
+  const Split split(at.total * heads, p.ctas);
+  if (c >= split.ctas) {
     pdl_wait();
     return;
   }
-  const int64_t f0 = share(total, c, ctas);
-  const int n_blocks = (int)(share(total, c + 1, ctas) - f0);
+  const int64_t f0 = split.first(c);
+  const int n_blocks = (int)(split.first(c + 1) - f0);
 
   // a place in the share: block k of nb of a (sequence, 16-row group of heads)
   struct At {
@@ -338,8 +337,8 @@ __global__ void __launch_bounds__(THREADS) decode_join_kernel(const __grid_const
   const int hk = unit / p.groups, h0 = hk * G + (unit % p.groups) * ROWS, rows = min(ROWS, (hk + 1) * G - h0);
   const Found at = find<S::BK>(a, [&](int64_t, int s, int64_t, int64_t) { return s == b; });
   const int nb = blocks_of<S::BK>(a, b);
-  const int64_t total = at.total * heads, first = at.before * heads + (int64_t)unit * nb;
-  const Parts parts = parts_of(total, first, nb, p.ctas, blockIdx.x);
+  const int64_t first = at.before * heads + (int64_t)unit * nb;
+  const Parts parts = parts_of(Split(at.total * heads, p.ctas), first, nb, p.ctas, blockIdx.x);
   pdl_wait();  // in every block: the grid must not end before the one it follows
   if (parts.n == 1 && !p.keep) return;  // one CTA held it whole
   for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(THREADS)
   const int heads = (int)a.kv_heads * s.groups;
   auto own_parts = [&](int g) {
     const int unit = hk * s.groups + g / single::ROWS, nb = single::blocks_of<S::BK>(a, t);
-    return parts_of(at.total * heads, at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
+    return parts_of(Split(at.total * heads, s.ctas), at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
   };
   if (!p.own) {
     own = own_parts(min((int)threadIdx.x / (DP / 4), G - 1));

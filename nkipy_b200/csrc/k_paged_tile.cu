@@ -144,7 +144,7 @@ struct Warp {
   static __device__ __forceinline__ void sync() { __syncwarp(); }
 };
 template <class Group>
-__device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair *pairs, int *seq_pairs) {
+__device__ __noinline__ void list_pairs(const Params &p, int64_t *head, Pair *pairs, int *seq_pairs) {
   const Args &a = p.a;
   const int per = 2 * p.P, B = (int)a.seqs, T = (int)a.tokens;
   const int lists = B + 2, front = p.prefix ? (T + per - 1) / per : 0;
@@ -758,13 +758,13 @@ __global__ void __launch_bounds__(JOIN) tile_join_kernel(const __grid_constant__
   const Args &a = p.a;
   const Walk walk(p, 0);
   if (walk.whole) return;
-  for (int item = blockIdx.x; item < (walk.ctas - 1) * PARTS; item += gridDim.x) {
+  for (int item = blockIdx.x; item < (walk.split.ctas - 1) * PARTS; item += gridDim.x) {
     const int c = item / PARTS + 1;
-    const int64_t cut = share(walk.total, c, walk.ctas);
+    const int64_t cut = walk.split.first(c);
     Segment s;
     walk.locate(cut, s, threadIdx.x % 32);
     if (s.k0 == 0) continue;  // the share begins with the unit
-    const Parts parts = parts_of(walk.total, cut - s.k0, s.k.n, p.max_ctas, 0);
+    const Parts parts = parts_of(walk.split, cut - s.k0, s.k.n, p.max_ctas, 0);
     if (parts.c0 != c - 1) continue;
     for (int i = threadIdx.x; i < 32 * (DP / 4); i += JOIN) {
       const int row = item % PARTS * 32 + i / (DP / 4), d = i % (DP / 4) * 4, t = row / BM, r = row % BM;

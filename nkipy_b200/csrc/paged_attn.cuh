@@ -28,17 +28,27 @@ __device__ __forceinline__ Visible visible(int64_t pos, int64_t cap, int64_t win
 
 // ---- work split evenly over the resident CTAs --------------------------------
 // The key blocks of all units, one run of `total`, are cut into equal shares.
-// CTAs that share the blocks: none of them is left without one
-__host__ __device__ __forceinline__ int workers(int64_t total, int ctas) { return total < ctas ? (int)total : ctas; }
-// first block of CTA c's share
-__device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) { return total * c / ctas; }
-// CTA whose share holds block f
-__device__ __forceinline__ int owner(int64_t total, int64_t f, int ctas) {
-  int c = (int)(f * ctas / total);
-  while (share(total, c + 1, ctas) <= f) ++c;
-  while (share(total, c, ctas) > f) --c;
-  return c;
+// (Few instructions, and few divisions among them: in calls of a few microseconds
+// each of these steps is run once, from memory.)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
+struct Split {
+  int64_t total, each;  // blocks; of a share, and one more for the first `more` CTAs
+  int ctas, more;       // CTAs that share: none of them is left without a block
+  __device__ __forceinline__ Split(int64_t blocks, int max_ctas)
+      : total(blocks), ctas(blocks < max_ctas ? max(1, (int)blocks) : max_ctas) {
+    each = quotient(total, ctas);
+    more = (int)(total - each * ctas);
+  }
+  // first block of CTA c's share
+  __device__ __forceinline__ int64_t first(int c) const { return each * c + min(c, more); }
+  // CTA whose share holds block f
+  __device__ __forceinline__ int owner(int64_t f) const {
+    const int64_t longer = (each + 1) * more;
+    return (int)(f < longer ? quotient(f, each + 1) : more + quotient(f - longer, each));
+  }
+};
 // The partials of a unit whose blocks are [first, first + nb): the slots they
 // lie in.  A CTA's first segment has slot 2c, a later one that goes on in the
 // next CTA 2c + 1; a unit that one CTA holds whole is written out at once, or,
@@ -47,12 +57,12 @@ struct Parts {
   int n, c0, s0;
   __device__ __forceinline__ int slot(int i) const { return i ? 2 * (c0 + i) : s0; }
 };
-__device__ __forceinline__ Parts parts_of(int64_t total, int64_t first, int64_t nb, int max_ctas, int64_t unit) {
-  const int ctas = workers(total, max_ctas), c0 = owner(total, first, ctas), c1 = owner(total, first + nb - 1, ctas);
+__device__ __forceinline__ Parts parts_of(const Split &split, int64_t first, int64_t nb, int max_ctas, int64_t unit) {
+  const int c0 = split.owner(first), c1 = split.owner(first + nb - 1);
   Parts p;
   p.n = c1 - c0 + 1;
   p.c0 = c0;
-  p.s0 = c0 == c1 ? 2 * max_ctas + (int)unit : 2 * c0 + (share(total, c0, ctas) != first);
+  p.s0 = c0 == c1 ? 2 * max_ctas + (int)unit : 2 * c0 + (split.first(c0) != first);
   return p;
 }
 
@@ -340,37 +350,35 @@ struct Segment {
 constexpr int WHOLE = 6;  // units per CTA from which they always stay whole
 __device__ __forceinline__ bool stay_whole(int64_t total, int64_t longest, int units, int ctas) {
   if (units >= WHOLE * ctas) return true;
-  const float n = (float)ctas, equal = (float)total / n, most = (float)longest;
+  // in blocks times CTAs
   const int rounds = (units + ctas - 1) / ctas;
-  const float whole = rounds == 1 ? most : fminf((float)rounds * most, equal + most / 2);
-  return whole <= equal + 3 + 6 * fminf((float)units / n, 4);
+  const int64_t one = longest * ctas, whole = rounds == 1 ? one : min(rounds * one, total + one / 2);
+  return whole <= total + 3 * ctas + 6 * min(units, 4 * ctas);
 }
 struct Walk {
   const Params &p;
   const List list;
-  int64_t total, f, f0, f1;
-  int ctas, c, pairs, units;
+  int pairs, c, units;
+  Split split;
+  int64_t f, f0, f1;
   bool whole;
   __device__ __forceinline__ Walk(const Params &q, int cta) : Walk(q, cta, q.head, q.pairs) {}
   __device__ __forceinline__ Walk(const Params &q, int cta, const int64_t *head, const Pair *items)
-      : p(q), list{q, head, items}, c(cta) {
-    pairs = list.size();
-    total = list.before(pairs) * p.a.kv_heads;
-    units = pairs * (int)p.a.kv_heads;
-    whole = stay_whole(total, list.longest(pairs), units, p.max_ctas);
-    ctas = workers(total, p.max_ctas);
-    f0 = c < ctas ? share(total, c, ctas) : 0;
-    f1 = c < ctas ? share(total, c + 1, ctas) : 0;
+      : p(q), list{q, head, items}, pairs(list.size()), c(cta), units(pairs * (int)p.a.kv_heads),
+        split(list.before(pairs) * p.a.kv_heads, p.max_ctas) {
+    whole = stay_whole(split.total, list.longest(pairs), units, p.max_ctas);
+    f0 = c < split.ctas ? split.first(c) : 0;
+    f1 = c < split.ctas ? split.first(c + 1) : 0;
     f = f0;
   }
   __device__ __forceinline__ Parts parts(int u, int hk, int64_t n) const {
     const int unit = u * (int)p.a.kv_heads + hk;
     if (whole) return Parts{1, 0, 2 * p.max_ctas + unit};
-    return parts_of(total, list.before(u) * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
+    return parts_of(split, list.before(u) * p.a.kv_heads + hk * n, n, p.max_ctas, unit);
   }
   // unit that holds block `at`: a whole warp looks, 32 pivots at a time
   __device__ __forceinline__ void locate(int64_t at, Segment &s, int lane) const {
-    const int64_t row = at / p.a.kv_heads;  // pairs are kv_heads * n blocks long
+    const int64_t row = quotient(at, p.a.kv_heads);  // pairs are kv_heads * n blocks long
     int lo = 0, n = pairs;
     while (n > 1) {
       const int step = (n + 31) / 32, i = lane * step;
