@@ -144,7 +144,7 @@ struct Warp {
   static __device__ __forceinline__ void sync() { __syncwarp(); }
 };
 template <class Group>
-__device__ __noinline__ void list_pairs(const Params &p, int64_t *head, Pair *pairs, int *seq_pairs) {
+__device__ __forceinline__ void list_pairs(const Params &p, int64_t *head, Pair *pairs, int *seq_pairs) {
   const Args &a = p.a;
   const int per = 2 * p.P, B = (int)a.seqs, T = (int)a.tokens;
   const int lists = B + 2, front = p.prefix ? (T + per - 1) / per : 0;
@@ -338,7 +338,9 @@ struct Desc {
   }
 };
 
-template <class T, int DP>
+// INSIDE: the CTA lists the pairs for itself.  (Two kernels, not a branch: with the
+// listing beside it the others' walk took 1 to 4 us more per call.)
+template <class T, int DP, bool INSIDE>
 __global__ void __launch_bounds__(THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
@@ -415,15 +417,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------- segments of this CTA's share, TMA producer ----------------
       const int ps = (int)a.page_size, box = min(ps, BN), npb = BN / box;  // pages (or page parts) per block
       uint32_t segs = 0, blk = 0;
-      OwnList *own = reinterpret_cast<OwnList *>(smem + C::OFF_LIST);
-      if (p.inside) {
+      const int64_t *head = p.head;
+      const Pair *pairs = p.pairs;
+      if constexpr (INSIDE) {
+        OwnList *own = reinterpret_cast<OwnList *>(smem + C::OFF_LIST);
         list_pairs<Warp>(p, own->head, own->pairs, own->seq_pairs);
         if (blockIdx.x == 0) {  // for the join
           for (int i = lane; i < own->head[0] + 3; i += 32) p.head[i] = own->head[i];
           for (int i = lane; i < own->head[0]; i += 32) p.pairs[i] = own->pairs[i];
         }
+        head = own->head;
+        pairs = own->pairs;
       }
-      Walk walk(p, blockIdx.x, p.inside ? own->head : p.head, p.inside ? own->pairs : p.pairs);
+      Walk walk(p, blockIdx.x, head, pairs);
       Segment s;
       while (ok) {
         const bool more = walk.next(s, lane);
@@ -820,7 +826,8 @@ template <class T, int DP>
 int launch(const Params &p, cudaStream_t st, int device) {
   static ContextOnce attr;
   if (int s = attr.run(device, []() -> int {
-        NKB_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
+        NKB_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
+        NKB_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
         return NKB_OK;
       }))
     return s;
@@ -839,7 +846,8 @@ int launch(const Params &p, cudaStream_t st, int device) {
     pairs_kernel<<<1, SCHED, 0, st>>>(p);
     if (int s = launch_status("paged pairs")) return s;
   }
-  NKB_CUDA_TRY(launch_pdl(listed, tile_kernel<T, DP>, dim3(p.max_ctas), dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
+  NKB_CUDA_TRY(launch_pdl(listed, p.inside ? tile_kernel<T, DP, true> : tile_kernel<T, DP, false>, dim3(p.max_ctas),
+                          dim3(THREADS), Cfg<DP>::SMEM, st, mq, mk, mv, p));
   if (int s = launch_status("paged_tile")) return s;
   // nothing to join where the tokens alone make enough units for them to stay whole
   const int64_t per = 2 * p.P, units = (a.tokens + per - 1) / per * a.kv_heads;
