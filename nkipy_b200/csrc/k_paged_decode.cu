@@ -16,9 +16,9 @@
 // ring that began anew at each, 8 sequences of 2048 keys took 22.3 us, 64 of 4100
 // 175 us.  Two CTAs to an SM keep 128 KB on their way there.  Measured (32 / 8 heads
 // of 128 bf16, GPU time with the join): 64 sequences of 4100 keys 171 us, 6.2 of the
-// 6.5 TB/s of a copy; 8 of 2048 19.6 us, 3.4 TB/s, of which some 5 us pass before the
-// first keys are there (length, page and key are read one after another) and 3 in
-// the join; one of 500 6.1 us.
+// 6.5 TB/s of a copy; 8 of 2048 19.2 us, 3.5 TB/s: a share is seven blocks there, and
+// before the first of them length, page and key are read one after another, after
+// the last comes the join; one of 500 5.9 us.  The matrix units are far from busy.
 //
 // In a CTA the (up to 16) query heads of the key head are the rows of one m16
 // tile; each of four warps takes every fourth group of WN keys through its own
