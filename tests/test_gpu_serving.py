@@ -453,6 +453,55 @@ def test_prefix(case):
     check_attention(got, want, mag, dtype)
 
 
+SHARES = [
+    # news, pasts, window, sinks, hq, hkv, d, page, dtype, layout
+    ([5] * 12, range(40, 52), 0, 0, 4, 2, 64, 16, BF16, "slots"),  # fewer units than CTAs: one each
+    ([200, 3], [3000, 0], 0, 0, 4, 2, 128, 32, F16, "slots"),  # few long ones: cut
+    ([7] * 40, range(40), 0, 0, 16, 8, 64, 16, BF16, "slots"),  # some units per CTA
+    ([70, 1] * 20, [30, 700] * 20, 60, 2, 32, 4, 128, 16, BF16, "slots"),
+    ([7] * 20, [6000] + [10] * 19, 0, 0, 8, 8, 64, 128, BF16, "slots"),  # one much longer than a share: cut
+    ([2] * 300, range(300), 0, 0, 2, 1, 64, 16, F16, "slots"),  # a long list
+    ([3] * 120, range(120), 0, 0, 8, 8, 128, 16, BF16, "slots"),  # many units per CTA
+]
+
+
+@pytest.mark.parametrize("case", range(len(SHARES)))
+def test_shares_of_work(case):
+    news, pasts, *rest = SHARES[case]
+    run_attention(400 + case, news, list(pasts), *rest)
+
+
+@pytest.mark.parametrize("prefix, news, hq, hkv", [
+    (40, [1] * 300, 64, 8),  # several rounds of whole units
+    (40, [3] * 90, 8, 8),    # with units of the sequences' own
+    (20, [1, 2], 4, 2),
+    (3000, [2, 1, 1], 4, 2),
+    (600, [1] * 130, 16, 1),
+])
+def test_prefix_shares_of_work(prefix, news, hq, hkv):
+    d, page = 64, 16
+    rng = np.random.default_rng(prefix + len(news))
+    n_pages = -(-prefix // page)
+    cache = Paged(rng, news, hkv, d, page, BF16, "slots", extra=n_pages)
+    pages, where = cache.free[:n_pages], np.arange(prefix)
+    at_p = torch.tensor(pages[where // page], dtype=torch.long, device="cuda"), torch.tensor(where % page, device="cuda")
+    for c in (cache.k, cache.v):
+        c[at_p] = randn(rng, (prefix, hkv, d), BF16)
+    pk, pv, T = f64(cache.k[at_p]), f64(cache.v[at_p]), sum(news)
+    q = randn(rng, (T, hq, d), BF16)
+    want, mag, at = np.zeros((T, hq, d)), np.zeros((T, hq, d)), 0
+    for b, n in enumerate(news):
+        cache.write(rng, b, np.arange(n), BF16)
+        k, v = (np.concatenate([p, cache.read(c, b, np.arange(n))]) for p, c in ((pk, cache.k), (pv, cache.v)))
+        seen = np.concatenate([np.ones((n, prefix), bool), seen_by(np.arange(n), n, 0, 0)], 1)
+        want[at : at + n], mag[at : at + n] = attention_reference(f64(q[at : at + n]), k, v, seen, 1 / math.sqrt(d), hkv)
+        at += n
+    one = all(n == 1 for n in news)
+    got = nk.prefix_attention(q, cache.k, cache.v, ints(pages), prefix, cache.device_table(), ints(news),
+                              q_start=None if one else ints(starts(news)))
+    check_attention(got, want, mag, BF16)
+
+
 def test_prefix_alone():
     """Sequences that have nothing of their own yet see the prefix."""
     rng = np.random.default_rng(10)
