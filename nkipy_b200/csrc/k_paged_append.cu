@@ -4,8 +4,8 @@
 // for the two halves (lo, hi) of the first rot_dim dimensions at position p,
 // in fp32, rounded once to the stored type.  Each row is read and written once, so
 // the bound is HBM.  Measured (GPU time): 8192 tokens of 32 + 2 * 8 rows of 128 bf16,
-// 202 MB, 47.3 us or 4.3 TB/s, where a plain copy would take 31 us; 1500 tokens of
-// 12 + 2 * 4 rows of 64 fp16 6.9 us, 8 tokens 2.4 us, which is the launch.
+// 202 MB, 40.3 us or 5.0 TB/s, where a plain copy would take 31 us; 1500 tokens of
+// 12 + 2 * 4 rows of 64 fp16 4.4 us, 8 tokens 2.2 us, which is the launch.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -111,16 +111,17 @@ struct Eight {
 // neighbouring pieces of the rest), one pair per thread and step.  Each byte is
 // moved once; a block takes one token, so its place is looked up once, while
 // the first rows are already on their way.  What a block waits for is the chain from
-// its sequence over the length to the page; four blocks to an SM hide it in part.
-// Two rows on the way per thread took as long (47.5 us for the 8192 tokens), two to
-// eight tokens per block 51 to 56 us (fewer blocks fit), streaming loads and stores
-// 46 to 50 us, and the stored rows would be gone from L2 when attention reads them.
+// its sequence over the length to the page, hidden by the other blocks of the SM:
+// the more fit, the better.  With 256 threads for every token, some of them without
+// a row, the 8192 tokens took 47.5 us and the 1500 6.9; so, two rows on the way per
+// thread took as long, two to eight tokens per block 51 to 56 us, streaming loads and
+// stores 46 to 50, and the stored rows would be gone from L2 when attention reads them.
 template <class T, class C, class R>
 __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__ Args a, int pieces, int unit) {
   __shared__ int found;
   const int t = blockIdx.x, half = (int)a.rot_dim / 2, D = (int)a.head_dim;
   const int hq = a.q_out ? (int)a.q_heads : 0, hkv = (int)a.kv_heads, rows = hq + 2 * hkv;
-  const int step = THREADS / unit, c = threadIdx.x % unit, h0 = threadIdx.x / unit + blockIdx.y * step;
+  const int step = blockDim.x / unit, c = threadIdx.x % unit, h0 = threadIdx.x / unit + blockIdx.y * step;
   const bool live = c < pieces && h0 < rows;
   const bool turns = c * 8 < half;
   // the pair's elements: d0 .. d0 + 7 and d1 .. d1 + 7 (none past the row's end)
@@ -241,14 +242,17 @@ int run(const Args &a, cudaStream_t st, int device) {
   const int pieces = (int)(a.rot_dim / 16 + (a.head_dim - a.rot_dim + 15) / 16);
   int unit = 1;
   while (unit < pieces) unit *= 2;
-  // a few tokens spread their rows over more blocks
-  const int rows = (int)((a.q_out ? a.q_heads : 0) + 2 * a.kv_heads), step = THREADS / unit;
+  // a few tokens spread their rows over more blocks, of a warp at least; no more
+  // threads than a block's rows need, in as many steps as a full block would take
+  const int64_t rows = (a.q_out ? a.q_heads : 0) + 2 * a.kv_heads;
   const int64_t want = (2 * num_sms(device) + a.tokens - 1) / a.tokens;
-  const unsigned split = (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + step - 1) / step, want));
+  const int64_t split = std::max<int64_t>(1, std::min<int64_t>((rows * unit + 31) / 32, want));
+  const int64_t per = (rows + split - 1) / split, steps = (per * unit + THREADS - 1) / THREADS;
+  const unsigned threads = (unsigned)(((per + steps - 1) / steps * unit + 31) / 32 * 32);
   paged::with_dtype(a.dtype, [&](auto t) {
     return paged::with_dtype(a.cache_dtype, [&](auto c) {
       return paged::with_dtype(a.rot_dim ? a.rope_dtype : NKB_F32, [&](auto r) {
-        append_kernel<decltype(t), decltype(c), decltype(r)><<<dim3((unsigned)a.tokens, split), THREADS, 0, st>>>(a, pieces, unit);
+        append_kernel<decltype(t), decltype(c), decltype(r)><<<dim3((unsigned)a.tokens, (unsigned)split), threads, 0, st>>>(a, pieces, unit);
         return 0;
       });
     });

@@ -18,10 +18,20 @@ namespace pattn {
 namespace {
 
 constexpr int THREADS = single::THREADS;
+// Rows per SM up to which a block takes one.  28 tokens of 5 heads 36 us, shared 19;
+// 56 of 8 28 and 25; 63 of 28 24 and 31, 64 of 32 56 and 63: more blocks, each with
+// its start, cost more than the shorter chain of reads gives.
+constexpr int FEW = 4;
 
+// A group of DP / 4 threads reads a row's partials, four outputs a thread.  With few
+// tokens all groups of the block share one row's partials (`share`), and a block has
+// one query head; else each group has a query head of its own.
 template <class T, int DP>
 __global__ void __launch_bounds__(THREADS)
-    prefix_join_kernel(const __grid_constant__ several::Params p, const __grid_constant__ single::Params s) {
+    prefix_join_kernel(const __grid_constant__ several::Params p, const __grid_constant__ single::Params s, int share) {
+  constexpr int LANES = DP / 4, GROUPS = THREADS / LANES;
+  __shared__ float4 s_x[THREADS];
+  __shared__ float2 s_ml[THREADS];
   using S = single::Shape<DP>;
   constexpr int SLOT = several::slot_floats(DP), ML = 2 * several::BM * DP;
   const Args &a = p.a;
@@ -55,31 +65,42 @@ __global__ void __launch_bounds__(THREADS)
     const int unit = hk * s.groups + g / single::ROWS, nb = single::blocks_of<S::BK>(a, t);
     return parts_of(Split(at.total * heads, s.ctas), at.before * heads + (int64_t)unit * nb, nb, s.ctas, (int64_t)t * heads + unit);
   };
+  const int group = threadIdx.x / LANES, d = threadIdx.x % LANES * 4, sub = group % share;
+  const int g0 = blockIdx.z * (GROUPS / share) + group / share, step = gridDim.z * (GROUPS / share);
   if (!p.own) {
-    own = own_parts(min((int)threadIdx.x / (DP / 4), G - 1));
+    own = own_parts(min(g0, G - 1));
     pdl_wait();
   }
-  for (int i = threadIdx.x; i < G * (DP / 4); i += THREADS) {
-    const int g = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (!p.own && i >= THREADS) own = own_parts(g);
+  for (int g = g0; g < G; g += step) {  // (with share > 1 the same in all threads)
+    if (!p.own && g != g0) own = own_parts(g);
     auto tile_part = [&](const Parts &x, int j, int tok) {
       const float *slot = p.ws + (int64_t)x.slot(j) * SLOT;
       const int row = tok / p.P * several::BM + tok % p.P * G + g;
       return Partial{slot + row * DP + d, slot + ML + 2 * row};
     };
-    if (d >= D) continue;
     Joined<8> x;
     if (seq != -2) {  // (a token of no sequence sees nothing)
-      x.add(pre.n, [&](int j) { return tile_part(pre, j, ptok); });
-      if (p.own) x.add(own.n, [&](int j) { return tile_part(own, j, otok); });
+      auto mine = [&](int n) { return (n - sub + share - 1) / share; };
+      x.add(mine(pre.n), [&](int j) { return tile_part(pre, sub + j * share, ptok); });
+      if (p.own) x.add(mine(own.n), [&](int j) { return tile_part(own, sub + j * share, otok); });
       else
-        x.add(own.n, [&](int j) {
-          const float *slot = s.ws + (int64_t)own.slot(j) * S::SLOT;
+        x.add(mine(own.n), [&](int j) {
+          const float *slot = s.ws + (int64_t)own.slot(sub + j * share) * S::SLOT;
           const int row = g % single::ROWS;
           return Partial{slot + row * DP + d, slot + single::ROWS * DP + 2 * row};
         });
     }
-    x.store(static_cast<T *>(a.out) + t * a.out_token + (hk * G + g) * a.out_head + d);
+    if (share > 1) {
+      __syncthreads();  // the row before is read
+      s_x[threadIdx.x] = make_float4(x.x[0], x.x[1], x.x[2], x.x[3]);
+      s_ml[threadIdx.x] = make_float2(x.m, x.l);
+      __syncthreads();
+      if (sub) continue;
+      Joined<8> all;
+      all.add_from(share, [&](int j) { return s_ml[threadIdx.x + j * LANES]; }, [&](int j) { return s_x[threadIdx.x + j * LANES]; });
+      x = all;
+    }
+    if (d < D) x.store(static_cast<T *>(a.out) + t * a.out_token + (hk * G + g) * a.out_head + d);
   }
 }
 
@@ -101,9 +122,12 @@ int prefix_run(const Args &a, cudaStream_t st, int device) {
   if (int e = tile_launch(p, st, device)) return e;
   if (!own)
     if (int e = decode_launch(s, st, device, true)) return e;
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.kv_heads);
-  auto join = [&](auto kernel) { return launch_pdl(true, kernel, grid, dim3(THREADS), 0, st, p, s); };
   const bool bf16 = a.dtype == NKB_BF16, small = a.head_dim <= 64;
+  const int64_t G = a.q_heads / a.kv_heads;
+  const bool shared = a.tokens * a.kv_heads * G <= FEW * num_sms(device);
+  const dim3 grid((unsigned)a.tokens, (unsigned)a.kv_heads, shared ? (unsigned)G : 1);
+  const int share = shared ? THREADS / (small ? 16 : 32) : 1;
+  auto join = [&](auto kernel) { return launch_pdl(true, kernel, grid, dim3(THREADS), 0, st, p, s, share); };
   NKB_CUDA_TRY(bf16 ? (small ? join(prefix_join_kernel<__nv_bfloat16, 64>) : join(prefix_join_kernel<__nv_bfloat16, 128>))
                     : (small ? join(prefix_join_kernel<__half, 64>) : join(prefix_join_kernel<__half, 128>)));
   return launch_status("paged prefix join");

@@ -96,6 +96,12 @@ struct Joined {
   float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
   template <class At>
   __device__ __forceinline__ void add(int n, At at) {
+    add_from(
+        n, [&](int j) { return __ldcg(reinterpret_cast<const float2 *>(at(j).ml)); },
+        [&](int j) { return __ldcg(reinterpret_cast<const float4 *>(at(j).o)); });
+  }
+  template <class Ml, class Out>
+  __device__ __forceinline__ void add_from(int n, Ml ml_at, Out o_at) {
     for (int j0 = 0; j0 < n; j0 += U) {
       float2 ml[U];
       float4 y[U];
@@ -104,9 +110,8 @@ struct Joined {
         ml[j] = make_float2(-INFINITY, 0.f);
         y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (j0 + j >= n) continue;
-        const Partial q = at(j0 + j);
-        ml[j] = __ldcg(reinterpret_cast<const float2 *>(q.ml));
-        y[j] = __ldcg(reinterpret_cast<const float4 *>(q.o));
+        ml[j] = ml_at(j0 + j);
+        y[j] = o_at(j0 + j);
       }
       float top = m;
 #pragma unroll
