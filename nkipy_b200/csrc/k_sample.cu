@@ -22,10 +22,10 @@
 //           linear in (max - x) / temperature, summed over the cluster (again
 //           within the threshold's bin if that holds too many); the elements of
 //           the threshold's bin go to every CTA, which narrows them down and sorts
-//           the last few: five (more for both); 21 and 151 us for p = 0.95
+//           the last few: five (more for both); 20 and 145 us for p = 0.95
 //   none    the kept weight of each warp, whose part of the row is contiguous; the
 //           warp in which the running sum passes u times the total walks its part:
-//           two; 6 and 50 us
+//           two; 6 and 47 us
 // Where that does not do (thousands of equal logits at a threshold) the threshold
 // is found bit by bit over the cluster.
 
@@ -403,7 +403,7 @@ __device__ __noinline__ u64 find_slowly(Shared &s, const Slice<T> &x, const Row 
 }
 
 template <class T, int C>
-__global__ void __launch_bounds__(NT, 3) cluster_kernel(const __grid_constant__ Args a, int slice) {
+__global__ void __launch_bounds__(NT, 2) cluster_kernel(const __grid_constant__ Args a, int slice) {
   using X = Slice<T>;
   constexpr int VEC = X::VEC;
   extern __shared__ __align__(16) uint8_t smem[];
