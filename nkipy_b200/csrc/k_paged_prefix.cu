@@ -7,7 +7,7 @@
 // Each sequence's own keys take the form for single tokens or for several, and
 // both leave partials (max, sum, unnormalised output) that the kernel here
 // joins per token and head.  Measured (32 / 8 heads of 128 bf16, GPU time): 64
-// sequences with some hundred keys each after a prefix of 8192, 47 us (the floor is
+// sequences with some hundred keys each after a prefix of 8192, 44 us (the floor is
 // 14 us of reads; prefix 22, own keys 19 and join 12 us one by one, each in part
 // under the next: few blocks per CTA, so each is mostly its start and its partials);
 // 4 sequences after a prefix of 1000, 15.5 us.
@@ -118,6 +118,11 @@ int prefix_run(const Args &a, cudaStream_t st, int device) {
   several::Params p;
   single::Params s = {};
   tile_params(a, device, a.workspace, own, true, true, &p);
+  // Where the sequences' own keys have a kernel of their own, it begins on the SMs
+  // that the prefix leaves it, and fewer CTAs write fewer partials: 64 sequences after
+  // 8192 tokens take 47 us with the prefix on all SMs, 44 on two thirds, 46 on half,
+  // 128 after 2000 40, 38 and 38.
+  if (!own) p.max_ctas = max(1, p.max_ctas * 2 / 3);
   decode_params(a, device, static_cast<char *>(a.workspace) + up(tile_workspace(a, device, own, true, true)), true, &s);
   if (int e = tile_launch(p, st, device)) return e;
   if (!own)
