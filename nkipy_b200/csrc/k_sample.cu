@@ -94,7 +94,10 @@ __device__ __forceinline__ u64 place(float u, u64 total) { return u >= 1.f ? tot
 constexpr int NT = 256, NW = NT / 32, MAX_C = 8;
 constexpr int CAP = 2048;         // elements that a CTA lists
 constexpr int FEW = 256;          // elements that are sorted one a thread
-constexpr int FAST_K = 128;       // top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit
+// Top-k that one CTA sorts: some 2 k to 3 k candidates are expected, CAP fit.  Sorted
+// and by histogram, us, with top-p 0.9 behind it: k = 200, 1 row of 32000 16 / 20, 128
+// of 151936 48 / 108; k = 256 17 / 22 and 54 / 110 (without top-p 17 / 16 and 54 / 94).
+constexpr int FAST_K = 256;
 constexpr int MAX_SLICE = 65528;  // elements per CTA: their low halves' sum stays in 32 bits
 constexpr int BINS = 512, QN = BINS * BINS;  // bins, and the finest ones, linear in (max - x) / temperature
 constexpr float SPAN = 22.25f;    // e^-SPAN < 2^-32
@@ -266,7 +269,7 @@ __device__ __noinline__ void sort_down_few(u64 *shared, u64 &v, int n) {
 // The rest of a row whose n candidates (rank words in s.list) hold its k largest
 // elements, by one CTA.
 __device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, int n, int k, float p, uint32_t key_pmin) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   if (n <= FEW) {
     u64 v = tid < n ? s.list[tid] : 0;
     sort_down_few(s.few, v, n);
@@ -277,42 +280,26 @@ __device__ void draw_sorted(Shared &s, const Args &a, int64_t r, const Row &f, i
     sort_down(s.list, n);
   }
   const int m = min(k, n);
-  static_assert(FAST_K <= 128, "four warps hold the k largest");
-  u64 w = 0, sum = 0;
+  static_assert(FAST_K <= NT, "one of the k largest a thread");
   uint32_t key = 0;
-  if (tid < 128) {
-    if (tid < m) {
-      key = (uint32_t)(s.list[tid] >> IDX_BITS);
-      w = Row::w(f.e(of_key(key)));
-    }
-    sum = w;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += y;
-    }
-    if (lane == 31) s.red[warp] = sum;
+  u64 w = 0, W;
+  if (tid < m) {
+    key = (uint32_t)(s.list[tid] >> IDX_BITS);
+    w = Row::w(f.e(of_key(key)));
   }
+  const u64 before = scan(s, w, &W), T = p < 1.f ? share_of(p, W) : ~0ull;
+  s.weights[tid] = tid < m && before < T && key >= key_pmin ? w : 0;
   __syncthreads();
-  if (tid < 128) {
-    for (int i = 0; i < warp; ++i) sum += s.red[i];
-    const u64 W = s.red[0] + s.red[1] + s.red[2] + s.red[3];
-    const u64 T = p < 1.f ? share_of(p, W) : ~0ull;
-    const bool keep = tid < m && sum - w < T && key >= key_pmin;
-    s.weights[tid] = keep ? w : 0;
+  if (tid >= m) return;
+  const u64 own = s.weights[tid], index = s.list[tid] & (MAX_VOCAB - 1);
+  u64 total = 0, upto = 0;  // of all, and of those up to this one in index order
+  for (int i = 0; i < m; ++i) {
+    const u64 x = s.weights[i];
+    total += x;
+    if ((s.list[i] & (MAX_VOCAB - 1)) >= index) upto += x;
   }
-  __syncthreads();
-  if (tid < 128) {
-    const u64 own = s.weights[tid];
-    u64 total = 0, upto = 0;  // of all, and of those up to this one in index order
-    for (int i = 0; i < m; ++i) {
-      const u64 x = s.weights[i];
-      total += x;
-      if (tid < m && (s.list[i] & (MAX_VOCAB - 1)) >= (s.list[tid] & (MAX_VOCAB - 1))) upto += x;
-    }
-    const u64 at = place(a.u[r], total);
-    if (own && upto > at && upto - own <= at) a.tokens[r] = (int)(MAX_VOCAB - 1 - (s.list[tid] & (MAX_VOCAB - 1)));
-  }
+  const u64 at = place(a.u[r], total);
+  if (own && upto > at && upto - own <= at) a.tokens[r] = (int)(MAX_VOCAB - 1 - index);
 }
 
 template <class T>
