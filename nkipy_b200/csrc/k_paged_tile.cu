@@ -517,13 +517,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Desc dq(smem_desc(smem_u32(smem + t * C::TILE), 16, 1024)), dk(smem_desc(smem_u32(smem + C::OFF_K), 16, 1024)),
           dv(smem_desc(smem_u32(smem + C::OFF_V), HALF, 1024));
       const uint32_t ts = tmem + T_S + t * 128, to = tmem + T_O + t * 128;
-      uint32_t segs = 0, blk = 0, cnt = 0, outs = 0;
+      uint32_t segs = 0, blk = 0, cnt = 0, outs = 0, turns = 0;
       Item x;
       while (ok && take(x)) {
         const int n = __shfl_sync(0xffffffffu, x.n, 0), nb = __shfl_sync(0xffffffffu, t ? x.nb_b : x.nb_a, 0);
+        const bool paired = __shfl_sync(0xffffffffu, x.nb_a > 0 && x.nb_b > 0, 0);
         // tile B begins when the softmax of A has done its first half: in step, both would want the special-function
-        // units at one time and the tensor cores at another.  (A cannot be a segment ahead: Q is shared.)
-        if (t == 1 && !(ok = wait_warp(b_go, segs & 1, abort_flag))) break;
+        // units at one time and the tensor cores at another.  Only where both tiles have a block: A's arrival is then
+        // behind this segment's Q, which is loaded when B has released the Q before, past its last wait here.  Without
+        // a block A would arrive as soon as it has the segment, and twice before B looks: a parity that is the old one.
+        if (paired && t == 1 && !(ok = wait_warp(b_go, turns++ & 1, abort_flag))) break;
         auto stage = [&](int c) { return (blk + c) % ST; };
         auto full = [&](uint64_t *bar, int c) { return wait_warp(&bar[stage(c)], ((blk + c) / ST) & 1, abort_flag); };
         auto qk = [&](int c, int j) {  // S = Q K^T of half j of block c
@@ -694,11 +697,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_ready[2 * t + j]);
-        if (h == 0 && warp == 0 && lane == 0) mbar_arrive(b_go);
+        if (h == 0 && warp == 0 && lane == 0 && x.nb_b > 0) mbar_arrive(b_go);
       }
       if (!ok) break;
       blk += x.n;
-      if (nb == 0 && warp == 0 && lane == 0) mbar_arrive(b_go);
       if (nb > 0) {
         const uint32_t last = ((cnt >> 1) - 1) & 1;
         if (!(ok = wait_warp(&o_done[2 * t], last, abort_flag) && wait_warp(&o_done[2 * t + 1], last, abort_flag))) break;

@@ -1,0 +1,90 @@
+"""Serving calls at the edges of what they take: padding tokens and empty
+sequences among others.  References, bounds and helpers are those of
+``test_gpu_serving``; after each call the device error flag is read."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from nkipy_b200 import runtime as nk  # noqa: E402
+from nkipy_b200.spike import _nkb  # noqa: E402
+from tests.test_gpu_serving import (BF16, F16, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
+                                    randn, seen_by)
+
+pytestmark = pytest.mark.gpu
+
+
+def no_device_error():
+    torch.cuda.synchronize()
+    flag = ctypes.c_int()
+    _nkb.call("nkb_device_error", ctypes.byref(flag))
+    assert flag.value == 0
+
+
+# ---------------------------------------------------------------------------
+# tokens without keys
+# ---------------------------------------------------------------------------
+def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=0):
+    """``front`` and ``behind`` tokens belong to no sequence; a sequence's length may be less than
+    its new tokens, whose first ones then lie before its first key."""
+    rng = np.random.default_rng(seed)
+    n_pages = -(-prefix // page)
+    cache = Paged(rng, lens, hkv, d, page, dtype, extra=n_pages)
+    pages, at_p = cache.free[:n_pages], np.arange(prefix)
+    place = torch.tensor(pages[at_p // page], dtype=torch.long, device="cuda"), torch.tensor(at_p % page, device="cuda")
+    for c in (cache.k, cache.v):
+        if prefix:
+            c[place] = randn(rng, (prefix, hkv, d), dtype)
+    pk, pv = f64(cache.k[place]), f64(cache.v[place])
+    T = front + sum(news) + behind
+    q = randn(rng, (T, hq, d), dtype)
+    want, mag, at = np.zeros((T, hq, d)), np.zeros((T, hq, d)), front
+    for b, (n, length) in enumerate(zip(news, lens)):
+        cache.write(rng, b, np.arange(length), dtype)
+        rows = np.arange(length)
+        k, v = (np.concatenate([x, cache.read(c, b, rows)]) for x, c in ((pk, cache.k), (pv, cache.v)))
+        seen = np.concatenate([np.ones((n, prefix), bool), seen_by(np.arange(length - n, length), length, 0, 0)], 1)
+        if n and seen.shape[1]:
+            want[at : at + n], mag[at : at + n] = attention_reference(f64(q[at : at + n]), k, v, seen, 1 / math.sqrt(d), hkv)
+        at += n
+    start = ints((front + np.cumsum([0] + list(news))).tolist())
+    args = (cache.device_table(), ints(lens))
+    out = torch.full_like(q, 9.0)
+    for _ in range(3):
+        if prefix:
+            got = nk.prefix_attention(q, cache.k, cache.v, ints(pages), prefix, *args, q_start=start, out=out.fill_(9.0))
+        else:
+            got = nk.paged_attention(q, cache.k, cache.v, *args, q_start=start, out=out.fill_(9.0))
+        no_device_error()
+        check_attention(got, want, mag, dtype)
+        assert bool((got[:front] == 0).all()) and bool((got[at:] == 0).all())
+
+
+EMPTY = [0, 0, 3, 0, 130, 0, 0, 17, 0, 0, 0, 0]
+PADDED = [
+    # front, news, lens, behind, hq, hkv, d, page, dtype
+    (0, [448], [4448], 64, 32, 8, 128, 16, BF16),  # a real unit and then empty ones, cut into shares
+    (64, [448], [4448], 0, 32, 8, 64, 16, F16),
+    (0, [1] * 300, [0, 5] * 150, 0, 16, 8, 64, 16, BF16),  # every second sequence is empty
+    (0, [40] * 12, EMPTY, 0, 32, 8, 128, 16, BF16),
+    (33, [20, 1, 300] * 4, EMPTY, 500, 8, 8, 64, 32, F16),
+    (0, [64] * 6, [0] * 6, 0, 32, 8, 128, 16, BF16),  # no key at all
+    (0, [9] * 64, [3, 0] * 32, 0, 32, 8, 128, 16, BF16),
+    (0, [64, 64, 64], [256, 0, 0], 1000, 8, 8, 128, 16, BF16),
+    (5, [200], [12], 5, 16, 2, 64, 8, F16),  # most tokens lie before the first key
+]
+
+
+@pytest.mark.parametrize("case", range(len(PADDED)))
+def test_padding(case):
+    run_padded(700 + case, *PADDED[case])
+
+
+@pytest.mark.parametrize("prefix", [20, 700])
+@pytest.mark.parametrize("case", range(len(PADDED)))
+def test_padding_after_a_prefix(case, prefix):
+    run_padded(800 + case, *PADDED[case], prefix=prefix)
