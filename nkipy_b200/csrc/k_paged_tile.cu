@@ -794,7 +794,9 @@ int log2_of(int64_t x) {
   return (int64_t(1) << s) == x ? s : -1;
 }
 
-// workspace: head | pairs | seq_pairs | partial slots
+// workspace: head | pairs | seq_pairs | partial slots, from its first 32-byte boundary
+// (the partials are written 32 bytes at a time; a caller's alignment is 16)
+constexpr size_t WS_ALIGN = 32, WS_SLACK = WS_ALIGN - 16;
 struct Layout {
   size_t next, pairs, seqs, ws, bytes;
   int max_pairs;
@@ -810,7 +812,7 @@ Layout layout(const Args &a, int max_ctas, bool own, bool prefix, bool keep) {
   x.seqs = x.pairs + up((size_t)x.max_pairs * sizeof(Pair));
   x.ws = x.seqs + up((size_t)(own ? a.seqs + 2 : 0) * 4);
   const size_t slot = (a.head_dim <= 64 ? Cfg<64>::SLOT : Cfg<128>::SLOT) * sizeof(float);
-  x.bytes = x.ws + (2 * (size_t)max_ctas + (keep ? (size_t)x.max_pairs * a.kv_heads : 0)) * slot;
+  x.bytes = x.ws + (2 * (size_t)max_ctas + (keep ? (size_t)x.max_pairs * a.kv_heads : 0)) * slot + WS_SLACK;
   return x;
 }
 
@@ -891,7 +893,7 @@ int tile_params(const Args &a, int device, void *workspace, bool own, bool prefi
   p->max_pairs = x.max_pairs;
   // (more units than CTAs may be handed out one by one, by a counter that the list's kernel sets)
   p->inside = own && x.max_pairs <= LIST && a.seqs <= LIST && x.max_pairs * a.kv_heads <= p->max_ctas;
-  char *w = static_cast<char *>(workspace);
+  char *w = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(workspace) + WS_ALIGN - 1) / WS_ALIGN * WS_ALIGN);
   p->head = reinterpret_cast<int64_t *>(w);
   p->next = reinterpret_cast<int *>(w + x.next);
   p->pairs = reinterpret_cast<Pair *>(w + x.pairs);

@@ -12,6 +12,7 @@ torch = pytest.importorskip("torch")
 
 from nkipy_b200 import runtime as nk  # noqa: E402
 from nkipy_b200.spike import _nkb  # noqa: E402
+from tests.test_serving_cpu import packed  # noqa: E402
 from tests.test_gpu_serving import (BF16, F16, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
                                     randn, seen_by)
 
@@ -88,3 +89,41 @@ def test_padding(case):
 @pytest.mark.parametrize("case", range(len(PADDED)))
 def test_padding_after_a_prefix(case, prefix):
     run_padded(800 + case, *PADDED[case], prefix=prefix)
+
+
+# ---------------------------------------------------------------------------
+# the C call's workspace
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("offset", [0, 16])
+@pytest.mark.parametrize("prefix, news, d", [(0, [200, 3], 128), (0, [200, 3], 64), (300, [30, 2], 64), (300, [1, 1], 128)])
+def test_workspace_at_any_16_byte_boundary(offset, prefix, news, d):
+    """Units cut into partials, with a workspace that starts at an odd multiple of 16 bytes: the torch call's
+    outputs, and nothing written in front of it or behind it."""
+    rng = np.random.default_rng(900)
+    hq, hkv, page, lens, pages = 4, 2, 16, [3000, 40], -(-prefix // 16)
+    cache = Paged(rng, lens, hkv, d, page, BF16, extra=pages, fill=0.0)
+    for b, n in enumerate(lens):
+        cache.write(rng, b, np.arange(n), BF16)
+    q, table, kv_len, ids = randn(rng, (sum(news), hq, d), BF16), cache.device_table(), ints(lens), ints(cache.free[:pages])
+    start = None if max(news) == 1 else ints(np.cumsum([0] + news).tolist())
+    if prefix:
+        want = nk.prefix_attention(q, cache.k, cache.v, ids, prefix, table, kv_len, q_start=start)
+    else:
+        want = nk.paged_attention(q, cache.k, cache.v, table, kv_len, q_start=start)
+    out = torch.zeros_like(q)
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    values = dict(q=at(q), out=at(out), k_cache=at(cache.k), v_cache=at(cache.v), page_table=at(table), kv_len=at(kv_len),
+                  q_start=at(start), prefix_pages=at(ids) if prefix else 0, tokens=sum(news), seqs=2, q_heads=hq, kv_heads=hkv,
+                  head_dim=d, q_token=hq * d, q_head=d, out_token=hq * d, out_head=d, pages=cache.k.shape[0], page_size=page,
+                  table_width=table.shape[1], table_stride=table.shape[1], prefix_len=prefix, scale=1 / math.sqrt(d))
+    for c, x in (("k", cache.k), ("v", cache.v)):
+        values.update({f"{c}_page": x.stride(0), f"{c}_slot": x.stride(1), f"{c}_cache_head": x.stride(2)})
+    need = ctypes.c_size_t()
+    _nkb.call("nkb_paged_attention_workspace", packed("attention", **values), ctypes.byref(need))
+    room = torch.full((need.value + 512,), 77, dtype=torch.uint8, device="cuda")
+    first = (-room.data_ptr()) % 256 + offset
+    values.update(workspace=room.data_ptr() + first, workspace_bytes=need.value)
+    _nkb.call("nkb_paged_attention", packed("attention", **values), torch.cuda.current_stream().cuda_stream)
+    no_device_error()
+    assert torch.equal(out, want)
+    assert bool((room[:first] == 77).all()) and bool((room[first + need.value :] == 77).all())
