@@ -329,8 +329,9 @@ NKB_API int nkb_paged_append(const nkb_paged_append_args *args, void *stream);
  * preceded by the same prefix_len tokens, held by prefix_pages (int32, one id
  * per page) and read once for the batch; page_table and kv_len then describe
  * what follows the prefix, all of the prefix is visible, and window must be 0.
- * Page ids outside the cache read as zero keys and values.  q, out and the
- * caches have one dtype; statistics and sums are fp32.  workspace: a device
+ * Page ids outside the cache read as zero keys and values.  scale is any finite
+ * number (zero and negative ones take a slower form with q_start or a prefix).
+ * q, out and the caches have one dtype; statistics and sums are fp32.  workspace: a device
  * array of nkb_paged_attention_workspace() bytes for this call alone, aligned to
  * 16 bytes (its contents need not be kept or cleared); the bytes depend on the
  * sizes and on whether q_start is given, not on the arrays. */

@@ -92,7 +92,7 @@ def _attend(q, k, v, seen, scale):
 
 
 def _attention_cpu(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, prefix_pages, prefix_len):
-    _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, prefix_pages, prefix_len)
+    _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, prefix_pages, prefix_len)
     scale = 1 / math.sqrt(q.shape[2]) if scale is None else scale
     out = np.zeros_like(q)
     before = np.arange(prefix_len)
@@ -212,12 +212,14 @@ def _check_append(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, s
     _check_tables(page_table, kv_len, q_start, k.shape[0])
 
 
-def _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, prefix_pages, prefix_len):
+def _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, prefix_pages, prefix_len):
     _check_caches(k_cache, v_cache)
     if len(q.shape) != 3 or q.shape[2] != k_cache.shape[3] or q.shape[1] % k_cache.shape[2] or q.dtype != k_cache.dtype:
         _fail(f"q {q.dtype} {tuple(q.shape)} does not go with caches {k_cache.dtype} {tuple(k_cache.shape)}")
     if window < 0 or sinks < 0 or prefix_len < 0:
         _fail("window, sinks and prefix_len must not be negative")
+    if scale is not None and not math.isfinite(scale):
+        _fail("scale must be finite")
     if prefix_len and (prefix_pages is None or len(prefix_pages.shape) != 1
                        or prefix_len > prefix_pages.shape[0] * k_cache.shape[1]):
         _fail(f"prefix of {prefix_len} tokens needs as many page ids as hold them")
@@ -276,7 +278,7 @@ def _paged_append_hlo(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, 
 
 
 def _attention_hlo(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, prefix_pages, prefix_len):
-    _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, prefix_pages, prefix_len)
+    _check_attention(q, k_cache, v_cache, page_table, kv_len, q_start, window, sinks, scale, prefix_pages, prefix_len)
     if prefix_len == 0:
         prefix_pages = None
     names = ["q", "k_cache", "v_cache", "page_table", "kv_len", "q_start", "prefix_pages"]

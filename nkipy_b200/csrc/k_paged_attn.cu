@@ -3,6 +3,9 @@
 //   out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j
 // over the keys j that the token at position p sees (j <= p, and with a window
 // w also j > p - w or j < sinks; all of the prefix).
+#include <cfloat>
+#include <cmath>
+
 #include "paged_attn.cuh"
 
 namespace nkb {
@@ -105,6 +108,7 @@ int check_arrays(const Args &a) {
   if (a.tokens && (!a.q || !a.out || !a.kv_len || (a.table_width && !a.page_table) || (a.pages && (!a.k_cache || !a.v_cache))))
     return bad("NULL array");
   if (a.tokens && a.prefix_len && !a.prefix_pages) return bad("a prefix needs its pages");
+  if (!std::isfinite(a.scale)) return bad("scale must be finite");
   return NKB_OK;
 }
 
@@ -114,6 +118,11 @@ int check_arrays(const Args &a) {
 bool decode_form(const Args &a) {
   return !a.q_start && a.dtype != NKB_F32 && a.head_dim <= 128 && a.seqs * a.q_heads <= INT32_MAX;
 }
+
+// The tiles mask a score before it is scaled, and take the largest score as the
+// largest scaled one: a scale (in their log2 units, fp32) that is zero, negative or
+// subnormal takes the form for any layout, which scales first.
+bool tile_scale(const Args &a) { return (float)(a.scale * LOG2E) >= FLT_MIN; }
 
 // Tokens by q_start: the tensor-core tiles, for page sizes that a block of 128
 // keys is made of.
@@ -140,12 +149,12 @@ int run(const Args &a, int device, cudaStream_t st) {
   if (reinterpret_cast<uintptr_t>(a.workspace) & 15) return fail(NKB_ERR_INVALID, "paged_attention: unaligned workspace");
   if (a.tokens == 0) return NKB_OK;
   if (a.prefix_len) {
-    if (prefix_form(a) && tile_strides(a)) return prefix_run(a, st, device);
+    if (prefix_form(a) && tile_strides(a) && tile_scale(a)) return prefix_run(a, st, device);
   } else if (decode_form(a) && aligned16(a)) {
     single::Params p;
     decode_params(a, device, a.workspace, false, &p);
     return decode_launch(p, st, device, false);
-  } else if (several_form(a) && tile_strides(a)) {
+  } else if (several_form(a) && tile_strides(a) && tile_scale(a)) {
     several::Params p;
     tile_params(a, device, a.workspace, true, false, false, &p);
     return tile_launch(p, st, device);

@@ -382,7 +382,7 @@ size_t decode_workspace(const Args &a, int device, bool keep) {
 int decode_params(const Args &a, int device, void *workspace, bool keep, Params *p) {
   p->a = a;
   p->groups = (int)((a.q_heads / a.kv_heads + ROWS - 1) / ROWS);
-  p->scale_log2 = (float)(a.scale * 1.4426950408889634);
+  p->scale_log2 = (float)(a.scale * LOG2E);
   p->ws = static_cast<float *>(workspace);
   p->ctas = grid_ctas(device);
   p->keep = keep;

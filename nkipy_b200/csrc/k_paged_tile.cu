@@ -887,7 +887,7 @@ int tile_params(const Args &a, int device, void *workspace, bool own, bool prefi
   p->own = own;
   p->prefix = prefix;
   p->keep = keep;
-  p->scale_log2 = (float)(a.scale * 1.4426950408889634);
+  p->scale_log2 = (float)(a.scale * LOG2E);
   p->wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_token % 16 == 0 && a.out_head % 16 == 0;
   const Layout x = layout(a, p->max_ctas, own, prefix, keep);
   p->max_pairs = x.max_pairs;

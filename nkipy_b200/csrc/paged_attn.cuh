@@ -7,6 +7,7 @@ namespace nkb {
 namespace pattn {
 
 using Args = nkb_paged_attention_args;
+constexpr double LOG2E = 1.4426950408889634;
 
 // Keys that the last token of a sequence sees, as one run of n "virtual" keys:
 // the first `ns` are keys 0 .. ns - 1 (the first tokens that stay visible), the

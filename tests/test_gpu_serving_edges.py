@@ -14,7 +14,7 @@ from nkipy_b200 import runtime as nk  # noqa: E402
 from nkipy_b200.spike import _nkb  # noqa: E402
 from tests.test_serving_cpu import packed  # noqa: E402
 from tests.test_gpu_serving import (BF16, F16, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
-                                    randn, seen_by)
+                                    randn, run_attention, seen_by)
 
 pytestmark = pytest.mark.gpu
 
@@ -29,7 +29,7 @@ def no_device_error():
 # ---------------------------------------------------------------------------
 # tokens without keys
 # ---------------------------------------------------------------------------
-def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=0):
+def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=0, scale=None):
     """``front`` and ``behind`` tokens belong to no sequence; a sequence's length may be less than
     its new tokens, whose first ones then lie before its first key."""
     rng = np.random.default_rng(seed)
@@ -50,16 +50,18 @@ def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=
         k, v = (np.concatenate([x, cache.read(c, b, rows)]) for x, c in ((pk, cache.k), (pv, cache.v)))
         seen = np.concatenate([np.ones((n, prefix), bool), seen_by(np.arange(length - n, length), length, 0, 0)], 1)
         if n and seen.shape[1]:
-            want[at : at + n], mag[at : at + n] = attention_reference(f64(q[at : at + n]), k, v, seen, 1 / math.sqrt(d), hkv)
+            want[at : at + n], mag[at : at + n] = attention_reference(f64(q[at : at + n]), k, v, seen,
+                                                                          1 / math.sqrt(d) if scale is None else scale, hkv)
         at += n
     start = ints((front + np.cumsum([0] + list(news))).tolist())
     args = (cache.device_table(), ints(lens))
     out = torch.full_like(q, 9.0)
     for _ in range(3):
         if prefix:
-            got = nk.prefix_attention(q, cache.k, cache.v, ints(pages), prefix, *args, q_start=start, out=out.fill_(9.0))
+            got = nk.prefix_attention(q, cache.k, cache.v, ints(pages), prefix, *args, q_start=start, scale=scale,
+                                      out=out.fill_(9.0))
         else:
-            got = nk.paged_attention(q, cache.k, cache.v, *args, q_start=start, out=out.fill_(9.0))
+            got = nk.paged_attention(q, cache.k, cache.v, *args, q_start=start, scale=scale, out=out.fill_(9.0))
         no_device_error()
         check_attention(got, want, mag, dtype)
         assert bool((got[:front] == 0).all()) and bool((got[at:] == 0).all())
@@ -127,3 +129,31 @@ def test_workspace_at_any_16_byte_boundary(offset, prefix, news, d):
     no_device_error()
     assert torch.equal(out, want)
     assert bool((room[:first] == 77).all()) and bool((room[first + need.value :] == 77).all())
+
+
+# ---------------------------------------------------------------------------
+# scale
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [0.0, -0.125, -1.0, 1e-42, 1e-60, 3.0])
+@pytest.mark.parametrize("news, pasts, dtype, page", [([1, 1], [9, 300], BF16, 16), ([70, 200], [0, 90], BF16, 16),
+                                                      ([70, 3], [5, 900], F16, 64), ([20, 1], [3, 70], BF16, 24)])
+def test_scale_of_any_sign(scale, news, pasts, dtype, page):
+    """Every form: uniform weights for 0 (and for what is as good as 0), the least product first for a negative one."""
+    for q_start in [True] + [False] * (max(news) == 1):
+        run_attention(1000, news, pasts, 0, 0, 4, 2, 64, page, dtype, scale=scale, q_start=q_start)
+        run_attention(1001, news, pasts, 50, 3, 4, 2, 128, page, dtype, scale=scale, q_start=q_start)
+    no_device_error()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.25])
+@pytest.mark.parametrize("news", [[1, 1], [30, 5]])
+def test_scale_of_any_sign_after_a_prefix(scale, news):
+    run_padded(1002, 0, news, [n + 40 for n in news], 0, 4, 2, 64, 16, BF16, prefix=300, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan")])
+def test_scale_that_is_not_finite(scale):
+    rng = np.random.default_rng(1003)
+    cache = Paged(rng, [20], 2, 64, 16, BF16)
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        nk.paged_attention(randn(rng, (1, 4, 64), BF16), cache.k, cache.v, cache.device_table(), ints([20]), scale=scale)
