@@ -218,7 +218,9 @@ int check_args(const Args &a) {
   if (a.rot_dim < 0 || a.rot_dim % 2 || a.rot_dim > a.head_dim) return bad("rot_dim must be even and at most head_dim");
   if (a.rot_dim && (!a.cos || !a.sin || a.rope_rows < 1 || !paged::float_dtype(a.rope_dtype)))
     return bad("rotating needs cos and sin tables of a float type");
-  if (a.q_heads < 0 || a.q_heads > 65535 || (a.q_heads > 0) != (a.q_out != nullptr) || (a.q != nullptr) != (a.q_out != nullptr))
+  // (an array without elements may be NULL, so a call without tokens says nothing by its pointers)
+  if (a.q_heads < 0 || a.q_heads > 65535 ||
+      (a.tokens && ((a.q_heads > 0) != (a.q_out != nullptr) || (a.q != nullptr) != (a.q_out != nullptr))))
     return bad("q, q_out and q_heads go together");
   if (a.tokens && (!a.k || !a.v || !a.kv_len || (a.table_width && !a.page_table) || (a.pages && (!a.k_cache || !a.v_cache))))
     return bad("NULL array");

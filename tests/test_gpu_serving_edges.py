@@ -157,3 +157,19 @@ def test_scale_that_is_not_finite(scale):
     cache = Paged(rng, [20], 2, 64, 16, BF16)
     with pytest.raises(RuntimeError, match="scale must be finite"):
         nk.paged_attention(randn(rng, (1, 4, 64), BF16), cache.k, cache.v, cache.device_table(), ints([20]), scale=scale)
+
+
+# ---------------------------------------------------------------------------
+# calls without tokens
+# ---------------------------------------------------------------------------
+def test_append_of_no_tokens_with_queries():
+    cache = Paged(np.random.default_rng(1100), [20], 2, 64, 16, BF16, fill=3.0)
+    none = lambda heads: torch.zeros((0, heads, 64), dtype=BF16, device="cuda")  # noqa: E731
+    cos = torch.ones((30, 32), device="cuda")
+    table, start = cache.device_table(), ints([0, 0])
+    for rope in (dict(), dict(cos=cos, sin=cos)):
+        got = nk.paged_append(none(2), none(2), cache.k, cache.v, table, ints([20]), q_start=start, q=none(4), **rope)
+        assert got.shape == (0, 4, 64) and got.dtype == BF16
+        got = nk.paged_append(none(2), none(2), cache.k, cache.v, table[:0], ints([]), q=none(4), **rope)
+        assert got.shape == (0, 4, 64)
+    assert bool((cache.k == 3).all())

@@ -19,3 +19,13 @@ def test_scale_that_is_not_finite(scale):
         T.paged_attention(q, kc, vc, table, lens, scale=scale)
     with pytest.raises(ValueError, match="finite"):
         NKIPyKernel.trace(lambda q, kc, vc, t, n: T.paged_attention(q, kc, vc, t, n, scale=scale)).specialize(q, kc, vc, table, lens)
+
+
+def test_append_of_no_tokens_with_queries():
+    """An empty step: arrays without elements have no address."""
+    none = dict(tokens=0, seqs=0, k=0, v=0, q=0, q_out=0, q_heads=4, q_token=256, q_head=64, q_out_token=256, q_out_head=64)
+    lib = _nkb.lib()
+    assert lib.nkb_paged_append(packed("append", **none), None) == 0
+    assert lib.nkb_paged_append(packed("append", **none, cos=16, sin=16, rot_dim=64, rope_rows=4, rope_stride=32), None) == 0
+    assert lib.nkb_paged_append(packed("append", **{**none, "q_heads": -1}), None) == 1
+    assert lib.nkb_paged_append(packed("append", q_heads=4), None) == 1
