@@ -331,6 +331,10 @@ NKB_API int nkb_paged_append(const nkb_paged_append_args *args, void *stream);
  * what follows the prefix, all of the prefix is visible, and window must be 0.
  * Page ids outside the cache read as zero keys and values.  scale is any finite
  * number (zero and negative ones take a slower form with q_start or a prefix).
+ * A score of NaN or +inf makes its row NaN, a key with a score of -inf has no
+ * weight.  What unseen keys hold does not matter, but an infinity or NaN in a
+ * value row may make NaN of other rows of its sequence in the same call that see
+ * some keys and not this one (zero weights meet it in the tensor-core tiles).
  * q, out and the caches have one dtype; statistics and sums are fp32.  workspace: a device
  * array of nkb_paged_attention_workspace() bytes for this call alone, aligned to
  * 16 bytes (its contents need not be kept or cleared); the bytes depend on the

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const __grid_const
     }
 #pragma unroll
     for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-    const float mn = fmaxf(m, x), f = m == -INFINITY ? 0.f : __expf(m - mn), p = mn == -INFINITY ? 0.f : __expf(x - mn);
+    const float mn = fmaxf(m, x), base = base_of(mn), f = __expf(m - base), p = __expf(x - base);
     m = mn;
     l = l * f + p;
 #pragma unroll
@@ -78,11 +78,12 @@ __global__ void __launch_bounds__(WARPS * 32) attn_any_kernel(const __grid_const
   __syncthreads();
   float M = -INFINITY, L = 0.f;
   for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w]);
-  for (int w = 0; w < WARPS; ++w) L += s_m[w] == -INFINITY ? 0.f : s_l[w] * __expf(s_m[w] - M);
+  const float base = base_of(M);
+  for (int w = 0; w < WARPS; ++w) L += s_l[w] == 0.f ? 0.f : s_l[w] * __expf(s_m[w] - base);
   for (int d = threadIdx.x; d < D; d += WARPS * 32) {
     float x = 0.f;
-    for (int w = 0; w < WARPS; ++w) x += s_m[w] == -INFINITY ? 0.f : s_o[w][d] * __expf(s_m[w] - M);
-    static_cast<T *>(a.out)[t * a.out_token + h * a.out_head + d] = paged::from_f32<T>(L > 0.f ? x / L : 0.f);
+    for (int w = 0; w < WARPS; ++w) x += s_l[w] == 0.f ? 0.f : s_o[w][d] * __expf(s_m[w] - base);
+    static_cast<T *>(a.out)[t * a.out_token + h * a.out_head + d] = paged::from_f32<T>(L == 0.f ? 0.f : x / L);
   }
 }
 

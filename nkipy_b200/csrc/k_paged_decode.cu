@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
       mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      base[i] = mx[i] == -INFINITY ? 0.f : mx[i];  // a warp whose keys are all masked so far
+      base[i] = base_of(mx[i]);
       alpha[i] = ex2(m[i] - base[i]);
       m[i] = mx[i];
     }
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(const __grid_constan
         x[3] += y.w * g;
       }
       if (whole) {
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = inverse(L);
         if (d < D)
           *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + now.b * a.out_token + (hk * G + g0 + r) * a.out_head + d) =
               make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));

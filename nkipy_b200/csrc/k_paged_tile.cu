@@ -38,6 +38,8 @@
 // keys seen (tensor pipe busy 44 %, issue slots 44 %); 500 tokens over 16400 keys,
 // 32 / 4 heads of 64 fp16, 132 us with 14 of them in the join, 501 TFLOP/s (tensor
 // 30 %, exponential unit 38 %, issue 52 %).
+#include <math_constants.h>
+
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 
@@ -278,9 +280,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// the largest of three, NaN if one is NaN
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -643,9 +646,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mx4[i] = max3(mx4[i], __uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1]));
-        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        mx = mx == -INFINITY ? -INFINITY : mx * p.scale_log2;
-        const bool raise = mx > m + RESCALE;
+        // a score that is NaN or +inf makes the maximum NaN, and so all of the row: the polynomials would take it for 2^-126
+        float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * p.scale_log2;
+        mx = mx == INFINITY ? CUDART_NAN_F : mx;
+        const bool raise = !(mx <= m + RESCALE);
         if (__any_sync(0xffffffffu, raise)) {
           const float m_new = raise ? mx : m;
           const float alpha = m == -INFINITY ? 0.f : raise ? ex2(m - m_new) : 1.f;
@@ -666,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           l *= alpha;
           m = m_new;
         }
-        const float mm = m == -INFINITY ? 0.f : m;
+        const float mm = base_of(m);
         const uint64_t base2 = pair2(-mm, -mm);
         uint64_t l2[2] = {0, 0};
         // of every eight pairs, `POLY` on the FMA pipe: the special-function unit alone would take 64 x 8 cycles a warp
@@ -686,7 +690,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             v[e / 2] = pack<T>(e0, e1);
           }
         };
-        if (masked) exps(std::false_type{});  // masked scores have to become zeros exactly
+        // masked scores, and rows whose scores are all -inf, have to become zeros exactly
+        if (masked || __any_sync(0xffffffffu, m == -INFINITY)) exps(std::false_type{});
         else exps(std::true_type{});
         tmem_st16(sc, v);
         tmem_st16(sc + 16, v + 16);
@@ -717,9 +722,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_arrive(&o_free[t]);  // the next segment's products may go on
       }
       if (!row_ok) continue;
+      if (l == 0.f) {  // saw nothing: zeros, where its zero weights have met an infinity or NaN that others see
+#pragma unroll
+        for (int i = 0; i < DP; ++i) o[i] = 0;
+      }
       const int D = (int)a.head_dim;
       if (x.final) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = inverse(l);
         T *dst = static_cast<T *>(a.out) + (x.tok0 + tok) * a.out_token + (x.hk * p.G + g) * a.out_head;
 #pragma unroll
         for (int i = 0; i < DP; i += 16) {

@@ -91,6 +91,13 @@ __device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t *>(&h);
 }
 
+// Running maxima may pass over NaN, which is then in the sum: a part with a maximum of -inf
+// has seen nothing (its sum and outputs are 0) or nothing but NaN (its sum is NaN).
+// `top` as the base of exponentials: 0 where nothing has been seen.
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
+// 1 / sum; 0 for a row that sees nothing, NaN for NaN
+__device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : l; }
+
 // Four outputs of a row, joined from partials that are read U at a time.
 template <int U>
 struct Joined {
@@ -117,7 +124,11 @@ struct Joined {
       float top = m;
 #pragma unroll
       for (int j = 0; j < U; ++j) top = fmaxf(top, ml[j].x);
-      if (top == -INFINITY) continue;  // nothing seen so far
+      if (top == -INFINITY) {  // nothing seen so far, or NaN
+#pragma unroll
+        for (int j = 0; j < U; ++j) l += ml[j].y;
+        continue;
+      }
       const float f = ex2(m - top);
       l *= f;
 #pragma unroll
@@ -125,7 +136,6 @@ struct Joined {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const float g = ex2(ml[j].x - top);
-        if (g == 0.f) continue;  // a part that saw nothing has nothing written for it to scale
         l += ml[j].y * g;
         x[0] += y[j].x * g;
         x[1] += y[j].y * g;
@@ -137,7 +147,7 @@ struct Joined {
   }
   template <class T>
   __device__ __forceinline__ void store(T *p) const {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = inverse(l);
     *reinterpret_cast<uint2 *>(p) = make_uint2(pack<T>(x[0] * inv, x[1] * inv), pack<T>(x[2] * inv, x[3] * inv));
   }
 };

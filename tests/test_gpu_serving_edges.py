@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 from nkipy_b200 import runtime as nk  # noqa: E402
 from nkipy_b200.spike import _nkb  # noqa: E402
 from tests.test_serving_cpu import packed  # noqa: E402
-from tests.test_gpu_serving import (BF16, F16, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
+from tests.test_gpu_serving import (BF16, F16, F32, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
                                     randn, run_attention, seen_by)
 
 pytestmark = pytest.mark.gpu
@@ -173,3 +173,146 @@ def test_append_of_no_tokens_with_queries():
         got = nk.paged_append(none(2), none(2), cache.k, cache.v, table[:0], ints([]), q=none(4), **rope)
         assert got.shape == (0, 4, 64)
     assert bool((cache.k == 3).all())
+
+
+# ---------------------------------------------------------------------------
+# NaN and infinities in what a token sees
+# ---------------------------------------------------------------------------
+INF, NAN = float("inf"), float("nan")
+SEEN = [
+    # news, pasts, hq, hkv, d, page, dtype, prefix
+    ([1, 1, 1], [699, 2, 1299], 8, 2, 128, 16, BF16, 0),  # single tokens, cut
+    ([1] * 200, [99] * 200, 16, 8, 64, 16, F16, 0),  # and some whole
+    ([70, 3], [300, 900], 6, 2, 64, 32, F16, 0),  # tiles, cut
+    ([130, 3], [300, 900], 8, 2, 128, 16, BF16, 0),
+    ([3, 130], [900, 300], 8, 2, 128, 16, BF16, 0),
+    ([7] * 40, range(140, 180), 16, 8, 128, 16, BF16, 0),  # tiles, whole
+    ([31, 9], [2, 260], 4, 2, 20, 5, F32, 0),  # any layout
+    ([1, 1], [2, 260], 4, 2, 64, 48, BF16, 0),
+    ([1] * 3, [3, 0, 200], 8, 2, 128, 16, BF16, 700),  # a prefix
+    ([5, 40], [3, 200], 8, 2, 64, 16, F16, 300),
+    ([3], [20], 4, 2, 20, 5, F32, 40),
+]
+
+
+class Seen:
+    """A call of one of the forms above: ``run`` repeats it with the present contents."""
+
+    def __init__(self, case, seed):
+        news, pasts, self.hq, self.hkv, d, page, dtype, prefix = SEEN[case]
+        self.news, self.pasts, self.d, self.dtype, self.prefix = list(news), list(pasts), d, dtype, prefix
+        self.rng = rng = np.random.default_rng(seed)
+        self.lens = [a + b for a, b in zip(self.news, self.pasts)]
+        pages = -(-prefix // page)
+        self.cache = cache = Paged(rng, self.lens, self.hkv, d, page, dtype, extra=pages)
+        for b, n in enumerate(self.lens):
+            cache.write(rng, b, np.arange(n), dtype)
+        at = np.arange(prefix)
+        self.before = cache.free[:pages]
+        self.where_before = (torch.tensor(self.before[at // page], dtype=torch.long, device="cuda"),
+                             torch.tensor(at % page, device="cuda"))
+        for c in (cache.k, cache.v):
+            if prefix:
+                c[self.where_before] = randn(rng, (prefix, self.hkv, d), dtype)
+        self.first = np.cumsum([0] + self.news)
+        self.q = randn(rng, (self.first[-1], self.hq, d), dtype)
+
+    def run(self):
+        start = None if max(self.news) == 1 else ints(self.first.tolist())
+        args = (self.cache.device_table(), ints(self.lens))
+        if self.prefix:
+            out = nk.prefix_attention(self.q, self.cache.k, self.cache.v, ints(self.before), self.prefix, *args, q_start=start)
+        else:
+            out = nk.paged_attention(self.q, self.cache.k, self.cache.v, *args, q_start=start)
+        no_device_error()
+        return out
+
+    def keys(self, b, j):
+        """Where key j of sequence b lies, the shared ones first."""
+        if j < self.prefix:
+            return self.where_before[0][j], self.where_before[1][j]
+        pages, slots = self.cache.where(b, [j - self.prefix])
+        return pages[0], slots[0]
+
+
+@pytest.mark.parametrize("case", range(len(SEEN)))
+def test_a_query_that_is_nan(case):
+    """Its row is NaN, whether its unit is cut or not, and no other changes."""
+    x = Seen(case, 1200)
+    plain = x.run()
+    T = x.q.shape[0]
+    for t, h in {(0, 0), (T - 1, x.hq - 1), (T // 2, x.hq // 2)}:
+        kept = x.q[t, h].clone()
+        x.q[t, h, 0] = NAN
+        got = x.run()
+        assert bool(got[t, h].isnan().all()), (t, h)
+        got[t, h] = plain[t, h]
+        assert torch.equal(got, plain)
+        x.q[t, h] = kept
+
+
+@pytest.mark.parametrize("case", range(len(SEEN)))
+def test_a_key_that_is_nan_or_infinite(case):
+    """Whatever its place in a block of keys: the rows that see it are NaN, the others as without it."""
+    x = Seen(case, 1300)
+    for value in (NAN, INF):
+        x.q[..., 0] = x.q[..., 0].abs() + 0.5  # +inf in a key's first dimension is a score of +inf
+        plain = x.run()
+        b = len(x.news) - 1
+        n = x.prefix + x.lens[b]
+        rows = slice(int(x.first[b]), int(x.first[b + 1]))
+        for j in sorted({*range(max(0, n // 3), n // 3 + 9), 0, n - 1}):
+            at = x.keys(b, j)
+            kept = x.cache.k[at].clone()
+            x.cache.k[at[0], at[1], :, 0] = value
+            got = x.run()
+            x.cache.k[at] = kept
+            sees = torch.zeros(len(plain), dtype=torch.bool, device="cuda")
+            if j < x.prefix:
+                sees[:] = True
+            else:
+                sees[rows] = torch.arange(x.pasts[b], x.lens[b], device="cuda") >= j - x.prefix
+            assert bool(got[sees].isnan().all()), (j, value)
+            assert torch.equal(got[~sees], plain[~sees])
+
+
+@pytest.mark.parametrize("case", range(len(SEEN)))
+def test_scores_of_minus_infinity(case):
+    """A key with such a score has no weight; a row that has only such scores is zero."""
+    x = Seen(case, 1400)
+    x.q[..., 0] = -(x.q[..., 0].abs() + 0.5)
+    b = len(x.news) - 1
+    n = x.prefix + x.lens[b]
+    gone = [j for j in range(0, n - x.news[b], 3)]
+    for j in gone:
+        at = x.keys(b, j)
+        x.cache.k[at[0], at[1], :, 0] = INF
+    got = x.run()
+    rows = slice(int(x.first[b]), int(x.first[b + 1]))
+    seen = seen_by(np.arange(x.prefix + x.pasts[b], n), n, 0, 0)
+    seen[:, gone] = False
+    at = [x.keys(b, j) for j in range(n)]
+    pages, slots = (torch.stack([a[i] for a in at]) for i in (0, 1))
+    k, v = f64(x.cache.k[pages, slots]), f64(x.cache.v[pages, slots])
+    want, mag = attention_reference(f64(x.q[rows]), k, v, seen, 1 / math.sqrt(x.d), x.hkv)
+    check_attention(got[rows], want, mag, x.dtype)
+    for j in range(n):
+        at = x.keys(b, j)
+        x.cache.k[at[0], at[1], :, 0] = INF
+    assert bool((x.run()[rows] == 0).all())
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+@pytest.mark.parametrize("dtype, d, page", [(BF16, 128, 16), (F16, 64, 16), (F32, 20, 5)])
+def test_rows_that_see_nothing_beside_values_that_are_not_finite(dtype, d, page, value):
+    rng = np.random.default_rng(1500)
+    cache = Paged(rng, [12, 30], 2, d, page, dtype)
+    for b, n in enumerate([12, 30]):
+        cache.write(rng, b, np.arange(n), dtype)
+    pages, slots = cache.where(0, [3])
+    cache.v[pages[0], slots[0]] = value
+    q = randn(rng, (60, 4, d), dtype)
+    got = nk.paged_attention(q, cache.k, cache.v, cache.device_table(), ints([12, 30]), q_start=ints([0, 40, 50]))
+    no_device_error()
+    assert bool((got[:28] == 0).all()) and bool((got[50:] == 0).all())  # before the first key, and of no sequence
+    assert not bool(got[31:40].isfinite().any()) and bool(got[40:50].isfinite().all())
