@@ -40,11 +40,13 @@ __global__ void __launch_bounds__(THREADS)
   if (p.own) pdl_wait();  // the pairs are a list of the kernels before
   else at = single::find<S::BK>(a, [&](int64_t, int b, int64_t, int64_t) { return b == t; });
   const several::Walk walk(p, 0);
-  auto unit_parts = [&](int u, int &tok, int &seq) {  // of pair u
+  // of pair u; -2 where the token is not one of its own (a list of starts that go back, which no caller means, is cut
+  // off at the pairs that there is room for)
+  auto unit_parts = [&](int u, int &tok, int &seq) {
     const several::Pair x = walk.list.pair(u);
     const int64_t n = several::blocks_of(p, x).n;
     tok = t - x.tok0;
-    seq = x.seq;
+    seq = tok >= 0 && tok < x.ntok ? x.seq : -2;
     return walk.parts(u, hk, n);
   };
   int ptok, otok = 0, seq = 0;

@@ -316,3 +316,21 @@ def test_rows_that_see_nothing_beside_values_that_are_not_finite(dtype, d, page,
     no_device_error()
     assert bool((got[:28] == 0).all()) and bool((got[50:] == 0).all())  # before the first key, and of no sequence
     assert not bool(got[31:40].isfinite().any()) and bool(got[40:50].isfinite().all())
+
+
+# ---------------------------------------------------------------------------
+# starts that go back
+# ---------------------------------------------------------------------------
+def test_starts_that_go_back_after_a_prefix():
+    """More pairs than the list has room for: the tokens that are not listed are zeros, and nothing is read for them."""
+    rng = np.random.default_rng(1600)
+    T, d, page = 1000, 64, 16
+    cache = Paged(rng, [0, T], 1, d, page, BF16, extra=2)
+    cache.write(rng, 1, np.arange(T), BF16)
+    for c in (cache.k, cache.v):
+        c[torch.tensor(cache.free[:2], dtype=torch.long)] = randn(rng, (2, page, 1, d), BF16)
+    q = randn(rng, (T, 32, d), BF16)
+    got = nk.prefix_attention(q, cache.k, cache.v, ints(cache.free[:2]), 20, cache.device_table(), ints([0, T]),
+                              q_start=ints([500, 0, T]))
+    no_device_error()
+    assert bool(got.isfinite().all()) and bool((got[600:] == 0).all())
