@@ -14,7 +14,8 @@ are int32; the new tokens lie in sequence order; ``kv_len`` counts a
 sequence's cached tokens with the new ones; ``q_start=None`` means one new
 token per sequence.  Lengths and tables are read on the device when the
 kernels run, nothing is synchronised, and every launch goes to the current
-torch stream, so a call can be captured into a CUDA graph.
+torch stream, so a call can be captured into a CUDA graph.  A kernel whose
+bounded wait runs out ends without its results; ``check_device_error`` tells.
 """
 
 import ctypes
@@ -101,3 +102,18 @@ def sample_tokens(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     the order temperature, top-k, top-p, min-p; a temperature of 0 takes the largest
     logit.  A row without a finite logit or +inf gives -1."""
     return _calls().sample_tokens(get_spike_singleton().device, logits, u, temperature, top_k, top_p, min_p, out)
+
+
+def check_device_error():
+    """Wait for the device, and raise ``NkbError`` if a kernel of this process has given up a
+    bounded wait since the last check (its results are then invalid; the device stays usable).
+    The calls above do not look by themselves, as that would synchronise: call this where the
+    host waits anyway, once per step or per some steps."""
+    import torch
+
+    with torch.cuda.device(get_spike_singleton().device):
+        torch.cuda.synchronize()
+        flag = ctypes.c_int()
+        _nkb.call("nkb_device_error", ctypes.byref(flag))
+    if flag.value:
+        raise _nkb.NkbError(7, "a kernel's bounded wait expired; results are invalid")

@@ -20,10 +20,26 @@ pytestmark = pytest.mark.gpu
 
 
 def no_device_error():
+    nk.check_device_error()
+
+
+def test_a_wait_that_runs_out_is_reported():
+    """A counter that nothing advances, with a limit of 2 ms, on a stream of its own: one error, then none."""
+    x, u = torch.zeros((2, 9), device="cuda"), torch.zeros(2, device="cuda")
+    nk.sample_tokens(x, u)
+    nk.check_device_error()
+    counter, limit = torch.zeros(1, dtype=torch.int32, device="cuda"), ctypes.c_uint64()
+    _nkb.call("nkb_get_wait_limit_us", ctypes.byref(limit))
     torch.cuda.synchronize()
-    flag = ctypes.c_int()
-    _nkb.call("nkb_device_error", ctypes.byref(flag))
-    assert flag.value == 0
+    try:
+        _nkb.call("nkb_set_wait_limit_us", 2000)
+        _nkb.call("nkb_wait_probe", counter.data_ptr(), 1, torch.cuda.Stream().cuda_stream)
+        with pytest.raises(_nkb.NkbError, match="bounded wait expired"):
+            nk.check_device_error()
+    finally:
+        _nkb.call("nkb_set_wait_limit_us", limit.value)
+    nk.check_device_error()
+    assert nk.sample_tokens(x, u).tolist() == [0, 0]
 
 
 # ---------------------------------------------------------------------------
