@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -52,6 +53,18 @@ void on_device(int64_t device, std::initializer_list<const Arg *> args) {
   for (const Arg *a : args)
     if (*a && (!(*a)->is_cuda() || (*a)->get_device() != device))
       invalid(c10::str(a->name, ": expected a tensor on cuda:", device, " (this process's device), got one on ", (*a)->device()));
+}
+
+// The calls record nothing for a backward pass: tensors that want one are refused.
+void without_gradient(std::initializer_list<const Arg *> args) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const Arg *a : args)
+    if (*a && (*a)->requires_grad())
+      fail(PyExc_RuntimeError, std::string(a->name) + ": requires a gradient, which this call does not have; call it under torch.no_grad(), or on detached tensors");
+}
+// A tensor that a call has written into: autograd sees that it changed.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 int64_t code_of(const Arg &a) {
@@ -150,6 +163,7 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   const int64_t device = integer(o[0]);
   const Arg k("k", o[1]), v("v", o[2]), kc("k_cache", o[3]), vc("v_cache", o[4]), table("page_table", o[5]), len("kv_len", o[6]),
       q_start("q_start", o[7]), q("q", o[8]), cos("cos", o[9]), sin("sin", o[10]), q_out("q_out", o[12]);
+  without_gradient({&k, &v, &kc, &vc, &q, &cos, &sin, &q_out});
   on_device(device, {&k, &v, &kc, &vc, &table, &len, &q_start, &q, &cos, &sin, &q_out});
   nkb_paged_append_args x = {};
   x.dtype = rows(k, 3);
@@ -195,9 +209,12 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   x.cos = cos.ptr();
   x.sin = sin.ptr();
   issue(nkb_paged_append, x, device);
+  written(*kc);
+  written(*vc);
   if (!q) Py_RETURN_NONE;
-  if (q_out) return Py_NewRef(o[12]);
-  return THPVariable_Wrap(std::move(out));
+  if (!q_out) return THPVariable_Wrap(std::move(out));
+  written(out);
+  return Py_NewRef(o[12]);
   END_HANDLE_TH_ERRORS
 }
 
@@ -208,6 +225,7 @@ PyObject *attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   const int64_t device = integer(o[0]);
   const Arg q("q", o[1]), kc("k_cache", o[2]), vc("v_cache", o[3]), table("page_table", o[4]), len("kv_len", o[5]),
       q_start("q_start", o[6]), given("out", o[10]), prefix("prefix_pages", o[11]);
+  without_gradient({&q, &kc, &vc, &given});
   on_device(device, {&q, &kc, &vc, &table, &len, &q_start, &given, &prefix});
   nkb_paged_attention_args x = {};
   x.dtype = rows(q, 3);
@@ -248,6 +266,7 @@ PyObject *attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   x.workspace = room.get();
   x.workspace_bytes = (int64_t)need;
   issue(nkb_paged_attention, x, device);
+  if (given) written(out);
   if (given) return Py_NewRef(o[10]);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -260,6 +279,7 @@ PyObject *sample_tokens(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   const int64_t device = integer(o[0]);
   const Arg logits("logits", o[1]), u("u", o[2]), temperature("temperature", o[3]), top_k("top_k", o[4]), top_p("top_p", o[5]),
       min_p("min_p", o[6]), given("out", o[7]);
+  without_gradient({&logits, &u, &temperature, &top_p, &min_p});
   on_device(device, {&logits, &u, &temperature, &top_k, &top_p, &min_p, &given});
   nkb_sample_args x = {};
   x.dtype = rows(logits, 2);
@@ -283,6 +303,7 @@ PyObject *sample_tokens(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
   x.min_p = min_p.ptr<float>();
   x.tokens = static_cast<int32_t *>(out.data_ptr());
   issue(nkb_sample_tokens, x, device);
+  if (given) written(out);
   if (given) return Py_NewRef(o[7]);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

@@ -14,7 +14,9 @@ are int32; the new tokens lie in sequence order; ``kv_len`` counts a
 sequence's cached tokens with the new ones; ``q_start=None`` means one new
 token per sequence.  Lengths and tables are read on the device when the
 kernels run, nothing is synchronised, and every launch goes to the current
-torch stream, so a call can be captured into a CUDA graph.  A kernel whose
+torch stream, so a call can be captured into a CUDA graph.  The calls have no
+gradient: where autograd records, tensors that require one are refused, and
+tensors that are written in place count as changed.  A kernel whose
 bounded wait runs out ends without its results; ``check_device_error`` tells.
 """
 

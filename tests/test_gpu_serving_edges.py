@@ -350,3 +350,32 @@ def test_starts_that_go_back_after_a_prefix():
                               q_start=ints([500, 0, T]))
     no_device_error()
     assert bool(got.isfinite().all()) and bool((got[600:] == 0).all())
+
+
+# ---------------------------------------------------------------------------
+# autograd
+# ---------------------------------------------------------------------------
+def test_gradients_are_refused_and_writes_are_seen():
+    rng = np.random.default_rng(1700)
+    cache = Paged(rng, [20], 2, 64, 16, BF16, fill=1.0)
+    k, q, table, lens = randn(rng, (1, 2, 64), BF16), randn(rng, (1, 4, 64), BF16), cache.device_table(), ints([20])
+    with pytest.raises(RuntimeError, match="q: requires a gradient"):
+        nk.paged_attention(q.clone().requires_grad_(), cache.k, cache.v, table, lens)
+    with torch.no_grad():
+        nk.paged_attention(q.clone().requires_grad_(), cache.k, cache.v, table, lens)
+    w = torch.ones((), dtype=BF16, device="cuda", requires_grad=True)
+    loss = (w * cache.k).sum()  # keeps the cache for its backward pass
+    versions = [cache.k._version, cache.v._version, q._version]
+    nk.paged_append(k, k, cache.k, cache.v, table, lens, q=q, q_out=q)
+    assert [cache.k._version, cache.v._version, q._version] == [x + 1 for x in versions]
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    out, tokens = torch.empty_like(q), torch.empty(1, dtype=torch.int32, device="cuda")
+    nk.paged_attention(q, cache.k, cache.v, table, lens, out=out)
+    nk.sample_tokens(torch.zeros((1, 9), device="cuda"), torch.zeros(1, device="cuda"), out=tokens)
+    assert out._version == 1 and tokens._version == 1
+    with torch.inference_mode():
+        x = torch.empty_like(q)
+        nk.paged_attention(q, cache.k, cache.v, table, lens, out=x)
+    nk.paged_attention(q, cache.k, cache.v, table, lens, out=x)  # has no version to raise
+    assert torch.equal(x, out)

@@ -29,3 +29,28 @@ def test_append_of_no_tokens_with_queries():
     assert lib.nkb_paged_append(packed("append", **none, cos=16, sin=16, rot_dim=64, rope_rows=4, rope_stride=32), None) == 0
     assert lib.nkb_paged_append(packed("append", **{**none, "q_heads": -1}), None) == 1
     assert lib.nkb_paged_append(packed("append", q_heads=4), None) == 1
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    torch = pytest.importorskip("torch")
+    from nkipy_b200.runtime import serving
+
+    calls = serving._calls()
+    x, u = torch.zeros(2, 3), torch.zeros(2)
+    q, cache, table = torch.zeros(2, 2, 8), torch.zeros(1, 16, 2, 8), torch.zeros(2, 1, dtype=torch.int32)
+    cos = torch.zeros(4, 4)
+    sample = lambda *a: calls.sample_tokens(0, *a, None, None)  # noqa: E731
+    attend = lambda q, k, v: calls.attention(0, q, k, v, table, table[:, 0], None, 0, 0, None, None, None, 0)  # noqa: E731
+    append = lambda k, v, kc, q, cos: calls.paged_append(0, k, v, kc, kc, table, table[:, 0], None, q, cos, cos, 0, None)  # noqa: E731
+    for call, args, names in ((sample, [x, u, u, None, u], ["logits", "u", "temperature", "", "top_p"]),
+                              (attend, [q, cache, cache], ["q", "k_cache", "v_cache"]),
+                              (append, [q, q, cache, q, cos], ["k", "v", "k_cache", "q", "cos"])):
+        for i, name in enumerate(names):
+            if not name:
+                continue
+            given = list(args)
+            given[i] = given[i].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match=f"^{name}: requires a gradient"):
+                call(*given)
+            with torch.no_grad(), pytest.raises(ValueError, match="cuda:0"):  # then the device is looked at
+                call(*given)
