@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -62,6 +63,21 @@ void without_gradient(std::initializer_list<const Arg *> args) {
     if (*a && (*a)->requires_grad())
       fail(PyExc_RuntimeError, std::string(a->name) + ": requires a gradient, which this call does not have; call it under torch.no_grad(), or on detached tensors");
 }
+// What a call writes repeats no element, and covers no part of `others` (a given output may be its own input).
+void apart(const Arg &out, std::initializer_list<const Arg *> others) {
+  if (!out) return;
+  if (at::has_internal_overlap(*out) == at::MemOverlap::Yes) invalid(std::string(out.name) + ": written, but some of its elements are the same memory");
+  for (const Arg *a : others)
+    if (*a) {
+      const at::MemOverlapStatus s = at::get_overlap_status(*out, **a);
+      if (s == at::MemOverlapStatus::Partial || s == at::MemOverlapStatus::Full) invalid(c10::str(out.name, ": written, but shares memory with ", a->name));
+    }
+}
+void apart_or_same(const Arg &out, const Arg &in) {
+  if (out && in && at::get_overlap_status(*out, *in) == at::MemOverlapStatus::Partial)
+    invalid(c10::str(out.name, ": written, but shares a part of its memory with ", in.name));
+}
+
 // A tensor that a call has written into: autograd sees that it changed.
 void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -165,6 +181,10 @@ PyObject *paged_append(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
       q_start("q_start", o[7]), q("q", o[8]), cos("cos", o[9]), sin("sin", o[10]), q_out("q_out", o[12]);
   without_gradient({&k, &v, &kc, &vc, &q, &cos, &sin, &q_out});
   on_device(device, {&k, &v, &kc, &vc, &table, &len, &q_start, &q, &cos, &sin, &q_out});
+  apart(kc, {&vc, &k, &v});
+  apart(vc, {&k, &v});
+  apart(q_out, {&k, &v});
+  apart_or_same(q_out, q);
   nkb_paged_append_args x = {};
   x.dtype = rows(k, 3);
   x.tokens = k->size(0);
@@ -227,6 +247,8 @@ PyObject *attention(PyObject *, PyObject *const *o, Py_ssize_t nargs) {
       q_start("q_start", o[6]), given("out", o[10]), prefix("prefix_pages", o[11]);
   without_gradient({&q, &kc, &vc, &given});
   on_device(device, {&q, &kc, &vc, &table, &len, &q_start, &given, &prefix});
+  apart(given, {&kc, &vc});
+  apart_or_same(given, q);
   nkb_paged_attention_args x = {};
   x.dtype = rows(q, 3);
   x.tokens = q->size(0);

@@ -379,3 +379,37 @@ def test_gradients_are_refused_and_writes_are_seen():
         nk.paged_attention(q, cache.k, cache.v, table, lens, out=x)
     nk.paged_attention(q, cache.k, cache.v, table, lens, out=x)  # has no version to raise
     assert torch.equal(x, out)
+
+
+# ---------------------------------------------------------------------------
+# written tensors
+# ---------------------------------------------------------------------------
+def test_written_tensors_that_share_memory_are_refused():
+    """Repeated elements and overlaps would be written by several blocks at once; nothing is launched."""
+    zeros = lambda *s: torch.zeros(s, device="cuda", dtype=BF16)  # noqa: E731
+    table, lens = torch.zeros((4, 1), dtype=torch.int32, device="cuda"), ints([1] * 4)
+    qkv, both, room = zeros(4, 6, 8), zeros(3, 2, 16, 2, 8), zeros(9, 2, 8)
+    q, k, v = qkv[:, :2], qkv[:, 2:4].contiguous(), qkv[:, 4:].contiguous()
+    kc, vc = both[:, 0], both[:, 1]  # side by side
+    append = lambda k, v, kc, vc, q, out: nk.paged_append(k, v, kc, vc, table, lens, q=q, q_out=out)  # noqa: E731
+    attend = lambda q, kc, out: nk.paged_attention(q, kc, kc, table, lens, out=out)  # noqa: E731
+    for call, what in (
+        (lambda: append(k, v, kc[:1].expand(3, 16, 2, 8), vc, None, None), "k_cache: written"),
+        (lambda: append(k, v, kc, vc[:, :1].expand(3, 16, 2, 8), None, None), "v_cache: written"),
+        (lambda: append(k, v, both[0, :1], both[0, :1], None, None), "k_cache: .* v_cache"),
+        (lambda: append(k, v, kc, vc, q, q[:1].expand(4, 2, 8)), "q_out: written"),
+        (lambda: append(k, v, kc, vc, k, k), "q_out: .* shares memory with k"),
+        (lambda: append(k, v, kc, vc, room[:4], room[1:5]), "q_out: .* part of its memory with q"),
+        (lambda: append(room[:4], v, room[:4].view(1, 4, 2, 8), vc[:1, :4], None, None), "k_cache: .* k"),
+        (lambda: attend(q, kc, q[:, :1].expand(4, 2, 8)), "out: written"),
+        (lambda: attend(room[:4], kc, room[1:5]), "out: .* part of its memory with q"),
+    ):
+        with pytest.raises(ValueError, match=what):
+            call()
+    # what may share: an output that is its input, parts of one projection, keys and values of one allocation
+    table.copy_(torch.tensor([[0], [1], [2], [-1]], dtype=torch.int32))
+    append(qkv[:, 2:4], qkv[:, 4:], kc, vc, q, q)
+    append(k, v, kc, vc, room[:4], room[4:8])
+    attend(q, kc, q)
+    attend(room[:4], kc, room[:4])
+    no_device_error()
