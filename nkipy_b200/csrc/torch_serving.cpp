@@ -346,5 +346,8 @@ PyMODINIT_FUNC PyInit_nkb_torch() {
   if (!nkb) return nullptr;
   check_status = PyObject_GetAttrString(nkb, "check");
   Py_DECREF(nkb);
-  return check_status ? PyModule_Create(&module) : nullptr;
+  if (!check_status) return nullptr;
+  PyObject *m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", NKB_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
 }

@@ -53,7 +53,9 @@ def attention_workspace(sizes, tokens_by_start) -> int:
 @functools.lru_cache(maxsize=1)
 def _calls():
     """The module that takes torch tensors (csrc/torch_serving.cpp)."""
-    import torch  # noqa: F401  (its libraries)
+    import torch
+
+    from nkipy_b200.build import built_for
 
     _nkb.lib()
     path = os.path.join(os.path.dirname(_nkb.LIB_PATH), "nkb_torch.so")
@@ -62,6 +64,8 @@ def _calls():
     spec = importlib.util.spec_from_file_location("nkb_torch", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.built_for != built_for(torch.__version__, torch.version.git_version):
+        raise ImportError(f"{path} was built for {module.built_for}: run `python -m nkipy_b200.build`")
     return module
 
 

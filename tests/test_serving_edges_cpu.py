@@ -54,3 +54,63 @@ def test_tensors_that_require_a_gradient_are_refused():
                 call(*given)
             with torch.no_grad(), pytest.raises(ValueError, match="cuda:0"):  # then the device is looked at
                 call(*given)
+
+
+# ---------------------------------------------------------------------------
+# the build of the module behind the torch calls
+# ---------------------------------------------------------------------------
+@pytest.fixture
+def torch_build(tmp_path, monkeypatch):
+    """The builder with a torch package and an output folder of its own; compiler commands are counted, not run."""
+    from nkipy_b200 import build
+
+    package, out = tmp_path / "torch", tmp_path / "_lib"
+    (package / "lib").mkdir(parents=True)
+    (out / "obj").mkdir(parents=True)
+    (package / "lib" / "libc10_cuda.so").touch()
+    (package / "version.py").write_text("__version__ = '2.0.0'\ngit_version = 'abc'\n")
+    commands = []
+
+    def run(cmd, **kwargs):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return build.subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "OUT_DIR", str(out))
+    monkeypatch.setattr(build, "OBJ_DIR", str(out / "obj"))
+    monkeypatch.setattr(build, "TORCH_LIB", str(out / "nkb_torch.so"))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    found = type("Spec", (), {"submodule_search_locations": [str(package)]})
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: found)
+    return build, package, commands
+
+
+def test_module_is_built_again_for_another_torch(torch_build):
+    build, package, commands = torch_build
+    for _ in range(2):
+        build._build_torch(False)
+    assert len(commands) == 1
+    (package / "version.py").write_text("__version__ = '2.1.0'\ngit_version = 'abc'\n")
+    for _ in range(2):
+        build._build_torch(False)
+    assert len(commands) == 2
+
+
+def test_no_module_for_a_torch_without_cuda(torch_build, capsys):
+    build, package, commands = torch_build
+    (package / "lib" / "libc10_cuda.so").unlink()
+    build._build_torch(False)  # builds nothing and raises nothing
+    assert not commands and "no CUDA" in capsys.readouterr().err
+
+
+def test_module_of_another_torch_is_not_used(monkeypatch):
+    pytest.importorskip("torch")
+    from nkipy_b200.runtime import serving
+
+    serving._calls()
+    serving._calls.cache_clear()
+    monkeypatch.setattr("torch.version.git_version", "another")
+    with pytest.raises(ImportError, match="was built for torch"):
+        serving._calls()
+    monkeypatch.undo()
+    serving._calls()
