@@ -97,8 +97,8 @@ int check_sizes(const Args &a) {
     return fail(NKB_ERR_UNSUPPORTED, "paged_attention: q, out and caches must be float32, bfloat16 or float16");
   if (a.q_heads < 1 || a.q_heads % a.kv_heads || a.q_heads > 65535) return bad("q_heads must be a multiple of kv_heads");
   if (a.head_dim > MAX_D) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: head_dim above 256");
-  if (a.window < 0 || a.sinks < 0 || a.prefix_len < 0 || a.prefix_len > INT32_MAX)
-    return bad("window, sinks and prefix_len must not be negative");
+  if (a.window < 0 || a.sinks < 0 || a.prefix_len < 0) return bad("window, sinks and prefix_len must not be negative");
+  if (a.prefix_len > paged::MAX_POSITIONS) return bad("prefix of more than 2^31 - 256 positions");
   if (a.prefix_len && a.window) return fail(NKB_ERR_UNSUPPORTED, "paged_attention: a window over a shared prefix");
   if (!a.q_start && a.tokens != a.seqs) return bad("without q_start there is one token per sequence");
   return NKB_OK;

@@ -88,6 +88,9 @@ int step_args(const Step &s, void *const *ptrs, int n_ptrs, int n_ints, const ch
   return NKB_OK;
 }
 
+// Positions that a page table or a prefix may hold: rounded up to a block of keys they stay in 32 bits.
+constexpr int64_t MAX_POSITIONS = (int64_t(1) << 31) - 256;
+
 // What every call on a paged cache requires of its sizes (names for messages).
 inline int check_cache(const char *what, int64_t tokens, int64_t seqs, int64_t kv_heads, int64_t head_dim, int64_t pages,
                        int64_t page_size, int64_t width, int64_t table_stride) {
@@ -96,7 +99,7 @@ inline int check_cache(const char *what, int64_t tokens, int64_t seqs, int64_t k
   if (kv_heads < 1 || head_dim < 1 || kv_heads > 65535) return bad("kv_heads or head_dim out of range");
   if (pages < 0 || pages > INT32_MAX || page_size < 1 || page_size > INT32_MAX) return bad("pages or page_size out of range");
   if (width < 0 || table_stride < 0 || (seqs > 1 && table_stride < width)) return bad("page table rows overlap");
-  if (width * page_size > INT32_MAX) return bad("page table holds more than 2^31 - 1 positions");
+  if (width > MAX_POSITIONS / page_size) return bad("page table holds more than 2^31 - 256 positions");
   return NKB_OK;
 }
 

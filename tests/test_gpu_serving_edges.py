@@ -413,3 +413,31 @@ def test_written_tensors_that_share_memory_are_refused():
     attend(q, kc, q)
     attend(room[:4], kc, room[:4])
     no_device_error()
+
+
+# ---------------------------------------------------------------------------
+# the last positions
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("dtype, hq", [(BF16, 4), (F32, 2)])
+def test_positions_up_to_the_limit(n, dtype, hq):
+    """A page table of 2^31 - 256 positions, full: a window over the last ones, and the first tokens."""
+    page, d, N = 8, 64, 2**31 - 256
+    window, sinks, last = 60, 3, 20
+    rng = np.random.default_rng(1800)
+    table = torch.full((1, N // page), -1, dtype=torch.int32, device="cuda")
+    order = rng.permutation(last + 1)
+    table[0, 0], table[0, -last:] = int(order[0]), ints(order[1:])
+    kc, vc = (randn(rng, (last + 1, page, 1, d), dtype) for _ in range(2))
+    k, v, q = randn(rng, (n, 1, d), dtype), randn(rng, (n, 1, d), dtype), randn(rng, (n, hq, d), dtype)
+    start = None if n == 1 else ints([0, n])
+    nk.paged_append(k, v, kc, vc, table, ints([N]), q_start=start)
+    rows = lambda c: np.concatenate([f64(c[order[0]])[:sinks], f64(c[order[1:]]).reshape(-1, 1, d)])  # noqa: E731
+    assert np.array_equal(rows(kc)[-n:], f64(k)) and np.array_equal(rows(vc)[-n:], f64(v))
+    at = np.concatenate([np.arange(sinks), N - last * page + np.arange(last * page)])
+    pos = np.arange(N - n, N)[:, None]
+    seen = (at <= pos) & ((at > pos - window) | (at < sinks))
+    want, mag = attention_reference(f64(q), rows(kc), rows(vc), seen, 1 / math.sqrt(d), 1)
+    got = nk.paged_attention(q, kc, vc, table, ints([N]), q_start=start, window=window, sinks=sinks)
+    no_device_error()
+    check_attention(got, want, mag, dtype)

@@ -114,3 +114,19 @@ def test_module_of_another_torch_is_not_used(monkeypatch):
         serving._calls()
     monkeypatch.undo()
     serving._calls()
+
+
+# ---------------------------------------------------------------------------
+# positions
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kind, change", [
+    ("append", dict(page_size=1, table_width=2**31 - 1, table_stride=2**31 - 1)),
+    ("attention", dict(page_size=1, table_width=2**31 - 1, table_stride=2**31 - 1)),
+    ("attention", dict(page_size=2**31 - 255, table_width=1, table_stride=1)),
+    ("append", dict(table_width=1 << 60, table_stride=1 << 60)),  # times the page size it is a multiple of 2^64
+    ("attention", dict(prefix_len=2**31 - 255, prefix_pages=16)),
+])
+def test_positions_that_blocks_of_keys_could_not_count(kind, change):
+    entry = {"append": "nkb_paged_append", "attention": "nkb_paged_attention"}[kind]
+    assert getattr(_nkb.lib(), entry)(packed(kind, **change), None) == 1
+    assert "2^31 - 256 positions" in _nkb.lib().nkb_last_error().decode()
