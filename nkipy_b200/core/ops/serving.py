@@ -61,6 +61,9 @@ paged_append = Op("paged_append")
 def _paged_append_cpu(k, v, k_cache, v_cache, page_table, kv_len, q_start=None, q=None, cos=None, sin=None, pos_offset=0):
     _check_append(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, sin)
     pages, size = k_cache.shape[:2]
+    # rows that are read from the caches are those of before the call
+    k, v, q, cos, sin = (x.copy() if x is not None and any(np.may_share_memory(x, c) for c in (k_cache, v_cache)) else x
+                         for x in (k, v, q, cos, sin))
     out = None if q is None else np.zeros_like(q)
     for b, t, n, p in _spans(page_table, kv_len, q_start, k.shape[0]):
         pos = np.arange(p, p + n)
@@ -198,6 +201,8 @@ def _check_caches(k_cache, v_cache):
 
 def _check_append(k, v, k_cache, v_cache, page_table, kv_len, q_start, q, cos, sin):
     _check_caches(k_cache, v_cache)
+    if k_cache is v_cache:
+        _fail("k_cache and v_cache are one tensor")
     if len(k.shape) != 3 or tuple(k.shape) != tuple(v.shape) or k.dtype != v.dtype or not _floating(k.dtype):
         _fail(f"k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)}: expected two (tokens, kv_heads, head_dim)")
     if tuple(k.shape[1:]) != tuple(k_cache.shape[2:]):

@@ -1243,6 +1243,11 @@ class Lowering:
         for n in ("page_table", "kv_len", "q_start"):
             if n in t:
                 views[n] = self.materialize(self.get(t[n]), dense=True)
+        # what is read from the caches themselves (rows that move to other places) is copied before they are written
+        caches = [self.get(t[n]) for n in ("k_cache", "v_cache")]
+        for n, v in views.items():
+            if any(self._refs_buf(c, v.buf) for c in caches):
+                views[n] = self.materialize(v, out=self.tmp_view(v.shape, v.dtype))
         views["k_cache"] = self.mutable_base(t["k_cache"], op)
         views["v_cache"] = self.mutable_base(t["v_cache"], op)
         k, kc = views["k"], views["k_cache"]

@@ -13,8 +13,10 @@ torch = pytest.importorskip("torch")
 from nkipy_b200 import runtime as nk  # noqa: E402
 from nkipy_b200.spike import _nkb  # noqa: E402
 from tests.test_serving_cpu import packed  # noqa: E402
+from tests.test_serving_edges_cpu import move_inputs, move_rows  # noqa: E402
 from tests.test_gpu_serving import (BF16, F16, F32, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
                                     randn, run_attention, seen_by)
+from tests.utils import on_device  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -441,3 +443,15 @@ def test_positions_up_to_the_limit(n, dtype, hq):
     got = nk.paged_attention(q, kc, vc, table, ints([N]), q_start=start, window=window, sinks=sinks)
     no_device_error()
     check_attention(got, want, mag, dtype)
+
+
+# ---------------------------------------------------------------------------
+# kernel bodies
+# ---------------------------------------------------------------------------
+def test_rows_that_move_inside_the_caches():
+    args = move_inputs()
+    host = [a.copy() for a in args]
+    move_rows(*host)
+    on_device(move_rows, *args)
+    for got, want in zip(args[:2], host[:2]):
+        np.testing.assert_array_equal(got.view(np.uint16), want.view(np.uint16))

@@ -5,6 +5,7 @@ import pytest
 
 from nkipy_b200.core import tensor_apis as T
 from nkipy_b200.core.trace import NKIPyKernel
+from nkipy_b200.planner.lower import Lowering
 from nkipy_b200.spike import _nkb
 from tests.test_serving_cpu import packed, step_inputs
 
@@ -130,3 +131,50 @@ def test_positions_that_blocks_of_keys_could_not_count(kind, change):
     entry = {"append": "nkb_paged_append", "attention": "nkb_paged_attention"}[kind]
     assert getattr(_nkb.lib(), entry)(packed(kind, **change), None) == 1
     assert "2^31 - 256 positions" in _nkb.lib().nkb_last_error().decode()
+
+
+# ---------------------------------------------------------------------------
+# appends that read the caches
+# ---------------------------------------------------------------------------
+def move_rows(kc, vc, table, lens):
+    """The first rows of the caches' page 6 become the new tokens' rows, twice (the second time of the changed caches)."""
+    T.paged_append(kc[6, :3], vc[6, :3], kc, vc, table, lens)
+    T.paged_append(kc[6, 3:6], vc[6, 3:6], kc, vc, table, lens - 1)
+
+
+def move_inputs():
+    rng = np.random.default_rng(6)
+    kc, vc = (rng.standard_normal((8, 16, 2, 64)).astype(np.float16) for _ in range(2))
+    # page 6 itself is written: a row that is read by the first append, and one that is read by the second
+    return kc, vc, np.array([[6, 1], [6, 7], [3, 6]], np.int32), np.array([2, 5, 19], np.int32)
+
+
+def test_rows_that_move_inside_the_caches():
+    """The rows are those of before the append, although some of them are written by it."""
+    kc, vc, table, lens = move_inputs()
+    want = [c.copy() for c in (kc, vc)]
+    for c in want:
+        c[6, [1, 4, 2]] = c[6, :3].copy()
+        c[6, [0, 3, 1]] = c[6, 3:6].copy()
+    move_rows(kc, vc, table, lens)
+    assert all((a == b).all() for a, b in zip((kc, vc), want))
+
+
+def test_rows_that_move_inside_the_caches_are_copied_first():
+    kernel = NKIPyKernel.trace(move_rows)
+    kernel.specialize(*move_inputs())
+    plan = Lowering(kernel._code).run()
+    appends = [s for s in plan.steps if s.kernel == "paged_append"]
+    assert len(appends) == 2
+    same = {0, 1} | {b for s in appends for b, _ in s.bufs[2:4]}  # the caches' buffers, as inputs and as results
+    for s in appends:
+        assert not {b for b, _ in s.bufs[:2]} & same
+
+
+def test_one_cache_for_keys_and_values_is_refused():
+    kc, _, table, lens = move_inputs()
+    k = np.zeros((3, 2, 64), np.float16)
+    with pytest.raises(ValueError, match="one tensor"):
+        T.paged_append(k, k, kc, kc, table, lens)
+    with pytest.raises(ValueError, match="one tensor"):
+        NKIPyKernel.trace(lambda k, kc, t, n: T.paged_append(k, k, kc, kc, t, n)).specialize(k, kc, table, lens)
