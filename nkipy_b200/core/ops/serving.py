@@ -148,7 +148,8 @@ def _sample_tokens_cpu(logits, u, temperature=None, top_k=None, top_p=None, min_
             continue
         with np.errstate(all="ignore"):
             e = np.exp((x - top) * (np.float32(1) / t), dtype=np.float32)
-        e = np.where(x == top, np.float32(1), np.where(x == -np.inf, np.float32(0), e))
+        # (a finite logit below an infinite one, at an infinite temperature, has a quotient of NaN)
+        e = np.where(x == top, np.float32(1), np.where((x == -np.inf) | np.isnan(e), np.float32(0), e))
         w = (e.astype(np.float64) * 2.0**32).astype(np.int64)  # whole numbers: sums are exact
         order = np.argsort(-x, kind="stable")
         k, p = int(value(top_k, r, 0)), np.float32(value(top_p, r, 1.0))

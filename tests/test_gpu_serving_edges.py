@@ -455,3 +455,19 @@ def test_rows_that_move_inside_the_caches():
     on_device(move_rows, *args)
     for got, want in zip(args[:2], host[:2]):
         np.testing.assert_array_equal(got.view(np.uint16), want.view(np.uint16))
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("vocab", [6, 5000, 500001])
+def test_infinite_logits_at_any_temperature(vocab):
+    """Only the infinite logits have a weight, as at any other temperature; in a cluster and in one long row."""
+    x = torch.zeros((3, vocab), device="cuda")
+    x[:, 1], x[:, 3], x[:, 4], x[:, 5] = INF, INF, -INF, NAN
+    u, t = torch.tensor([0.2, 0.7, 0.7], device="cuda"), torch.tensor([1.0, 1e30, INF], device="cuda")
+    for k, p, m in ((None, None, None), (ints([4] * 3), None, None), (None, torch.full((3,), 0.9, device="cuda"), None),
+                    (None, None, torch.full((3,), 0.1, device="cuda")), (ints([1] * 3), None, None)):
+        want = [1, 1, 1] if k is not None and int(k[0]) == 1 else [1, 3, 3]
+        assert nk.sample_tokens(x, u, t, k, p, m).tolist() == want
+    assert nk.sample_tokens(x, u, torch.zeros(3, device="cuda")).tolist() == [1, 1, 1]

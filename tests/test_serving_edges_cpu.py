@@ -178,3 +178,13 @@ def test_one_cache_for_keys_and_values_is_refused():
         T.paged_append(k, k, kc, kc, table, lens)
     with pytest.raises(ValueError, match="one tensor"):
         NKIPyKernel.trace(lambda k, kc, t, n: T.paged_append(k, k, kc, kc, t, n)).specialize(k, kc, table, lens)
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+def test_infinite_logits_at_an_infinite_temperature():
+    """Only the infinite logits have a weight, as at any other temperature."""
+    x = np.array([[0.0, np.inf, 1.0, np.inf, -np.inf, np.nan]] * 2, np.float32)
+    for t in (1.0, 1e30, np.inf):
+        assert T.sample_tokens(x, np.array([0.2, 0.7], np.float32), np.full(2, t, np.float32)).tolist() == [1, 3]
