@@ -11,8 +11,10 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from nkipy_b200 import runtime as nk  # noqa: E402
+from nkipy_b200 import workloads as W  # noqa: E402
+from nkipy_b200.core import tensor_apis as T  # noqa: E402
 from nkipy_b200.spike import _nkb  # noqa: E402
-from tests.test_serving_cpu import packed  # noqa: E402
+from tests.test_serving_cpu import packed, step_inputs  # noqa: E402
 from tests.test_serving_edges_cpu import move_inputs, move_rows  # noqa: E402
 from tests.test_gpu_serving import (BF16, F16, F32, Paged, attention_reference, check_attention, f64, ints,  # noqa: E402
                                     randn, run_attention, seen_by)
@@ -471,3 +473,111 @@ def test_infinite_logits_at_any_temperature(vocab):
         want = [1, 1, 1] if k is not None and int(k[0]) == 1 else [1, 3, 3]
         assert nk.sample_tokens(x, u, t, k, p, m).tolist() == want
     assert nk.sample_tokens(x, u, torch.zeros(3, device="cuda")).tolist() == [1, 1, 1]
+
+
+def rows64(args, n_heads, n_kv_heads, q_start=None, last=None, prefix_pages=None, prefix_len=0, window=0, sinks=0, eps=1e-6):
+    """Where ``workloads.paged_step_kernel`` writes, and the keys, values and queries in 64 bits, each with a bound: with
+    u = 2^-8 for a value rounded to bf16, the normalised rows and the projection's result are rounded once each (2 u of
+    the terms' magnitudes), rotated rows once more."""
+    u = 2.0**-8
+    x, norm, w = (np.asarray(a).astype(np.float64) for a in args[:3])
+    table, kv_len, cos, sin = args[7], args[8], args[9].astype(np.float64), args[10].astype(np.float64)
+    page, d = args[5].shape[1], args[5].shape[3]
+    starts = np.arange(len(kv_len) + 1) if q_start is None else q_start
+    h = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * norm
+    split = lambda a: [p.reshape(len(x), -1, d) for p in np.split(a, [n_heads * d, (n_heads + n_kv_heads) * d], -1)]  # noqa: E731
+    (q, k, v), (mq, mk, mv) = split(h @ w), split(abs(h) @ abs(w))
+    pos = np.concatenate([np.arange(n - (e - s), n) for s, e, n in zip(starts, starts[1:], kv_len)])
+    seq = np.repeat(np.arange(len(kv_len)), np.diff(starts))
+    c, s = cos[pos + prefix_len][:, None], sin[pos + prefix_len][:, None]
+
+    def turned(a, m):
+        (lo, hi), (ml, mh) = np.split(a, 2, -1), np.split(m, 2, -1)
+        return (np.concatenate([lo * c - hi * s, lo * s + hi * c], -1),
+                3 * u * np.concatenate([ml * abs(c) + mh * abs(s), ml * abs(s) + mh * abs(c)], -1))
+
+    return seq, pos, (table[seq, pos // page], pos % page), turned(k, mk), (v, 2 * u * mv), turned(q, mq)
+
+
+def step_parts(x, norm_weight, qkv_weight, o_weight, head_weight, cache_k, cache_v, page_table, kv_len, cos, sin, u, temperature,
+               top_k, top_p, min_p, q_start=None, last=None, prefix_pages=None, prefix_len=0, n_heads=4, n_kv_heads=2, window=0,
+               sinks=0, eps=1e-6):
+    """``workloads.paged_step_kernel`` with what lies between its calls: queries, attention, logits and tokens."""
+    tokens, d = x.shape[0], cache_k.shape[3]
+    h = W.qk_rmsnorm(x, norm_weight, eps)
+    q, k, v = np.split((h @ qkv_weight).astype(x.dtype), [n_heads * d, (n_heads + n_kv_heads) * d], axis=-1)
+    q, k, v = q.reshape(tokens, n_heads, d), k.reshape(tokens, n_kv_heads, d), v.reshape(tokens, n_kv_heads, d)
+    q = T.paged_append(k, v, cache_k, cache_v, page_table, kv_len, q_start=q_start, q=q, cos=cos, sin=sin, pos_offset=prefix_len)
+    if prefix_len:
+        attn = T.prefix_attention(q, cache_k, cache_v, prefix_pages, prefix_len, page_table, kv_len, q_start=q_start)
+    else:
+        attn = T.paged_attention(q, cache_k, cache_v, page_table, kv_len, q_start=q_start, window=window, sinks=sinks)
+    y = x + attn.reshape(tokens, n_heads * d) @ o_weight
+    if last is not None:
+        y = np.take(y, last, axis=0)
+    logits = (y @ head_weight).astype(x.dtype)
+    return q, attn, logits, T.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+
+
+STEPS = [(None, (1, 20, 64)), ((3, 1, 20), (30, 20, 64)), ((64, 2, 9), (64, 40, 9))]
+
+
+def step_case(form, news, lens, seed):
+    args, kwargs = step_inputs(seed=seed, news=news, lens=lens, prefix=37 if form == "prefix" else 0)
+    if form == "window":
+        kwargs.update(window=16, sinks=2)
+    args = list(args)
+    args[12] = np.zeros(3, np.float32)  # greedy
+    return args, kwargs
+
+
+def check_written(args, old, where, keys, values):
+    """Of the caches the new rows alone have changed, each within its bound."""
+    for cache, before, (want, err) in zip(args[5:7], old, (keys, values)):
+        assert np.all(abs(cache[where].astype(np.float64) - want) <= err)
+        after = cache.copy()
+        after[where] = before[where]
+        np.testing.assert_array_equal(after.view(np.uint16), before.view(np.uint16))
+
+
+@pytest.mark.parametrize("news, lens", STEPS)
+@pytest.mark.parametrize("form", ["all", "window", "prefix"])
+def test_rows_of_a_step(form, news, lens):
+    args, kwargs = step_case(form, news, lens, 8)
+    old = [args[i].copy() for i in (5, 6)]
+    _, _, where, keys, values, _ = rows64(args, **kwargs)
+    tokens = np.asarray(on_device(W.paged_step_kernel, *args, **kwargs))
+    check_written(args, old, where, keys, values)
+    assert tokens.shape == (3,) and tokens.min() >= 0 and tokens.max() < args[4].shape[1]
+
+
+@pytest.mark.parametrize("news, lens", STEPS)
+@pytest.mark.parametrize("form", ["all", "window", "prefix"])
+def test_parts_of_a_step(form, news, lens):
+    """Each call of a step against 64 bits, on what the calls before it gave; the tokens are the logits' largest."""
+    args, kwargs = step_case(form, news, lens, 9)
+    old = [args[i].copy() for i in (5, 6)]
+    seq, pos, where, keys, values, (want, err) = rows64(args, **kwargs)
+    q, attn, logits, tokens = (np.asarray(a) for a in on_device(step_parts, *args, **kwargs))
+    check_written(args, old, where, keys, values)
+    q, attn, logits = (a.astype(np.float64) for a in (q, attn, logits))
+    assert np.all(abs(q - want) <= err)
+    u, (kc, vc), table = 2.0**-8, (a.astype(np.float64) for a in args[5:7]), args[7]
+    page, hkv, d = kc.shape[1:]
+    before = np.arange(kwargs.get("prefix_len", 0))
+    for t, (b, p) in enumerate(zip(seq, pos)):
+        at = np.arange(p + 1)
+        pages, slots = table[b, at // page], at % page
+        seen = seen_by(np.array([p]), p + 1, kwargs.get("window", 0), kwargs.get("sinks", 0))
+        if len(before):
+            pages, slots = np.concatenate([kwargs["prefix_pages"][before // page], pages]), np.concatenate([before % page, slots])
+            seen = np.concatenate([np.ones((1, len(before)), bool), seen], 1)
+        want, mag = attention_reference(q[t : t + 1], kc[pages, slots], vc[pages, slots], seen, 1 / math.sqrt(d), hkv)
+        assert np.all(abs(attn[t] - want[0]) <= u * (mag[0] + abs(want[0])) + 2.0**-16 * mag[0])
+    x, wo, head = (np.asarray(args[i]).astype(np.float64) for i in (0, 3, 4))
+    a = attn.reshape(len(x), -1)
+    y, dy = x + a @ wo, 2 * u * (abs(x) + abs(a) @ abs(wo))  # the product and the sum, rounded once each
+    if "last" in kwargs:
+        y, dy = y[kwargs["last"]], dy[kwargs["last"]]
+    assert np.all(abs(logits - y @ head) <= dy @ abs(head) + u * abs(y) @ abs(head))
+    np.testing.assert_array_equal(tokens, logits.argmax(1))
