@@ -121,10 +121,16 @@ int prefix_run(const Args &a, cudaStream_t st, int device) {
   single::Params s = {};
   tile_params(a, device, a.workspace, own, true, true, &p);
   // Where the sequences' own keys have a kernel of their own, it begins on the SMs
-  // that the prefix leaves it, and fewer CTAs write fewer partials: 64 sequences after
-  // 8192 tokens take 47 us with the prefix on all SMs, 44 on two thirds, 46 on half,
-  // 128 after 2000 40, 38 and 38.
-  if (!own) p.max_ctas = max(1, p.max_ctas * 2 / 3);
+  // that a short prefix leaves it: two thirds for the prefix, and fewer partials.  A
+  // long prefix is then what takes the time, and gets all SMs.  32 / 8 heads of 128
+  // bf16, us with two thirds and with all, for 50, 400 and 2000 own keys: 64 after
+  // 2000 (1 block per CTA) 28, 43, 108 and 29, 46, 112; 64 after 8192 (3.5) 35, 54,
+  // 128 and 34, 56, 124; 128 after 8192 (7) 54, 88, 213 and 51, 88, 218; 256 after 8192
+  // (14) 99, 155, 400 and 92, 145, 409; 128 after 32768 (28) 118, 146, 264 and 97, 128, 260.
+  if (!own) {
+    const int64_t per = 2 * p.P, units = (a.tokens + per - 1) / per * a.kv_heads;
+    if (units * ((a.prefix_len + several::BN - 1) / several::BN) <= 8 * (int64_t)p.max_ctas) p.max_ctas = max(1, p.max_ctas * 2 / 3);
+  }
   decode_params(a, device, static_cast<char *>(a.workspace) + up(tile_workspace(a, device, own, true, true)), true, &s);
   if (int e = tile_launch(p, st, device)) return e;
   if (!own)

@@ -49,7 +49,7 @@ def test_a_wait_that_runs_out_is_reported():
 # ---------------------------------------------------------------------------
 # tokens without keys
 # ---------------------------------------------------------------------------
-def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=0, scale=None):
+def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=0, scale=None, single=False):
     """``front`` and ``behind`` tokens belong to no sequence; a sequence's length may be less than
     its new tokens, whose first ones then lie before its first key."""
     rng = np.random.default_rng(seed)
@@ -73,7 +73,7 @@ def run_padded(seed, front, news, lens, behind, hq, hkv, d, page, dtype, prefix=
             want[at : at + n], mag[at : at + n] = attention_reference(f64(q[at : at + n]), k, v, seen,
                                                                           1 / math.sqrt(d) if scale is None else scale, hkv)
         at += n
-    start = ints((front + np.cumsum([0] + list(news))).tolist())
+    start = None if single else ints((front + np.cumsum([0] + list(news))).tolist())
     args = (cache.device_table(), ints(lens))
     out = torch.full_like(q, 9.0)
     for _ in range(3):
@@ -111,6 +111,12 @@ def test_padding(case):
 @pytest.mark.parametrize("case", range(len(PADDED)))
 def test_padding_after_a_prefix(case, prefix):
     run_padded(800 + case, *PADDED[case], prefix=prefix)
+
+
+@pytest.mark.parametrize("prefix", [700, 6000])
+def test_single_tokens_after_a_prefix(prefix):
+    """A short prefix shares the SMs with the sequences' own keys, a long one takes all."""
+    run_padded(900, 0, [1] * 130, [0, 1, 70, 5, 300] * 26, 0, 64, 4, 64, 16, BF16, prefix=prefix, single=True)
 
 
 # ---------------------------------------------------------------------------
