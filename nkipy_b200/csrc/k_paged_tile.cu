@@ -646,12 +646,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mx4[i] = max3(mx4[i], __uint_as_float(v[e + 2 * i]), __uint_as_float(v[e + 2 * i + 1]));
-        // a score that is NaN or +inf makes the maximum NaN, and so all of the row: the polynomials would take it for 2^-126
-        float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * p.scale_log2;
-        mx = mx == INFINITY ? CUDART_NAN_F : mx;
+        const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * p.scale_log2;
         const bool raise = !(mx <= m + RESCALE);
-        if (__any_sync(0xffffffffu, raise)) {
-          const float m_new = raise ? mx : m;
+        bool exact = masked;  // zeros have to be zeros: masked scores, and rows whose scores are all -inf
+        if (__any_sync(0xffffffffu, raise || (!masked && mx == -INFINITY))) {
+          // a score of NaN or +inf makes the maximum NaN, and so all of the row: the polynomials would take it for 2^-126
+          const float m_new = raise ? (mx == INFINITY ? CUDART_NAN_F : mx) : m;
           const float alpha = m == -INFINITY ? 0.f : raise ? ex2(m - m_new) : 1.f;
           // (rows that have seen no key so far have O = 0 already)
           if (h > 0 && __any_sync(0xffffffffu, raise && m > -INFINITY)) {
@@ -669,6 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           l *= alpha;
           m = m_new;
+          exact |= __any_sync(0xffffffffu, m == -INFINITY) != 0;
         }
         const float mm = base_of(m);
         const uint64_t base2 = pair2(-mm, -mm);
@@ -690,8 +691,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             v[e / 2] = pack<T>(e0, e1);
           }
         };
-        // masked scores, and rows whose scores are all -inf, have to become zeros exactly
-        if (masked || __any_sync(0xffffffffu, m == -INFINITY)) exps(std::false_type{});
+        if (exact) exps(std::false_type{});
         else exps(std::true_type{});
         tmem_st16(sc, v);
         tmem_st16(sc + 16, v + 16);
