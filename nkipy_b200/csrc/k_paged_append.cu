@@ -4,7 +4,7 @@
 // for the two halves (lo, hi) of the first rot_dim dimensions at position p,
 // in fp32, rounded once to the stored type.  Each row is read and written once, so
 // the bound is HBM.  Measured (GPU time): 8192 tokens of 32 + 2 * 8 rows of 128 bf16,
-// 202 MB, 40.3 us or 5.0 TB/s, where a plain copy would take 31 us; 1500 tokens of
+// 202 MB, 40.4 us or 5.0 TB/s, where a plain copy would take 31 us; 1500 tokens of
 // 12 + 2 * 4 rows of 64 fp16 4.4 us, 8 tokens 2.2 us, which is the launch.
 #include <algorithm>
 

@@ -8,9 +8,9 @@
 // both leave partials (max, sum, unnormalised output) that the kernel here
 // joins per token and head.  Measured (32 / 8 heads of 128 bf16, GPU time): 64
 // sequences with some hundred keys each after a prefix of 8192, 44 us (the floor is
-// 14 us of reads; prefix 22, own keys 19 and join 12 us one by one, each in part
-// under the next: few blocks per CTA, so each is mostly its start and its partials);
-// 4 sequences after a prefix of 1000, 15.5 us.
+// 14 us of reads; prefix 29 on two thirds of the SMs, own keys 21 and join 12 us one by
+// one with cold caches, each in part under the next: few blocks per CTA, so each is
+// mostly its start and its partials); 4 sequences after a prefix of 1000, 15.7 us.
 #include "paged_attn.cuh"
 
 namespace nkb {

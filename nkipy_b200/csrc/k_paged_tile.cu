@@ -33,11 +33,12 @@
 //
 // What bounds it is the softmax between the two products: the exponentials take as
 // many cycles as the products at head dimension 128 and twice as many at 64, so
-// 3/8 of them are polynomials on the FMA pipe.  Measured (GPU time): 4 prompts of
-// 2048 tokens, window 1024, 32 / 8 heads of 128 bf16, 134 us or 773 TFLOP/s of the
-// keys seen (tensor pipe busy 44 %, issue slots 44 %); 500 tokens over 16400 keys,
-// 32 / 4 heads of 64 fp16, 132 us with 14 of them in the join, 501 TFLOP/s (tensor
-// 30 %, exponential unit 38 %, issue 52 %).
+// 3/8 of them are polynomials on the FMA pipe.  Measured (replays of a graph of 30
+// calls, then one call after another on changing inputs): 4 prompts of 2048 tokens,
+// window 1024, 32 / 8 heads of 128 bf16, 135 and 154 us, 766 and 671 TFLOP/s of the
+// keys seen (tensor pipe busy 41 %, issue slots 41 %); 500 tokens over 16400 keys,
+// 32 / 4 heads of 64 fp16, 129 and 132 us with 15 of them in the join, 511 and 500
+// TFLOP/s (tensor 25 %, issue 44 %).
 #include <math_constants.h>
 
 #include "paged_attn.cuh"
@@ -290,7 +291,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^y for two values on the FMA pipe: y = n + r with |r| <= 1/2, 2^r by its
 // minimax polynomial (least squares reweighted to an even relative error: 7.5e-5
 // for degree 3, 2.7e-6 for degree 4, a tenth of the rounding of P to bf16 and to
-// fp16), n added to the exponent.  y below -126 gives 2^-126.
+// fp16), n added to the exponent.  y below -126 gives 2^-126.  P is rounded because the
+// matrix product takes both operands in one type; the sums keep fp32 terms.  Outputs
+// are 0.0021 (bf16) and 0.00029 (fp16) from 64-bit values in the root mean square, where
+// fp32 probabilities and exact exponentials give 0.0016 and 0.00021.
 template <class T>
 __device__ __forceinline__ void exp2_poly(uint64_t y2, float &e0, float &e1) {
   constexpr bool fine = std::is_same<T, __half>::value;

@@ -9,10 +9,12 @@
 // kept set is "rank word >= threshold", with e >= min_p.
 //
 // A cluster of up to 8 CTAs holds a row in its shared memory: the logits are read
-// from memory once.  What bounds the kernel is then the instructions per element and
-// the cluster's meetings (about a microsecond each), so each way of filtering has
-// the fewest it can (GPU times for 1 row of 32000 fp32, and 128 rows of 151936 bf16,
-// whose 39 MB a copy reads in 6 us):
+// from memory once.  What bounds the kernel is then waiting: shared memory lets two CTAs
+// of 8 warps on an SM, which issue in 24 % of the cycles (128 mixed rows), through
+// the cluster's meetings (about a microsecond each), shared memory's latency and short
+// serial steps; 128 rows of 4 CTAs are 1.7 waves besides.  So each way of filtering has
+// the fewest meetings it can (GPU times for 1 row of 32000 fp32, and 128 rows of 151936
+// bf16, whose 39 MB a copy reads in 6 us):
 //   greedy  the CTAs' maxima: one meeting; 3 and 16 us
 //   top-k   of up to FAST_K: the CTAs' largest thread maxima bound the row's k-th
 //           largest element; what passes (two to three k elements) goes to one CTA,
