@@ -95,7 +95,7 @@ int64_t code_of(const Arg &a) {
 int64_t rows(const Arg &a, int64_t ndim) {
   const int64_t code = code_of(a);
   if (a->dim() != ndim) invalid(c10::str(a.name, ": expected ", ndim, " axes, got shape ", a->sizes()));
-  if (a->stride(-1) != 1 && a->size(-1) > 1) invalid(std::string(a.name) + ": the last axis must be contiguous");
+  if (a->stride(-1) != 1 && a->size(-1) > 1 && a->numel()) invalid(std::string(a.name) + ": the last axis must be contiguous");
   return code;
 }
 // a contiguous vector of `length` elements (-1: any number)
@@ -126,7 +126,7 @@ int64_t cache_and_batch(Args &x, const Arg &k, const Arg &v, const Arg &table, c
   x.seqs = table->size(0);
   x.table_width = table->size(1);
   x.table_stride = table->stride(0);
-  if (table->stride(1) != 1 && x.table_width > 1) invalid("page_table: the last axis must be contiguous");
+  if (table->stride(1) != 1 && x.table_width > 1 && x.seqs) invalid("page_table: the last axis must be contiguous");
   vector(kv_len, at::kInt, x.seqs);
   if (q_start)
     vector(q_start, at::kInt, x.seqs + 1);

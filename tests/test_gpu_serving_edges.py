@@ -201,6 +201,20 @@ def test_append_of_no_tokens_with_queries():
     assert bool((cache.k == 3).all())
 
 
+def test_calls_without_tokens_at_any_strides():
+    """An array without elements has no layout."""
+    cache = Paged(np.random.default_rng(1101), [20], 2, 64, 16, BF16)
+    table, start = cache.device_table(), ints([0, 0])
+    for make in (lambda *s: torch.empty_strided(s, (0,) * len(s), dtype=BF16, device="cuda"),
+                 lambda *s: torch.tensor(np.zeros(s)).to(BF16).cuda()):
+        got = nk.paged_append(make(0, 2, 64), make(0, 2, 64), cache.k, cache.v, table, ints([20]), q_start=start, q=make(0, 4, 64))
+        assert got.shape == (0, 4, 64)
+        assert nk.paged_attention(make(0, 4, 64), cache.k, cache.v, table, ints([20]), q_start=start).shape == (0, 4, 64)
+        none = torch.empty_strided((0, 3), (0, 0), dtype=torch.int32, device="cuda")
+        assert nk.paged_attention(make(0, 4, 64), cache.k, cache.v, none, ints([])).shape == (0, 4, 64)
+        assert nk.sample_tokens(make(0, 9), torch.zeros(0, device="cuda")).shape == (0,)
+
+
 # ---------------------------------------------------------------------------
 # NaN and infinities in what a token sees
 # ---------------------------------------------------------------------------
